@@ -24,6 +24,7 @@
 #include <stdint.h>
 
 #include "lum_llir.h"
+#include "lum_tree.h"   /* operators of speculative decoding */
 
 #ifdef __cplusplus
 extern "C" {

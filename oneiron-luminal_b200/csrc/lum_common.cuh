@@ -33,6 +33,8 @@ enum : uint32_t {
     LUM_ST_WAIT_GRID = 1u << 5,   // a grid-wide barrier of the persistent kernel was not reached by every CTA in time
     LUM_ST_WAIT_TMEM = 1u << 6,   // a wait on the tensor-core hand-over (accumulators ready / drained) ran out of budget
     LUM_ST_WAIT_PEER = 1u << 7,   // tensor parallel: another rank's partial vector did not arrive in time
+    LUM_ST_BAD_TREE = 1u << 8,    // drafted tokens: a parent that is no earlier node, or accepted nodes that are no path
+    LUM_ST_BAD_PAGE = 1u << 9,    // drafted tokens: a cache row, or the page that should hold it, outside the cache
 };
 
 // Budget for any single wait, in SM clock cycles (about two seconds at 2 GHz).  The SM-local cycle

@@ -55,6 +55,7 @@ size_t lum_generic_launches(const lum_generic_plan* p);
 size_t lum_generic_nodes(const lum_generic_plan* p);
 cudaError_t lum_generic_to_f32(const void* src, uint32_t dtype, size_t n, float* dst, cudaStream_t st);
 uint32_t* lum_static_sample_status();   // csrc/lum_gemv.cu
+uint32_t* lum_tree_status_word();       // csrc/lum_tree.cu
 
 namespace {
 
@@ -3438,7 +3439,7 @@ int32_t lum_op_status(void* stream) {
     if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) { g_create_error = "op_status: cannot query the current device"; return LUM_E_CUDA; }
     cudaError_t e = cudaStreamSynchronize((cudaStream_t)stream);
     if (e != cudaSuccess) return op_fail("op_status", e);
-    uint32_t* words[3] = {g_op_words[dev], g_sample_scratch[dev].status, lum_static_sample_status()};
+    uint32_t* words[4] = {g_op_words[dev], g_sample_scratch[dev].status, lum_static_sample_status(), lum_tree_status_word()};
     uint32_t seen = 0;
     for (uint32_t* w : words) {
         if (!w) continue;
@@ -3448,8 +3449,9 @@ int32_t lum_op_status(void* stream) {
         if (v) { seen |= v; cudaMemset(w, 0, 4); }
     }
     if (seen) {
-        char buf[96];
-        snprintf(buf, sizeof buf, "a stand-alone operator reported device status 0x%x (a bounded wait ran out)", seen);
+        char buf[160];
+        const char* why = seen & LUM_ST_BAD_TREE ? "drafted tokens that are no tree, or no path through one" : seen & (LUM_ST_BAD_PAGE | LUM_ST_BAD_POS) ? "a sequence, cache row or page outside what the call named" : "a bounded wait ran out";
+        snprintf(buf, sizeof buf, "a stand-alone operator reported device status 0x%x (%s)", seen, why);
         g_create_error = buf;
         return LUM_E_DEVICE;
     }

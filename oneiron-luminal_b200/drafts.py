@@ -1,0 +1,239 @@
+"""Operators of speculative decoding on torch tensors: thin calls of ``include/lum_tree.h``.
+
+A step verifies, for every sequence of a batch, a tree of drafted tokens: node 0 is the token decoding stands at, the others are guesses of what
+follows their parent.  Node ``i``'s key and value lie at cache row ``prefix + i``.
+
+    tree = DraftTree(row_start, prefix, parent, max_rows=64, max_prefix=4096)
+    cache = KvMap(rows=k.shape[0], page_table=table, page_rows=64, max_seq=4160)
+    out = attn_tree(q, k, v, tree, cache, n_kv_heads=8, head_dim=128)           # per layer
+    path, n_accepted, next_token = tree_accept(tree, tokens, logits=logits)     # the nodes that stand, and what follows them
+    kv_compact(planes, cache, tree, path, n_accepted)                           # their rows close up, in every layer
+
+All calls are asynchronous on the current stream of the tensors' device and can be captured into a CUDA graph.  A call that cannot be made
+raises :class:`LumError`; what the kernels find wrong in the arrays (a parent that is no earlier node, a page outside the pool, ...) is left out
+and raised by the next :func:`status`.
+"""
+from __future__ import annotations
+
+import ctypes as C
+
+from .runtime import DraftTreeDesc, KvMapDesc, LumError, TreeAttnDesc, load_library
+
+MAX_NODES = 256
+_F32, _BF16 = 0, 2
+_INVALID = -1
+
+
+def _torch():
+    import torch       # the package itself does not need it
+    return torch
+
+
+def _bad(why: str):
+    raise LumError(_INVALID, why)
+
+
+def _ints(name, t, device, dims=1, optional=False):
+    """Address of a contiguous int32 tensor on ``device``."""
+    if t is None and optional:
+        return None
+    torch = _torch()
+    if not isinstance(t, torch.Tensor) or t.dtype != torch.int32 or t.dim() != dims or not t.is_contiguous() or t.device != device or not t.is_cuda:
+        _bad(f"{name}: a contiguous {dims}-d int32 tensor on {device} is wanted")
+    return t.data_ptr()
+
+
+def _check(rc: int) -> None:
+    if rc:
+        raise LumError(rc, load_library().lum_last_error(None).decode())
+
+
+class _On:
+    """Makes the tensors' device the current one for a call and hands out its current stream."""
+
+    __slots__ = ("index", "before")
+
+    def __init__(self, device):
+        self.index = device.index
+
+    def __enter__(self):
+        cuda = _torch().cuda
+        self.before = cuda.current_device()
+        if self.before != self.index:
+            cuda.set_device(self.index)
+        return cuda.current_stream().cuda_stream
+
+    def __exit__(self, *exc):
+        if self.before != self.index:
+            _torch().cuda.set_device(self.before)
+
+
+class DraftTree:
+    """The trees of a batch.  ``row_start`` [n_seq + 1], ``prefix`` [n_seq] and ``parent`` [rows of the batch] are int32 tensors on the GPU; ``slot`` [n_seq] names
+    the cache slots (None: sequence s is slot s); no tree has more than ``max_rows`` nodes, no sequence more than ``max_prefix`` cached rows before it."""
+
+    def __init__(self, row_start, prefix, parent, *, max_rows: int, max_prefix: int, slot=None):
+        device = getattr(parent, "device", None)
+        n_seq = prefix.numel()
+        self.device, self.tensors = device, (row_start, prefix, parent, slot)
+        self.desc = DraftTreeDesc(_ints("row_start", row_start, device), _ints("prefix", prefix, device), _ints("parent", parent, device),
+                                  _ints("slot", slot, device, optional=True), n_seq, parent.numel(), max_rows, max_prefix)
+        if row_start.numel() != n_seq + 1 or (slot is not None and slot.numel() != n_seq):
+            _bad(f"row_start has {row_start.numel()} entries, slot {n_seq if slot is None else slot.numel()}, for {n_seq} sequences")
+
+
+class KvMap:
+    """Where the cached rows of a slot are: ``rows`` in all, contiguous slots of ``max_seq`` rows, or pages of ``page_rows`` rows named by ``page_table``
+    [slots, pages per slot]."""
+
+    def __init__(self, rows: int, *, max_seq: int, page_table=None, page_rows: int = 0, slots: int = 0):
+        self.tensors, self.rows = (page_table,), rows
+        if (page_table is None) != (page_rows == 0):
+            _bad("pages come with a page table")
+        if page_table is None:
+            self.desc = KvMapDesc(None, rows, slots or max(1, rows // max(1, max_seq)), max_seq, 0, 0)
+        else:
+            self.desc = KvMapDesc(_ints("page_table", page_table, page_table.device, dims=2), rows, page_table.shape[0], max_seq, page_rows, page_table.shape[1])
+
+
+def _rows_of(name, t, device, width, rows):
+    """(address, row stride) of a tensor whose rows are ``width`` elements, dense in a row."""
+    if t.device != device or t.dim() < 2 or t.shape[0] != rows:
+        _bad(f"{name}: {rows} rows on {device} are wanted, got {tuple(t.shape)} on {t.device}")
+    inner = 1
+    for size, stride in zip(reversed(t.shape[1:]), reversed(t.stride()[1:])):
+        if size != 1 and stride != inner:
+            _bad(f"{name}: the elements of a row must follow each other")
+        inner *= size
+    if inner != width:
+        _bad(f"{name}: rows of {width} elements are wanted, got {tuple(t.shape[1:])}")
+    return t.data_ptr(), (t.stride(0) if rows > 1 else width)
+
+
+def attn_tree(q, k, v, tree: DraftTree, cache: KvMap, *, n_kv_heads: int, head_dim: int, scale: float = 0.0, window: int = 0, sinks=None, out=None, workspace=None):
+    """Attention of the drafted nodes over their sequences' cached rows and their own ancestors.
+
+    ``q`` [rows, heads * head_dim] (or [rows, heads, head_dim]) in bf16 or f32; ``k`` and ``v`` [cache rows, n_kv_heads * head_dim] in bf16, or in f32 with f32
+    queries; rows may be strided.  ``scale`` 0: 1 / sqrt(head_dim).  ``window``: a node sees only what is fewer than so many places before its own.  ``sinks``
+    [heads] f32: a logit per head that joins the softmax's denominator.  Returns ``out`` (like q; rows of no sequence are left as they were; without ``out``
+    given they are not set).  ``workspace``: scratch to use, a uint8 tensor of at least :func:`attn_tree_workspace` bytes (None: taken from torch)."""
+    torch = _torch()
+    device, types = q.device, {torch.float32: _F32, torch.bfloat16: _BF16}
+    if device != tree.device or q.dtype not in types or k.dtype not in types or v.dtype != k.dtype:
+        _bad(f"attn_tree: q {q.dtype} on {device}, tree on {tree.device}, k {k.dtype}, v {v.dtype}: bf16 or f32 on one device are wanted")
+    rows = tree.desc.n_rows
+    width = q[0].numel() if rows else q.shape[1] if q.dim() > 1 else 0
+    if out is None:
+        out = torch.empty_like(q, memory_format=torch.contiguous_format)
+    elif out.dtype != q.dtype:
+        _bad(f"attn_tree: out is {out.dtype}, q {q.dtype}")
+    q_at, q_stride = _rows_of("q", q, device, width, rows)
+    o_at, o_stride = _rows_of("out", out, device, width, rows)
+    k_at, k_stride = _rows_of("k", k, device, n_kv_heads * head_dim, cache.rows)
+    v_at, v_stride = _rows_of("v", v, device, n_kv_heads * head_dim, cache.rows)
+    if v_stride != k_stride or width % head_dim:
+        _bad(f"attn_tree: k and v rows {k_stride} and {v_stride} elements apart, q rows of {width} for heads of {head_dim}")
+    s_at = None
+    if sinks is not None:
+        if sinks.device != device or sinks.dtype != torch.float32 or not sinks.is_contiguous() or sinks.numel() != width // head_dim:
+            _bad(f"attn_tree: sinks must be {width // head_dim} contiguous f32 values on {device}")
+        s_at = sinks.data_ptr()
+    desc = TreeAttnDesc(types[q.dtype], types[k.dtype], width // head_dim, n_kv_heads, head_dim, window, scale, 0, q_stride, k_stride, o_stride)
+    lib = load_library()
+    with _On(device) as stream:
+        need = lib.lum_op_attn_tree_workspace(desc, tree.desc, cache.desc)
+        if need == C.c_size_t(-1).value:
+            _check(_INVALID)
+        if need and workspace is None:
+            workspace = torch.empty(need, dtype=torch.uint8, device=device)
+        w_at, w_bytes = (workspace.data_ptr(), workspace.numel() * workspace.element_size()) if workspace is not None else (None, 0)
+        _check(lib.lum_op_attn_tree(desc, tree.desc, cache.desc, q_at, k_at, v_at, s_at, o_at, w_at, w_bytes, stream))
+    return out
+
+
+def tree_accept(tree: DraftTree, tokens, *, logits=None, picks=None, path_len: int = 0):
+    """The nodes that stand: ``(path [n_seq, path_len], n_accepted [n_seq], next_token [n_seq])``, int32.
+
+    Node 0 stands; at a node the model picks the arg-max of its row of ``logits`` [rows, vocab] f32 (the last maximum, as the greedy sample does) or
+    ``picks`` [rows] (what a sampler drew); the first child whose token (``tokens`` [rows]) is the pick stands next.  ``path`` has -1 behind the nodes that stand;
+    ``next_token`` is the pick at the last of them."""
+    torch = _torch()
+    device, n, rows = tree.device, tree.desc.n_seq, tree.desc.n_rows
+    path_len = path_len or tree.desc.max_rows
+    t_at, p_at = _ints("tokens", tokens, device), _ints("picks", picks, device, optional=True)
+    if tokens.numel() != rows or (picks is not None and picks.numel() != rows):
+        _bad(f"tree_accept: {tokens.numel()} tokens for {rows} rows")
+    l_at, vocab, ld = None, 0, 0
+    if logits is not None:
+        if logits.dtype != torch.float32 or logits.dim() != 2 or logits.device != device or logits.shape[0] != rows or logits.stride(1) != 1:
+            _bad(f"tree_accept: logits must be [{rows}, vocab] f32 on {device}, dense in a row")
+        l_at, vocab, ld = logits.data_ptr(), logits.shape[1], (logits.stride(0) if rows > 1 else 0)
+    path = torch.empty((n, path_len), dtype=torch.int32, device=device)
+    count, after = torch.empty((2, n), dtype=torch.int32, device=device).unbind(0)
+    lib = load_library()
+    with _On(device) as stream:
+        w_at, need = None, 0
+        if logits is not None:
+            need = lib.lum_op_tree_accept_workspace(tree.desc, vocab)
+            if need == C.c_size_t(-1).value:
+                _check(_INVALID)
+            if need:
+                workspace = torch.empty(need, dtype=torch.uint8, device=device)
+                w_at = workspace.data_ptr()
+        _check(lib.lum_op_tree_accept(tree.desc, t_at, l_at, vocab, ld, p_at, path.data_ptr(), path_len, count.data_ptr(), after.data_ptr(), w_at, need, stream))
+    return path, count, after
+
+
+def _planes(planes):
+    torch = _torch()
+    if planes.dtype != torch.int64 or planes.dim() != 2 or planes.shape[1] != 2 or not planes.is_contiguous() or not planes.is_cuda:
+        _bad("planes: a contiguous [planes, 2] int64 tensor on the GPU is wanted (address and bytes of a row)")
+    return planes.data_ptr(), planes.shape[0]
+
+
+def kv_planes(tensors):
+    """The table of planes that :func:`kv_compact` and :func:`kv_copy` take, of 2-d (or 3-d: one plane per first index) cache tensors whose rows follow each
+    other.  Made once for a cache; the tensors have to outlive it."""
+    torch = _torch()
+    entries, device = [], None
+    for t in tensors:
+        for p in (t.unbind(0) if t.dim() == 3 else [t]):
+            bytes_ = p.shape[1] * p.element_size()
+            if p.dim() != 2 or not p.is_contiguous() or bytes_ % 16 or p.data_ptr() % 16:
+                _bad("kv_planes: contiguous rows of a multiple of 16 bytes, 16-byte aligned, are wanted")
+            if device is not None and p.device != device:
+                _bad("kv_planes: the planes are on different devices")
+            device = p.device
+            entries.append([p.data_ptr(), bytes_])
+    if not entries:
+        _bad("kv_planes: no planes")
+    return torch.tensor(entries, dtype=torch.int64).to(device)
+
+
+def kv_compact(planes, cache: KvMap, tree: DraftTree, path, n_accepted) -> None:
+    """Row ``prefix + path[s, i]`` of every plane becomes row ``prefix + i``, for i < n_accepted[s]."""
+    p_at, n = _planes(planes)
+    device = planes.device
+    path_at, n_at = _ints("path", path, device, dims=2), _ints("n_accepted", n_accepted, device)
+    if device != tree.device or path.shape[0] != tree.desc.n_seq or n_accepted.numel() != tree.desc.n_seq:
+        _bad(f"kv_compact: paths of {path.shape[0]} and counts of {n_accepted.numel()} sequences for {tree.desc.n_seq}")
+    with _On(device) as stream:
+        _check(load_library().lum_op_kv_compact(p_at, n, cache.desc, tree.desc, path_at, path.shape[1], n_at, stream))
+
+
+def kv_copy(planes, rows: int, spans, *, max_rows: int) -> None:
+    """Copies spans of rows in every plane of ``rows`` rows: ``spans`` [n, 3] int32 of {first source row, first destination row, rows <= max_rows}.
+    Destinations overlap neither each other nor a source."""
+    p_at, n = _planes(planes)
+    s_at = _ints("spans", spans, planes.device, dims=2)
+    if spans.shape[1] != 3:
+        _bad("kv_copy: spans are [n, 3]")
+    with _On(planes.device) as stream:
+        _check(load_library().lum_op_kv_copy(p_at, n, rows, s_at, spans.shape[0], max_rows, stream))
+
+
+def status(device=None) -> None:
+    """Waits for the current stream of ``device`` and raises what a kernel of these operators found wrong since the last call."""
+    torch = _torch()
+    with _On(torch.device("cuda", torch.cuda.current_device()) if device is None else torch.device(device)) as stream:
+        _check(load_library().lum_op_status(stream))

@@ -103,6 +103,34 @@ class Sampling(C.Structure):
     _fields_ = [("temperature", C.c_float), ("top_p", C.c_float), ("top_k", C.c_int32), ("reserved", C.c_int32), ("seed", C.c_uint64)]
 
 
+class DraftTreeDesc(C.Structure):
+    """Mirror of ``lum_draft_tree`` (include/lum_tree.h): the drafted trees of a batch."""
+
+    _fields_ = [("row_start", C.c_void_p), ("prefix", C.c_void_p), ("parent", C.c_void_p), ("slot", C.c_void_p),
+                ("n_seq", C.c_int32), ("n_rows", C.c_int32), ("max_rows", C.c_int32), ("max_prefix", C.c_int32)]
+
+
+class KvMapDesc(C.Structure):
+    """Mirror of ``lum_kv_map`` (include/lum_tree.h): where the cached rows of a slot are."""
+
+    _fields_ = [("page_table", C.c_void_p), ("rows", C.c_int64), ("slots", C.c_int32), ("max_seq", C.c_int32), ("page_rows", C.c_int32),
+                ("pages_per_seq", C.c_int32)]
+
+
+class TreeAttnDesc(C.Structure):
+    """Mirror of ``lum_tree_attn`` (include/lum_tree.h): types, heads and strides of the attention of drafted trees."""
+
+    _fields_ = [("q_dtype", C.c_uint32), ("kv_dtype", C.c_uint32), ("n_q_heads", C.c_int32), ("n_kv_heads", C.c_int32), ("head_dim", C.c_int32),
+                ("window", C.c_int32), ("scale", C.c_float), ("reserved", C.c_int32), ("q_stride", C.c_int64), ("kv_stride", C.c_int64),
+                ("out_stride", C.c_int64)]
+
+
+class KvPlaneDesc(C.Structure):
+    """Mirror of ``lum_kv_plane`` (include/lum_tree.h): the rows of one K or V cache."""
+
+    _fields_ = [("rows", C.c_void_p), ("row_bytes", C.c_uint64)]
+
+
 def _desc(**kw) -> ModelDesc:
     d = ModelDesc()
     base = dict(max_seq=4096, rms_eps=1e-5, rope_style=0, qk_norm=0, tied_head=0, max_new_tokens=4096, tp_size=1, tp_rank=0, max_batch=1)
@@ -292,6 +320,12 @@ def load_library() -> C.CDLL:
         "lum_op_q8_0_dequant": (i32, [vp, vp, sz, vp, vp]),
         "lum_op_synth_q8_0": (i32, [u64, u64, sz, vp, vp, vp]),
         "lum_op_synth_normal": (i32, [u64, u64, u32, sz, i32, vp, vp]),
+        "lum_op_attn_tree_workspace": (sz, [P(TreeAttnDesc), P(DraftTreeDesc), P(KvMapDesc)]),
+        "lum_op_attn_tree": (i32, [P(TreeAttnDesc), P(DraftTreeDesc), P(KvMapDesc), vp, vp, vp, vp, vp, vp, sz, vp]),
+        "lum_op_tree_accept_workspace": (sz, [P(DraftTreeDesc), i32]),
+        "lum_op_tree_accept": (i32, [P(DraftTreeDesc), vp, vp, i32, C.c_int64, vp, vp, i32, vp, vp, vp, sz, vp]),
+        "lum_op_kv_compact": (i32, [vp, i32, P(KvMapDesc), P(DraftTreeDesc), vp, i32, vp, vp]),
+        "lum_op_kv_copy": (i32, [vp, i32, C.c_int64, vp, i32, i32, vp]),
     }
     for name, (res, args) in sig.items():
         fn = getattr(lib, name)   # AttributeError here = header and library disagree: fail loudly

@@ -1,0 +1,429 @@
+"""The operators of speculative decoding (include/lum_tree.h, oneiron_luminal_b200.drafts) against float64 statements of them."""
+import numpy as np
+import pytest
+
+import drafts_plain as plain
+
+pytestmark = pytest.mark.gpu
+
+
+@pytest.fixture(scope="module")
+def torch():
+    import torch as t
+    assert t.cuda.is_available(), "GPU tests need a CUDA device"
+    t.cuda.set_device(0)
+    return t
+
+
+@pytest.fixture(scope="module")
+def ops(pkg):
+    return pkg.drafts
+
+
+class Batch:
+    """Sequences with their trees, a cache that holds nothing but NaN where no sequence has a row, and the same facts as numpy arrays."""
+
+    def __init__(self, torch, ops, nodes, prefix, *, n_kv=2, group=2, dim=64, q="bf16", cache=None, page=0, seed=0, kind="mixed", slots=None, gap=0, head=0, q_pad=0, kv_pad=0, sinks=False,
+                 hint=0):
+        rng = np.random.default_rng(seed)
+        self.torch, self.ops, self.nodes, self.prefix, self.n_kv, self.dim, self.heads = torch, ops, nodes, prefix, n_kv, dim, n_kv * group
+        cache = cache or "bf16"
+        types = {"bf16": torch.bfloat16, "f32": torch.float32}
+        n = len(nodes)
+        self.parents = [plain.random_parents(rng, t, kind) for t in nodes]
+        self.start = np.concatenate([[0], np.cumsum(nodes)]) + head
+        self.rows = int(self.start[-1]) + gap
+        i32 = dict(dtype=torch.int32, device="cuda")
+        flat = [-7] * head + sum(self.parents, []) + [-7] * gap
+        most = max(t + p for t, p in zip(nodes, prefix))
+        self.slot = slots if slots is not None else list(range(n))
+        n_slots = max(self.slot) + 2
+        width = n_kv * dim
+        if page:
+            per = -(-most // page) + 1
+            need = [-(-(t + p) // page) for t, p in zip(nodes, prefix)]
+            order = rng.permutation(sum(need) + 5)
+            table = np.full((n_slots, per), -1, np.int32)
+            at = 0
+            for s, m in zip(self.slot, need):
+                table[s, :m] = order[at:at + m]
+                at += m
+            total = (sum(need) + 5) * page
+            self.where = [(table[s, np.arange(t + p) // page].astype(np.int64) * page + np.arange(t + p) % page) for s, t, p in zip(self.slot, nodes, prefix)]
+            self.map = ops.KvMap(total, max_seq=per * page, page_table=torch.tensor(table, **i32), page_rows=page)
+        else:
+            total = n_slots * most
+            self.where = [s * most + np.arange(t + p) for s, t, p in zip(self.slot, nodes, prefix)]
+            self.map = ops.KvMap(total, max_seq=most, slots=n_slots)
+
+        def cache_rows():
+            full = torch.full((total, width + kv_pad), float("nan"), dtype=types[cache])
+            x = torch.tensor(rng.standard_normal((total, width)), dtype=types[cache])
+            for w in self.where:
+                full[w, :width] = x[w]
+            return full.cuda()[:, :width]
+
+        self.k, self.v = cache_rows(), cache_rows()
+        qw = self.heads * dim
+        self.q = torch.tensor(rng.standard_normal((self.rows, qw + q_pad)) * 1.5, dtype=types[q]).cuda()[:, :qw]
+        self.sinks = torch.tensor(rng.standard_normal(self.heads), dtype=torch.float32).cuda() if sinks else None
+        self.tree = ops.DraftTree(torch.tensor(self.start, **i32), torch.tensor(prefix, **i32), torch.tensor(flat, **i32), max_rows=max(max(nodes), 1), max_prefix=max(prefix) + hint,
+                                  slot=None if slots is None else torch.tensor(slots, **i32))
+
+    def run(self, **kw):
+        return self.ops.attn_tree(self.q, self.k, self.v, self.tree, self.map, n_kv_heads=self.n_kv, head_dim=self.dim, sinks=self.sinks, **kw)
+
+    def want(self, window=0, scale=None):
+        """(result, bound) as [rows, heads * dim], NaN where the rows belong to no sequence."""
+        out = np.full((self.rows, self.heads, self.dim), np.nan)
+        off = np.zeros_like(out)
+        k, v, q = (x.double().cpu().numpy() for x in (self.k, self.v, self.q))
+        sinks = None if self.sinks is None else self.sinks.double().cpu().numpy()
+        for s, w in enumerate(self.where):
+            a, b = self.start[s], self.start[s + 1]
+            if a < b:
+                shape = (len(w), self.n_kv, self.dim)
+                out[a:b], off[a:b] = plain.attention(q[a:b].reshape(-1, self.heads, self.dim), k[w].reshape(shape), v[w].reshape(shape), self.parents[s], self.prefix[s], self.n_kv, window, sinks,
+                                                     scale)
+        return out.reshape(self.rows, -1), off.reshape(self.rows, -1)
+
+    def check(self, got, window=0, scale=None):
+        want, off = self.want(window, scale)
+        live = ~np.isnan(want[:, 0])
+        g = got.double().cpu().numpy()[live]
+        want, off = want[live], off[live]
+        if got.dtype == self.torch.bfloat16:
+            off = off + 2.0 ** -8 * (np.abs(want) + off) + 2.0 ** -16 * np.abs(self.v[np.concatenate(self.where)].double().cpu().numpy()).max()
+        bad = ~(np.abs(g - want) <= off)
+        assert not bad.any(), f"{bad.sum()} of {bad.size} off, worst {np.nanmax(np.abs(g - want) / off)} of the bound, NaN {np.isnan(g).sum()}"
+
+
+TYPES = [("bf16", "bf16"), ("f32", "bf16"), ("f32", "f32")]
+
+
+@pytest.mark.parametrize("q, cache", TYPES)
+@pytest.mark.parametrize("dim", [64, 128])
+@pytest.mark.parametrize("nodes, prefix", [([1], [0]), ([1], [1]), ([2], [63]), ([5], [64]), ([8], [500]), ([64], [130]), ([33], [31]), ([3, 1, 17, 9], [0, 200, 77, 129])])
+def test_attention(torch, ops, q, cache, dim, nodes, prefix):
+    b = Batch(torch, ops, nodes, prefix, dim=dim, q=q, cache=cache, seed=len(nodes) + prefix[0])
+    b.check(b.run())
+    ops.status()
+
+
+@pytest.mark.parametrize("q, cache", TYPES)
+@pytest.mark.parametrize("page", [16, 64, 128])
+def test_attention_pages_and_slots(torch, ops, q, cache, page):
+    b = Batch(torch, ops, [7, 20, 1], [150, 15, 64], q=q, cache=cache, page=page, slots=[4, 0, 2], seed=page)
+    b.check(b.run())
+    ops.status()
+
+
+@pytest.mark.parametrize("q, cache", TYPES)
+@pytest.mark.parametrize("group, n_kv, nodes", [(1, 3, 40), (3, 2, 43), (8, 1, 33), (7, 2, 19), (16, 1, 9), (1, 1, 200), (5, 1, 26), (64, 1, 3)])
+def test_attention_heads(torch, ops, q, cache, group, n_kv, nodes):
+    b = Batch(torch, ops, [nodes], [90], n_kv=n_kv, group=group, q=q, cache=cache, seed=group)
+    b.check(b.run())
+
+
+@pytest.mark.parametrize("q, cache", TYPES)
+@pytest.mark.parametrize("kind", ["chain", "star", "forest"])
+def test_attention_of_tree_shapes(torch, ops, q, cache, kind):
+    b = Batch(torch, ops, [256, 100], [70, 3], n_kv=1, group=2, q=q, cache=cache, kind=kind)
+    b.check(b.run())
+
+
+@pytest.mark.parametrize("q, cache", TYPES)
+@pytest.mark.parametrize("window", [1, 2, 63, 64, 65, 200, 100000])
+@pytest.mark.parametrize("page", [0, 16])
+def test_attention_window_and_sinks(torch, ops, q, cache, window, page):
+    b = Batch(torch, ops, [30, 6], [333, 0], q=q, cache=cache, kind="mixed", page=page, sinks=True, seed=window)
+    b.check(b.run(window=window), window=window)
+    b = Batch(torch, ops, [30, 6], [333, 0], q=q, cache=cache, kind="chain", page=page, seed=window)
+    b.check(b.run(window=window), window=window)
+
+
+@pytest.mark.parametrize("q, cache", TYPES)
+def test_attention_strides_scale_and_rows_of_nobody(torch, ops, q, cache):
+    b = Batch(torch, ops, [4, 0, 9], [100, 5, 31], q=q, cache=cache, head=2, gap=3, q_pad=16, kv_pad=32)
+    out = torch.full((b.rows, b.q.shape[1] + 8), 5.0, dtype=b.q.dtype, device="cuda")
+    got = b.run(out=out[:, :-8], scale=0.37)
+    b.check(got, scale=0.37)
+    assert (out[:2] == 5.0).all() and (out[-3:] == 5.0).all() and (out[:, -8:] == 5.0).all()
+    ops.status()
+
+
+@pytest.mark.parametrize("q, cache", TYPES)
+def test_attention_of_long_and_uneven_batches(torch, ops, q, cache):
+    """Chunks of keys that are joined, sequences of very different lengths, a bound on the lengths that is far above them."""
+    for hint in (0, 20000):
+        b = Batch(torch, ops, [3, 12, 1], [5000, 64, 1], n_kv=1, group=4, dim=128, q=q, cache=cache, page=64, hint=hint)
+        b.check(b.run())
+        ops.status()
+
+
+@pytest.mark.parametrize("q, cache", TYPES)
+@pytest.mark.parametrize("value", [float("inf"), float("-inf"), float("nan"), 3.0e38])
+def test_attention_leaves_out_what_is_masked_whatever_it_holds(torch, ops, q, cache, value):
+    """A node that the others do not see, a row of the cache outside the window, and keys of the next sequence hold infinities: only who sees them is touched."""
+    b = Batch(torch, ops, [6, 4], [70, 66], q=q, cache=cache, kind="star", seed=3)
+    want, _ = b.want(window=40)
+    rows = [int(b.where[0][70 + 3]), int(b.where[0][2]), int(b.where[1][66 + 2])]      # node 3, a far row, node 2 of the other
+    for r in rows:
+        b.k[r], b.v[r] = value, value
+    got = b.run(window=40).double().cpu().numpy()
+    sees = {3, 6 + 2}
+    for i in range(10):
+        if i in sees:
+            if not abs(value) < 1e39:
+                assert not np.isfinite(got[i]).all()
+        else:
+            assert np.abs(got[i] - want[i]).max() < 0.05, i
+    ops.status()
+
+
+@pytest.mark.parametrize("q, cache", TYPES)
+def test_attention_large_scores(torch, ops, q, cache):
+    """One key takes everything, scores of some hundred: no overflow, and -inf keys weigh nothing."""
+    b = Batch(torch, ops, [5], [100], q=q, cache=cache, kind="chain")
+    b.k[int(b.where[0][17])] *= 200.0
+    b.check(b.run())
+    b = Batch(torch, ops, [2], [40], q=q, cache=cache)
+    b.q[:] = b.q.abs()
+    b.k[int(b.where[0][7])] = float("-inf")
+    got = b.run().double().cpu().numpy()
+    b.k[int(b.where[0][7])] = -1e4
+    want, off = b.want()
+    assert np.abs(got - want).max() < 0.05
+
+
+def test_attention_under_capture_on_another_stream_and_twice_at_once(torch, ops):
+    b = Batch(torch, ops, [9, 30], [700, 90], dim=128, group=4, page=64)
+    c = Batch(torch, ops, [3], [2000], dim=64, group=8, q="f32", seed=5)
+    first, second = b.run().clone(), c.run().clone()
+    s1, s2 = torch.cuda.Stream(), torch.cuda.Stream()
+    torch.cuda.synchronize()
+    outs = []
+    for _ in range(10):
+        with torch.cuda.stream(s1):
+            x = b.run()
+        with torch.cuda.stream(s2):
+            y = c.run()
+        outs.append((x, y))
+    torch.cuda.synchronize()
+    for x, y in outs:
+        assert torch.equal(x, first) and torch.equal(y, second)
+    out = torch.zeros_like(b.q.contiguous())
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        b.run(out=out)
+        y = c.run()
+    out.zero_()
+    b.q.mul_(0.5)
+    for _ in range(3):
+        graph.replay()
+    torch.cuda.synchronize()
+    b.check(out)
+    assert torch.equal(y, second)
+    ops.status()
+
+
+def test_attention_bad_numbers_on_the_device_are_left_out_and_reported(torch, ops, pkg):
+    def refused():
+        with pytest.raises(pkg.LumError) as e:
+            ops.status()
+        assert e.value.code == -4
+        ops.status()
+
+    b = Batch(torch, ops, [4, 5], [100, 40], page=16)
+    good = b.run().clone()
+    b.map.tensors[0][1, 1] = 10 ** 6                         # a page outside the pool: the other sequence is untouched
+    got = b.run()
+    assert torch.equal(got[:4], good[:4])
+    refused()
+    b = Batch(torch, ops, [4, 5], [100, 40])
+    good = b.run().clone()
+    b.tree.tensors[1][1] = 10 ** 6                           # more cached rows than the call named
+    out = torch.full_like(b.q, 3.0)
+    b.run(out=out)
+    assert torch.equal(out[:4], good[:4]) and (out[4:] == 3.0).all()
+    refused()
+    b.tree.tensors[1][1] = 40
+    b.tree.tensors[2][6] = 3                                 # a parent that is a later node
+    assert torch.equal(b.run()[:4], good[:4])
+    refused()
+    b.tree.tensors[2][6] = 0
+    b.tree.tensors[0][2] = 10 ** 6                           # rows outside the batch
+    assert torch.equal(b.run()[:4], good[:4])
+    refused()
+
+
+# ---------------------------------------------------------------------------------------------------- accepted nodes
+
+
+def accept_case(torch, ops, nodes, vocab, seed, agree=0.7, spread=0):
+    rng = np.random.default_rng(seed)
+    parents = [plain.random_parents(rng, t) for t in nodes]
+    start = np.concatenate([[0], np.cumsum(nodes)])
+    rows = int(start[-1])
+    tokens = rng.integers(0, vocab, rows).astype(np.int32)
+    logits = rng.standard_normal((rows, vocab)).astype(np.float32)
+    for s, ps in enumerate(parents):
+        for i, p in enumerate(ps):
+            if p >= 0 and rng.random() < agree:
+                logits[start[s] + p, tokens[start[s] + i]] = 20.0 + i
+    i32 = dict(dtype=torch.int32, device="cuda")
+    tree = ops.DraftTree(torch.tensor(start, **i32), torch.zeros(len(nodes), **i32), torch.tensor(sum(parents, []), **i32), max_rows=max(nodes), max_prefix=0)
+    return parents, start, tokens, logits, tree, torch.tensor(tokens, **i32)
+
+
+def check_accept(got, parents, start, tokens, picks):
+    path, count, after = (x.cpu().numpy() for x in got)
+    for s, ps in enumerate(parents):
+        a, b = start[s], start[s + 1]
+        want, nxt = plain.accept(tokens[a:b], ps, picks[a:b])
+        assert count[s] == len(want) and after[s] == nxt, (s, want, path[s], count[s], after[s], nxt)
+        assert list(path[s][:len(want)]) == want and (path[s][len(want):] == -1).all()
+
+
+@pytest.mark.parametrize("nodes, vocab", [([1], 5), ([8], 1000), ([64, 1, 30], 4097), ([256], 300), ([5] * 40, 50), ([16] * 8, 32064), ([3, 0, 2], 1), ([2], 128256), ([64], 128256)])
+def test_accept(torch, ops, nodes, vocab):
+    for seed in range(3):
+        parents, start, tokens, logits, tree, t = accept_case(torch, ops, nodes, vocab, seed)
+        picks = [plain.pick(r) for r in logits]
+        check_accept(ops.tree_accept(tree, t, logits=torch.tensor(logits).cuda()), parents, start, tokens, picks)
+        check_accept(ops.tree_accept(tree, t, picks=torch.tensor(picks, dtype=torch.int32, device="cuda"), path_len=max(nodes) + 3), parents, start, tokens, picks)
+        wide = torch.full((len(tokens), vocab + 3), 1e30).cuda()
+        wide[:, :vocab] = torch.tensor(logits).cuda()
+        check_accept(ops.tree_accept(tree, t, logits=wide[:, :vocab]), parents, start, tokens, picks)
+    ops.status()
+
+
+@pytest.mark.parametrize("vocab", [7, 33, 4096, 130000])
+def test_accept_ties_and_undefined_logits(torch, ops, vocab):
+    """The last maximum wins, NaN counts as -inf, -0 equals 0; the same token twice under one node: the first of them."""
+    i32 = dict(dtype=torch.int32, device="cuda")
+    tree = ops.DraftTree(torch.tensor([0, 5], **i32), torch.zeros(1, **i32), torch.tensor([-1, 0, 0, 2, 1], **i32), max_rows=5, max_prefix=0)
+    last = vocab - 1
+    tokens = np.array([0, last, last, 2, 3], np.int32)
+    rows = np.zeros((5, vocab), np.float32)
+    rows[0, 1] = -0.0
+    rows[1] = np.nan
+    rows[1, 3] = -5.0
+    rows[4] = np.nan
+    picks = [plain.pick(r) for r in rows]
+    assert picks[0] == last and picks[1] == 3 and picks[4] == last
+    got = ops.tree_accept(tree, torch.tensor(tokens, **i32), logits=torch.tensor(rows).cuda())
+    check_accept(got, [[-1, 0, 0, 2, 1]], [0, 5], tokens, picks)
+    rows[0] = -np.inf
+    rows[0, 2] = np.inf
+    rows[0, 4] = np.inf
+    check_accept(ops.tree_accept(tree, torch.tensor(tokens, **i32), logits=torch.tensor(rows).cuda()), [[-1, 0, 0, 2, 1]], [0, 5], tokens, [plain.pick(r) for r in rows])
+
+
+def test_accept_bad_trees_are_reported(torch, ops, pkg):
+    parents, start, tokens, logits, tree, t = accept_case(torch, ops, [6, 6], 50, 1)
+    tree.tensors[2][2] = 4
+    ops.tree_accept(tree, t, logits=torch.tensor(logits).cuda())
+    with pytest.raises(pkg.LumError):
+        ops.status()
+    tree.tensors[0][1] = -3
+    ops.tree_accept(tree, t, logits=torch.tensor(logits).cuda())
+    with pytest.raises(pkg.LumError):
+        ops.status()
+
+
+# ---------------------------------------------------------------------------------------------------- cache rows
+
+
+@pytest.mark.parametrize("page", [0, 16, 64])
+@pytest.mark.parametrize("row_bytes", [16, 48, 1024, 2080])
+def test_compact(torch, ops, page, row_bytes):
+    rng = np.random.default_rng(page + row_bytes)
+    b = Batch(torch, ops, [40, 1, 256, 9], [10, 3, 130, 0], page=page, slots=[2, 0, 5, 1])
+    planes = [torch.randint(-30000, 30000, (b.map.rows, n), dtype=torch.int16, device="cuda") for n in (row_bytes // 2, 8)]
+    want = [p.clone() for p in planes]
+    path, count = np.full((4, 256), -1, np.int32), []
+    for s, t in enumerate(b.nodes):
+        n = [17, 1, 256, 0][s]
+        pick = np.sort(rng.choice(t, n, replace=False)) if n else np.zeros(0, int)
+        path[s, :n] = pick
+        count.append(n)
+        w, p = b.where[s], b.prefix[s]
+        for x, y in zip(want, planes):
+            x[torch.tensor(w[p:p + n])] = y[torch.tensor(w[p + pick])]
+    i32 = dict(dtype=torch.int32, device="cuda")
+    ops.kv_compact(ops.kv_planes(planes), b.map, b.tree, torch.tensor(path, **i32), torch.tensor(count, **i32))
+    for x, y in zip(planes, want):
+        assert torch.equal(x, y)
+    ops.status()
+
+
+def test_compact_refuses_what_is_no_path(torch, ops, pkg):
+    b = Batch(torch, ops, [6, 6], [4, 5])
+    planes = [torch.randn(b.map.rows, 16, device="cuda")]
+    before = planes[0].clone()
+    i32 = dict(dtype=torch.int32, device="cuda")
+    table = ops.kv_planes(planes)
+    for path, count in (([[0, 3, 2], [0, 1, 2]], [3, 3]), ([[0, 6, 7], [0, 1, 2]], [3, 3]), ([[0, 1, 2], [0, 1, 2]], [7, 3]), ([[0, 1, 2], [0, 1, 2]], [-1, 3]), ([[-1, 1, 2], [0, 1, 2]], [2, 3])):
+        ops.kv_compact(table, b.map, b.tree, torch.tensor(path, **i32), torch.tensor(count, **i32))
+        with pytest.raises(pkg.LumError):
+            ops.status()
+        assert torch.equal(planes[0], before)
+
+
+@pytest.mark.parametrize("row_elems", [8, 40, 512])
+@pytest.mark.parametrize("lens", [[1], [3, 0, 5], [700, 1, 64], [37] * 50])
+def test_copy(torch, ops, row_elems, lens):
+    rng = np.random.default_rng(len(lens))
+    most = max(lens)
+    rows = 2 * len(lens) * most + 3
+    kv = torch.randn(5, rows, row_elems, device="cuda").to(torch.bfloat16)
+    first = rng.permutation(2 * len(lens)) * most + 3
+    spans = [[first[i], first[len(lens) + i], n] for i, n in enumerate(lens)]
+    want = kv.clone()
+    for a, b, n in spans:
+        want[:, b:b + n] = kv[:, a:a + n]
+    i32 = dict(dtype=torch.int32, device="cuda")
+    ops.kv_copy(ops.kv_planes([kv]), rows, torch.tensor(np.array(spans), **i32), max_rows=most)
+    assert torch.equal(kv, want)
+    ops.status()
+
+
+def test_copy_of_spans_outside_the_cache_is_left_out(torch, ops, pkg):
+    kv = torch.randn(2, 100, 64, device="cuda")
+    want = kv.clone()
+    want[:, 50:60] = kv[:, 0:10]
+    i32 = dict(dtype=torch.int32, device="cuda")
+    ops.kv_copy(ops.kv_planes([kv]), 100, torch.tensor([[0, 50, 10], [95, 20, 6], [10, 96, 5], [-1, 30, 2], [0, 70, 11]], **i32), max_rows=10)
+    with pytest.raises(pkg.LumError):
+        ops.status()
+    assert torch.equal(kv, want)
+
+
+def test_a_step_of_speculative_decoding(torch, ops):
+    """Attention over drafts, acceptance, compaction: the kept rows are those of the path, and attending again from a chain over them gives what the tree gave."""
+    b = Batch(torch, ops, [12, 7], [100, 33], page=16, q="f32", dim=64)
+    out = b.run().clone()
+    rng = np.random.default_rng(9)
+    tokens = rng.integers(0, 90, b.rows).astype(np.int32)
+    logits = rng.standard_normal((b.rows, 90)).astype(np.float32)
+    for s, ps in enumerate(b.parents):
+        at = 0
+        for i, p in enumerate(ps):
+            if p == at and len(set(tokens[b.start[s]:b.start[s + 1]])) > 0:
+                logits[b.start[s] + at, tokens[b.start[s] + i]] = 30.0
+                at = i
+    i32 = dict(dtype=torch.int32, device="cuda")
+    path, count, after = ops.tree_accept(b.tree, torch.tensor(tokens, **i32), logits=torch.tensor(logits).cuda())
+    check_accept((path, count, after), b.parents, b.start, tokens, [plain.pick(r) for r in logits])
+    kept = [path[s, :int(count[s])].cpu().numpy() for s in range(2)]
+    assert all(len(p) > 1 for p in kept)
+    ops.kv_compact(ops.kv_planes([b.k, b.v]), b.map, b.tree, path, count)
+    chain = [list(range(-1, len(p) - 1)) for p in kept]
+    start = np.concatenate([[0], np.cumsum([len(p) for p in kept])])
+    tree = ops.DraftTree(torch.tensor(start, **i32), b.tree.tensors[1], torch.tensor(sum(chain, []), **i32), max_rows=12, max_prefix=100)
+    rows = np.concatenate([b.start[s] + p for s, p in enumerate(kept)])
+    again = ops.attn_tree(b.q[torch.tensor(rows)], b.k, b.v, tree, b.map, n_kv_heads=b.n_kv, head_dim=b.dim)
+    # other tiles, another order of sums: two f32 results, each within the bound of the same exact one
+    assert (again - out[torch.tensor(rows)]).abs().max().item() < 2e-5
+    ops.status()
