@@ -41,17 +41,27 @@ struct TreeAcceptArgs {
 };
 struct KvPlane { void* rows; uint64_t row_bytes; };
 
-// Sequence s of a batch, as far as it can be trusted: false (and a status bit) where its numbers do not fit what the call named.
+// Sequence s of a batch, as far as it can be trusted: its numbers, and false (and a status bit) where they do not fit what the call named.
 struct TreeSeq { int r0, n, prefix, slot; };
-__device__ __forceinline__ bool tree_seq(const TreeBatch& t, const TreeMap* m, int s, TreeSeq* o, uint32_t* status) {
-    o->r0 = __ldg(t.row_start + s);
-    o->n = __ldg(t.row_start + s + 1) - o->r0;
-    o->prefix = __ldg(t.prefix + s);
-    o->slot = t.slot ? __ldg(t.slot + s) : s;
-    const bool ok = o->r0 >= 0 && o->n >= 0 && o->n <= t.max_rows && o->r0 <= t.n_rows - o->n && o->prefix >= 0 && o->prefix <= t.max_prefix &&
-                    (!m || (o->slot >= 0 && o->slot < m->slots && o->prefix <= m->max_seq - o->n));
+__device__ __forceinline__ TreeSeq tree_seq_load(const TreeBatch& t, int s) {
+    TreeSeq o;
+    o.r0 = __ldg(t.row_start + s);
+    o.n = __ldg(t.row_start + s + 1);
+    o.prefix = __ldg(t.prefix + s);
+    o.slot = t.slot ? __ldg(t.slot + s) : s;
+    return o;
+}
+__device__ __forceinline__ bool tree_seq_ok(const TreeBatch& t, const TreeMap* m, TreeSeq* o, uint32_t* status) {      // once, behind tree_seq_load: n becomes a count
+    const long long n = (long long)o->n - o->r0;
+    const bool ok = o->r0 >= 0 && n >= 0 && n <= t.max_rows && o->n <= t.n_rows && o->prefix >= 0 && o->prefix <= t.max_prefix &&
+                    (!m || (o->slot >= 0 && o->slot < m->slots && o->prefix <= m->max_seq - n));
+    o->n = (int)n;
     if (!ok && status) atomicOr(status, LUM_ST_BAD_POS);
     return ok;
+}
+__device__ __forceinline__ bool tree_seq(const TreeBatch& t, const TreeMap* m, int s, TreeSeq* o, uint32_t* status) {
+    *o = tree_seq_load(t, s);
+    return tree_seq_ok(t, m, o, status);
 }
 // Physical row of a slot's row, -1 (and a status bit) where the page table or the cache does not hold it.
 __device__ __forceinline__ long long tree_row(const TreeMap& m, int slot, int row, uint32_t* status) {

@@ -28,16 +28,16 @@ __host__ __device__ inline TreeWork tree_work(int prefix, int n, int window) {
     return w;
 }
 
-// The tree in shared memory: depths and, as bits, the nodes that a node sees (itself and its ancestors, fewer than `window` places before it).  All
-// threads of the CTA; synchronise before and after.
+// The tree in shared memory: depths and, as bits, the nodes that a node sees (itself and its ancestors, fewer than `window` places before it).  By
+// `threads` threads that share barrier `id` (0: the whole CTA); synchronise afterwards.
 struct TreeNodes { unsigned int anc[kTreeMax][kTreeWords]; short depth[kTreeMax]; short parent[kTreeMax]; };
-__device__ __forceinline__ void tree_load(TreeNodes& s, const TreeBatch& t, const TreeSeq& q, int window, int tid, int threads, uint32_t* status) {
+__device__ __forceinline__ void tree_load(TreeNodes& s, const TreeBatch& t, const TreeSeq& q, int window, int tid, int threads, int id, uint32_t* status) {
     for (int i = tid; i < q.n; i += threads) {
         int p = __ldg(t.parent + q.r0 + i);
         if (p < -1 || p >= i) { p = -1; if (status) atomicOr(status, LUM_ST_BAD_TREE); }
         s.parent[i] = (short)p;
     }
-    __syncthreads();
+    named_sync(id, threads);
     for (int i = tid; i < q.n; i += threads) {
         unsigned int w[kTreeWords];
 #pragma unroll
@@ -93,7 +93,7 @@ __global__ void __launch_bounds__(256) attn_tree_rows(const TreeAttnArgs a, cons
     if (!tree_seq(a.t, &a.m, s, &q, a.status) || f0 >= q.n * G) return;
     const TreeWork w = tree_work(q.prefix, q.n, a.window);
     if (chunk * part.tiles >= w.n_tiles) return;
-    tree_load(tree, a.t, q, a.window, tid, 256, a.status);
+    tree_load(tree, a.t, q, a.window, tid, 256, 0, a.status);
     for (int x = tid; x < kRowsTile * HD / 4; x += 256) {
         const int r = x / (HD / 4), c = x % (HD / 4) * 4, f = f0 + r;
         float4 v = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
@@ -205,8 +205,8 @@ __global__ void __launch_bounds__(256) attn_tree_rows(const TreeAttnArgs a, cons
 }
 
 // ---- products on the tensor core (tcgen05): a bf16 cache
-// CTA = chunk x (K/V head, 128 query rows) x sequence: four softmax warps, a thread per query row; one warp that asks for keys and values, one that issues
-// the products.  Per tile of 64 cache rows:
+// CTA = chunk x (K/V head, 128 query rows) x sequence: four softmax warps, a thread per query row; one warp that asks for keys, one for
+// values, one that issues the products.  Per tile of 64 cache rows:
 //     S = Q K^T             M 128, N 64; Q in shared memory, one bf16 term (bf16 queries) or three (f32 queries, 24 bits)
 //     p = 2^(S - m)         a thread reads its row's 64 scores, masks, exponentiates, and stores the weights' terms over them
 //     O (+)= P V            M 128, N head_dim; P from tensor memory, V as stored (MN-major)
@@ -220,7 +220,7 @@ __global__ void __launch_bounds__(256) attn_tree_rows(const TreeAttnArgs a, cons
 //     thousands of keys the cuts add up.  Low terms go first.
 // A key that a row does not see has weight 0, but 0 times infinity is no zero: rows of V behind the last node or before the window are zeroed, and a row whose
 // result is not finite is computed again by tree_row_plain, key by key.
-constexpr int kTcThreads = 192;
+constexpr int kTcThreads = 224;                     // four softmax warps, K, products, V
 constexpr int kTcGroup = 128 * 16 + 16;              // Q: 16-byte column groups of 128 rows, the next one 16 bytes further on (banks)
 template <int HD, bool F32>
 struct TcShape {
@@ -260,12 +260,25 @@ __device__ __forceinline__ void tc_st16(uint32_t at, const uint32_t* v) {
 }
 __device__ __forceinline__ void tc_st_wait() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
 __device__ __forceinline__ float tc_ex2(float x) { float y; asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x)); return y; }
+// two at a time: the softmax warps are bound by what they issue (beside their exponentials)
+__device__ __forceinline__ float2 fma2(float2 a, float2 b, float2 c) {
+    float2 d;
+    asm("{\n\t.reg .b64 a, b, c, d;\n\tmov.b64 a, {%2, %3};\n\tmov.b64 b, {%4, %5};\n\tmov.b64 c, {%6, %7};\n\tfma.rn.f32x2 d, a, b, c;\n\tmov.b64 {%0, %1}, d;\n\t}"
+        : "=f"(d.x), "=f"(d.y) : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y), "f"(c.x), "f"(c.y));
+    return d;
+}
+__device__ __forceinline__ float2 add2(float2 a, float2 b) {
+    float2 d;
+    asm("{\n\t.reg .b64 a, b, d;\n\tmov.b64 a, {%2, %3};\n\tmov.b64 b, {%4, %5};\n\tadd.rn.f32x2 d, a, b;\n\tmov.b64 {%0, %1}, d;\n\t}"
+        : "=f"(d.x), "=f"(d.y) : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y));
+    return d;
+}
 // (x0, x1) as packed bf16, rounded; what is left of them goes back
 __device__ __forceinline__ uint32_t tc_term(float* x0, float* x1) {
     const __nv_bfloat162 h = __floats2bfloat162_rn(*x0, *x1);
     const uint32_t b = *(const uint32_t*)&h;
-    *x0 -= __uint_as_float(b << 16);
-    *x1 -= __uint_as_float(b & 0xffff0000u);
+    const float2 r = fma2(make_float2(__uint_as_float(b << 16), __uint_as_float(b & 0xffff0000u)), make_float2(-1.0f, -1.0f), make_float2(*x0, *x1));
+    *x0 = r.x; *x1 = r.y;
     return b;
 }
 __device__ __forceinline__ void tma_box(uint32_t dst, const CUtensorMap* map, int row, int col, uint32_t bar) {
@@ -323,11 +336,7 @@ __global__ void __launch_bounds__(kTcThreads, TcShape<HD, F32>::ctas) attn_tree_
     unsigned int* s_odd = (unsigned int*)(tc_smem + S::off_misc + 96);       // [4]: rows whose result is not finite
     TreeNodes& tree = *(TreeNodes*)(tc_smem + S::off_tree);
     if (part.chunks > 1) pdl_launch_dependents();    // (tree_combine waits for this kernel's end)
-    TreeSeq q;
-    if (!tree_seq(a.t, &a.m, s, &q, a.status) || f0 >= q.n * G) return;
-    const TreeWork w = tree_work(q.prefix, q.n, a.window);
-    const int t_first = w.t_lo + chunk * part.tiles, n_tiles = min(part.tiles, w.t_lo + w.n_tiles - t_first);
-    if (n_tiles <= 0) return;
+    TreeSeq q = tree_seq_load(a.t, s);               // on its way while the CTA sets itself up
     if (tid == 0) {
         for (int i = 0; i < 2; i++) {
             mbar_init(bar_k + 8 * i, 1);             // K(t) has landed
@@ -345,75 +354,102 @@ __global__ void __launch_bounds__(kTcThreads, TcShape<HD, F32>::ctas) attn_tree_
     __syncthreads();
     tc_fence_after_sync();
     const uint32_t tmem = *(volatile uint32_t*)(tc_smem + S::off_misc + 80);
+    const bool ok = tree_seq_ok(a.t, &a.m, &q, a.status);
+    const TreeWork w = tree_work(q.prefix, q.n, a.window);
+    const int t_first = w.t_lo + chunk * part.tiles, n_tiles = min(part.tiles, w.t_lo + w.n_tiles - t_first);
+    if (!ok || f0 >= q.n * G || n_tiles <= 0) {
+        if (warp == 5) tmem_dealloc(tmem, S::cols);
+        return;
+    }
     const int live_rows = min(128, q.n * G - f0);
+    const uint32_t magic = 0xffffffffu / (uint32_t)G + 1u;               // f / G = f magic / 2^32 for f < 2^18, 2 <= G <= 2^10
+    auto node_of = [&](int f) { return G == 1 ? f : (int)__umulhi((uint32_t)f, magic); };
 
-    // A wait that runs out of its budget is remembered; what follows neither waits nor multiplies any more, but meets every barrier.
+    // A wait that runs out of its budget is remembered; what follows hardly waits and multiplies no more, but meets every barrier.
     auto wait = [&](uint32_t bar, int t) {
-        if (*gave_up) return;
-        if (!mbar_wait(bar + 8u * (t & 1), (uint32_t)(t >> 1) & 1u)) *gave_up = 1;
+        const uint32_t at = bar + 8u * (t & 1), parity = (uint32_t)(t >> 1) & 1u;
+        if (mbar_try_wait(at, parity)) return;
+        if (!mbar_wait_abortable(at, parity, gave_up)) *gave_up = 1;
     };
     constexpr int kHalves = HD / 64;
-    auto load = [&](const CUtensorMap* map, int t, uint32_t dst, uint32_t full) {      // the producer's warp: a lane per box
+    // Where this lane's box of tile t starts in the cache (a lane per box); one page-table entry on its way while the tile before is waited for.
+    auto box_row = [&](int t) {
+        const int j = (t_first + t) * kTileKeys + lane * box_rows;
+        if (t >= n_tiles || lane >= kTileKeys / box_rows || j >= w.n_keys || j + box_rows <= w.low) return (int)a.m.rows;     // outside the tensor: zeros
+        const long long row = tree_row(a.m, q.slot, j, a.status);
+        return (int)(row < 0 ? a.m.rows : row);
+    };
+    auto load = [&](const CUtensorMap* map, int t, int row, uint32_t dst, uint32_t full) {
         const uint32_t bar = full + 8u * (t & 1);
+        dst += (uint32_t)(t & 1) * S::tile;
         if (lane == 0) mbar_arrive_expect_tx(bar, S::tile);
         __syncwarp();
-        if (lane < kTileKeys / box_rows) {
-            const int j = (t_first + t) * kTileKeys + lane * box_rows;
-            long long row = a.m.rows;                // outside the tensor: zeros
-            if (j < w.n_keys && j + box_rows > w.low) {
-                row = tree_row(a.m, q.slot, max(j, 0), a.status);
-                if (row < 0) row = a.m.rows;
-            }
-            // a box holds its halves of 64 dimensions one behind the other; a whole tile's are kTileKeys rows apart
-            if (box_rows == kTileKeys) tma_box(dst + (t & 1) * S::tile, map, (int)row, kvh * kHalves, bar);
-            else
-                for (int h = 0; h < kHalves; h++) tma_box(dst + (t & 1) * S::tile + h * (kTileKeys * 128) + lane * box_rows * 128, map, (int)row, kvh * kHalves + h, bar);
-        }
+        // a box holds its halves of 64 dimensions one behind the other; a whole tile's are kTileKeys rows apart
+        if (box_rows == kTileKeys) { if (elect_one()) tma_box(dst, map, row, kvh * kHalves, bar); }
+        else if (lane < kTileKeys / box_rows)
+#pragma unroll
+            for (int h = 0; h < kHalves; h++) tma_box(dst + h * (kTileKeys * 128) + lane * box_rows * 128, map, row, kvh * kHalves + h, bar);
     };
-    if (warp == 4) {
-        load(&map_k, 0, base + S::off_k, bar_k);
-        if (n_tiles > 1) load(&map_k, 1, base + S::off_k, bar_k);
-        load(&map_v, 0, base + S::off_v, bar_v);
-        if (n_tiles > 1) load(&map_v, 1, base + S::off_v, bar_v);
+    const bool loads_k = warp == 4, loads = loads_k || warp == 6;
+    int next_row = 0;
+    if (loads) {
+        const int first = box_row(0);
+        const int second = box_row(1);
+        next_row = box_row(2);
+        load(loads_k ? &map_k : &map_v, 0, first, base + (loads_k ? S::off_k : S::off_v), loads_k ? bar_k : bar_v);
+        if (n_tiles > 1) load(loads_k ? &map_k : &map_v, 1, second, base + (loads_k ? S::off_k : S::off_v), loads_k ? bar_k : bar_v);
     }
-    // ---- the tree and the queries
-    tree_load(tree, a.t, q, a.window, tid, kTcThreads, a.status);
-    for (int x = tid; x < 128 * (HD / 8); x += kTcThreads) {
-        const int r = x / (HD / 8), c = x % (HD / 8), f = f0 + r;
-        uint4 t[3] = {};
-        if (r < live_rows) {
-            const TQ* src = (const TQ*)a.q + (size_t)(q.r0 + f / G) * a.q_stride + ((size_t)kvh * G + f % G) * HD + c * 8;
-            if constexpr (F32) {
-                float y[8];
-                *(float4*)y = *(const float4*)src; *(float4*)(y + 4) = *(const float4*)(src + 4);
+    // ---- the tree, by the warps that then only issue; the queries, by the others
+    if (loads) {
+        tree_load(tree, a.t, q, a.window, (warp == 6 ? 32 : 0) + lane, 64, 1, a.status);
+        named_arrive(3, 192);
+    } else if (warp < 4) {
+        // (rows beyond the last query are left as they are: nobody reads what they make)
+        constexpr int kPieces = HD / 8, kStep = 128 / kPieces, kAhead = F32 ? 2 : 4;
+        const int c = tid % kPieces;
+        for (int r0 = tid / kPieces; r0 < live_rows; r0 += kStep * kAhead) {
+            uint4 raw[kAhead][F32 ? 2 : 1];
 #pragma unroll
-                for (int e = 0; e < 3; e++) t[e] = make_uint4(tc_term(y, y + 1), tc_term(y + 2, y + 3), tc_term(y + 4, y + 5), tc_term(y + 6, y + 7));
-            } else t[0] = *(const uint4*)src;
+            for (int u = 0; u < kAhead; u++) {
+                const int f = f0 + min(r0 + u * kStep, live_rows - 1), node = node_of(f);
+                const uint4* src = (const uint4*)((const TQ*)a.q + (size_t)(q.r0 + node) * a.q_stride + ((size_t)kvh * G + f - node * G) * HD + c * 8);
+#pragma unroll
+                for (int e = 0; e < (F32 ? 2 : 1); e++) raw[u][e] = src[e];
+            }
+#pragma unroll
+            for (int u = 0; u < kAhead; u++) {
+                const int r = r0 + u * kStep;
+                if (r >= live_rows) break;
+                unsigned char* dst = tc_smem + S::off_q + c * kTcGroup + r * 16;
+                if constexpr (F32) {
+                    float* y = (float*)raw[u];
+#pragma unroll
+                    for (int e = 0; e < 3; e++) *(uint4*)(dst + e * S::q_bytes) = make_uint4(tc_term(y, y + 1), tc_term(y + 2, y + 3), tc_term(y + 4, y + 5), tc_term(y + 6, y + 7));
+                } else *(uint4*)dst = raw[u][0];
+            }
         }
-#pragma unroll
-        for (int e = 0; e < S::q_terms; e++) *(uint4*)(tc_smem + S::off_q + e * S::q_bytes + c * kTcGroup + r * 16) = t[e];
-    }
-    fence_proxy_async_smem();
-    __syncthreads();
+        fence_proxy_async_smem();
+        named_arrive(2, 160);
+    } else named_sync(2, 160);                       // (the queries are there)
 
     float m_run = -INFINITY, l_run = 0.0f;
     float o[F32 ? HD : 1];
     const uint32_t mine = tmem + ((uint32_t)((warp & 3) * 32) << 16);
-    const int row = warp * 32 + lane, f = f0 + row, node = row < live_rows && warp < 4 ? f / G : -1;
-    if (warp == 4) {
+    const int row = warp * 32 + lane, f = f0 + row, node = row < live_rows && warp < 4 ? node_of(f) : -1;
+    if (loads) {
         // K(t + 2) goes out when S(t) is there, V(t + 2) when O holds tile t
-        int last_k = min(n_tiles, 2) - 1, last_v = last_k;
+        const CUtensorMap* map = loads_k ? &map_k : &map_v;
+        const uint32_t dst = base + (loads_k ? S::off_k : S::off_v), full = loads_k ? bar_k : bar_v, used = loads_k ? bar_s : bar_o;
+        int last = min(n_tiles, 2) - 1;
         for (int t = 2; t < n_tiles; t++) {
-            wait(bar_s, t - 2);
+            const int row = next_row;
+            next_row = box_row(t + 1);
+            wait(used, t - 2);
             if (__any_sync(0xffffffffu, *gave_up)) break;
-            load(&map_k, last_k = t, base + S::off_k, bar_k);
-            wait(bar_o, t - 2);
-            if (__any_sync(0xffffffffu, *gave_up)) break;
-            load(&map_v, last_v = t, base + S::off_v, bar_v);
+            load(map, last = t, row, dst, full);
         }
         // no copy is on its way when the CTA ends (they have landed long ago, unless a wait was given up)
-        for (int t = max(last_k - 1, 0); t <= last_k; t++) mbar_wait(bar_k + 8u * (t & 1), (uint32_t)(t >> 1) & 1u);
-        for (int t = max(last_v - 1, 0); t <= last_v; t++) mbar_wait(bar_v + 8u * (t & 1), (uint32_t)(t >> 1) & 1u);
+        for (int t = max(last - 1, 0); t <= last; t++) mbar_wait(full + 8u * (t & 1), (uint32_t)(t >> 1) & 1u);
     } else if (warp == 5) {
         constexpr uint32_t id_s = tc_idesc(kTileKeys, false), id_o = tc_idesc(HD, true);
         if (elect_one()) {
@@ -454,7 +490,6 @@ __global__ void __launch_bounds__(kTcThreads, TcShape<HD, F32>::ctas) attn_tree_
 #pragma unroll
             for (int i = 0; i < HD; i++) o[i] = 0.0f;
         const float scale = a.scale * kLog2e;
-        const int place = node >= 0 ? q.prefix + tree.depth[node] : 0;
         auto zero_v = [&](int t) {                   // rows of V(t) that no query row may see
             const int j0 = (t_first + t) * kTileKeys;
             if (j0 >= w.low && j0 + kTileKeys <= w.n_keys) return;
@@ -472,6 +507,7 @@ __global__ void __launch_bounds__(kTcThreads, TcShape<HD, F32>::ctas) attn_tree_
             zero_v(t);
             wait(bar_s, t);
             tc_fence_after_sync();
+            if (t == 0) named_sync(3, 192);          // (the tree is there)
             if (warp * 32 < live_rows) {             // (a warp without live rows leaves its rows of P as they are: nobody reads what they make)
                 const uint32_t sc = mine + (uint32_t)(t & 1) * 64u;
                 float v[64];
@@ -484,7 +520,7 @@ __global__ void __launch_bounds__(kTcThreads, TcShape<HD, F32>::ctas) attn_tree_
                     if (node >= 0) {
                         const int cached = q.prefix - j0;                // keys of the tile before the tree
                         see = cached >= 64 ? ~0ull : cached > 0 ? (1ull << cached) - 1 : 0ull;
-                        const int first = place - a.window + 1 - j0;
+                        const int first = q.prefix + tree.depth[node] - a.window + 1 - j0;
                         if (a.window > 0 && first > 0) see = first >= 64 ? 0ull : see & (~0ull << first);
 #pragma unroll
                         for (int k = 0; k < kTreeWords; k++) {           // nodes 32 k .. 32 k + 31 are the keys from 32 k + cached on
@@ -498,20 +534,28 @@ __global__ void __launch_bounds__(kTcThreads, TcShape<HD, F32>::ctas) attn_tree_
                         if (!((uint32_t)(see >> 32) >> i & 1u)) v[32 + i] = -INFINITY;
                     }
                 }
-                float top[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+                float top[4] = {v[0], v[1], v[2], v[3]};
 #pragma unroll
-                for (int i = 0; i < 64; i++) top[i & 3] = fmaxf(top[i & 3], v[i]);
-                const float tm = fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3])) * scale;
+                for (int i = 4; i < 60; i += 8)
+#pragma unroll
+                    for (int e = 0; e < 4; e++) top[e] = fmaxf(top[e], fmaxf(v[i + e], v[i + 4 + e]));
+#pragma unroll
+                for (int e = 0; e < 4; e++) top[e] = fmaxf(top[e], v[60 + e]);
+                const float tm = node >= 0 ? fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3])) * scale : -INFINITY;
                 // the reference of the exponents: kept while nothing is more than 2^8 times it
                 const bool grows = tm > m_run + (F32 ? 0.0f : 8.0f) || m_run == -INFINITY;
                 const float m_new = grows ? fmaxf(tm, m_run) : m_run;
                 const float alpha = m_new == m_run ? 1.0f : tc_ex2(m_run - m_new);
                 m_run = m_new;
                 const float off = m_new == -INFINITY ? 0.0f : -m_new;
-                float sum[2] = {0.0f, 0.0f};
+                float2 sum[2] = {};
 #pragma unroll
-                for (int i = 0; i < 64; i++) { v[i] = tc_ex2(fmaf(v[i], scale, off)); sum[i & 1] += v[i]; }
-                l_run = l_run * alpha + (sum[0] + sum[1]);
+                for (int i = 0; i < 64; i += 2) {
+                    const float2 x = fma2(make_float2(v[i], v[i + 1]), make_float2(scale, scale), make_float2(off, off));
+                    v[i] = tc_ex2(x.x); v[i + 1] = tc_ex2(x.y);
+                    sum[i >> 1 & 1] = add2(sum[i >> 1 & 1], make_float2(v[i], v[i + 1]));
+                }
+                l_run = l_run * alpha + ((sum[0].x + sum[0].y) + (sum[1].x + sum[1].y));
                 if constexpr (F32) {
                     uint32_t pk[16];
 #pragma unroll
@@ -568,7 +612,7 @@ __global__ void __launch_bounds__(kTcThreads, TcShape<HD, F32>::ctas) attn_tree_
         tc_fence_after_sync();
         // ---- out = O / l, or this chunk's share
         if (warp * 32 < live_rows) {
-            const int h = kvh * G + f % G, out_row = q.r0 + max(node, 0);
+            const int h = kvh * G + (node >= 0 ? f - node * G : 0), out_row = q.r0 + max(node, 0);
             const float inv = part.chunks == 1 && node >= 0 ? tree_inverse(a, h, m_run, l_run) : 1.0f;
             float odd = l_run * 0.0f;                // 0, or NaN where something is not finite
             const size_t at = part_at(a, chunk, out_row, h);
