@@ -230,6 +230,7 @@ int32_t check_attn(const lum_tree_attn* d, const lum_draft_tree* tree, const lum
     if (a->q_stride * qe % 16 || a->out_stride * qe % 16 || a->kv_stride * ke % 16) return refuse(op, "row strides must be multiples of 16 bytes");
     a->n_q = d->n_q_heads; a->n_kv = d->n_kv_heads; a->hd = d->head_dim; a->q_bf16 = qb; a->kv_bf16 = kb; a->window = d->window;
     a->scale = d->scale != 0.0f ? d->scale : 1.0f / __builtin_sqrtf((float)d->head_dim);
+    if (a->t.n_seq && a->t.n_rows && !tree_attn_supported(*a)) return refuse(op, "more than 128 query heads per K/V head, or a batch of 2^31 tiles of 64 keys (sequences x heads x cached rows)", LUM_E_UNSUPPORTED);
     return 0;
 }
 

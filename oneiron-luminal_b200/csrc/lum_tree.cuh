@@ -76,6 +76,7 @@ __device__ __forceinline__ long long tree_row(const TreeMap& m, int slot, int ro
     return -1;
 }
 
+bool tree_attn_supported(const TreeAttnArgs& a);     // heads per K/V head, and sizes that can be counted
 size_t tree_attn_workspace(const TreeAttnArgs& a, int sm_count);
 cudaError_t launch_tree_attn(const TreeAttnArgs& a, int sm_count, cudaStream_t st);
 size_t tree_accept_workspace(const TreeBatch& t, int vocab, int sm_count);

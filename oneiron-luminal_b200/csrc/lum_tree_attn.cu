@@ -2,9 +2,9 @@
 // (row p + a) and itself:
 //     o_i = sum_j w_ij v_j,   w_ij = exp(x_ij) / (sum_j exp(x_ij) + exp(sink)),   x_ij = scale q_i . k_j
 // One pass over the keys with the running maximum and sum of the softmax.  All nodes of a tree and the G query heads of a K/V head share every key: row
-// f = node * G + head of a K/V head's query rows.  The keys of a sequence are cut into chunks, one CTA each; where there are several, every chunk leaves its
-// (maximum, sum, outputs) in the workspace and tree_combine joins them.
+// f = node * G + head of a K/V head's query rows.
 #include <cuda.h>
+#include <algorithm>
 #include <type_traits>
 
 #include "lum_tree.cuh"
@@ -14,7 +14,7 @@ namespace lum {
 namespace {
 
 constexpr float kLog2e = 1.4426950408889634f;
-constexpr int kTileKeys = 64;                        // chunks are whole tiles of so many cache rows, from the first visible one's tile on
+constexpr int kTileKeys = 64;                        // tiles of so many cache rows, from the first visible one's tile on
 
 struct TreeWork {                                    // the keys of a sequence that any node sees: rows low .. n_keys - 1, tiles t_lo .. t_lo + n_tiles - 1
     int low, n_keys, t_lo, n_tiles;
@@ -61,145 +61,238 @@ __device__ __forceinline__ bool tree_sees(const TreeNodes& s, const TreeSeq& q, 
     return s.anc[i][a >> 5] >> (a & 31) & 1u;
 }
 
-struct Part {                                        // where chunk c leaves its share of (row, head); out is used where there is one chunk
-    float *o, *ml;                                   // [chunk][row][head][hd], [chunk][row][head][2]
-    int chunks, tiles;                               // chunks of the longest sequence, tiles of a chunk
+// How the work is shared out.  A unit is a (sequence, K/V head, tile of query rows); it may be cut into equal pieces of its tiles of keys, one CTA per piece.  How
+// long a piece may be is chosen on the device, where the lengths are.  A whole unit is finished by its CTA; a unit in pieces leaves a share (maximum, sum,
+// outputs) of each in the workspace, and tree_combine joins them.
+struct Share {
+    int* plan;                                       // [0] tiles of a piece at most, [1 + s] the first share of sequence s; written by CTA 0
+    float *ml, *o;                                   // [share][rows][2], [share][rows][hd]
+    int grid, shares, slots;                         // CTAs launched, shares there is room for, CTAs that run at once
+    int copies, rows, tile_rows;                     // copies of a query row in a tile, query rows of a share, of a unit
 };
-__device__ __forceinline__ size_t part_at(const TreeAttnArgs& a, int c, int row, int h) { return ((size_t)c * a.t.n_rows + row) * a.n_q + h; }
+__device__ __forceinline__ size_t share_at(const Share& p, int share, int r) { return (size_t)share * p.rows + r; }
+
+struct Piece {
+    TreeSeq q;
+    TreeWork w;
+    int s, kvh, f0, tile, tiles, share;              // sequence, K/V head, first query row, tiles [tile, tile + tiles) of the unit's; share -1: the whole unit
+};
+struct SeqWork { int units, tiles; };                // units of a sequence (0: none, or its numbers are wrong), tiles of keys of each
+__device__ __forceinline__ SeqWork seq_work(const TreeAttnArgs& a, const Share& p, int s, TreeSeq* q, TreeWork* w) {
+    const bool ok = tree_seq(a.t, &a.m, s, q, a.status);
+    *w = tree_work(q->prefix, q->n, a.window);
+    return {ok ? a.n_kv * ((q->n * (a.n_q / a.n_kv) + p.tile_rows - 1) / p.tile_rows) : 0, w->n_tiles};
+}
+__device__ __forceinline__ int pieces_of(int tiles, int per) { return (tiles + per - 1) / per; }
+__device__ __forceinline__ int warp_scan(int x, int lane) {                    // inclusive
+#pragma unroll
+    for (int i = 1; i < 32; i <<= 1) { const int y = __shfl_up_sync(0xffffffffu, x, i); if (lane >= i) x += y; }
+    return x;
+}
+// The CTA's piece, by one warp: {sequence or -1, unit, which of its pieces, first share of the unit or -1}; CTA 0 writes the plan down.
+// A piece is at most `per` tiles long.  Where there are fewer units than CTAs that run at once, the pieces should be as many as those, nearly: the even share of all
+// tiles, longer by what rounding up makes of it.  (Pieces are at most units + tiles / per, so the third choice always fits.)  Where there are more units, only one longer
+// than twice the even share is cut.  Short code: every CTA runs it once, cold.
+__device__ __forceinline__ int4 piece_find(const TreeAttnArgs& a, const Share& p, int lane, int* per_out) {
+    auto work = [&](int s) {
+        TreeSeq q;
+        TreeWork w;
+        return s < a.t.n_seq ? seq_work(a, p, s, &q, &w) : SeqWork{0, 1};
+    };
+    const SeqWork mine = work(lane);                 // (batches of up to 32 sequences: all there is)
+    int units = mine.units, total = mine.units * mine.tiles;                   // (the call bounds them)
+#pragma unroll 1
+    for (int s0 = 32; s0 < a.t.n_seq; s0 += 32) { const SeqWork x = work(s0 + lane); units += x.units; total += x.units * x.tiles; }
+    units = __reduce_add_sync(0xffffffffu, units);
+    total = __reduce_add_sync(0xffffffffu, total);
+    const float even = (float)total / (float)p.slots;
+    int per = (int)(2.0f * even) + 1;
+    if (units < p.slots) {
+        per = (int)even + 1;
+#pragma unroll 1
+        for (int i = 0; i < 2; i++) {
+            int n = mine.units * pieces_of(mine.tiles, per);
+#pragma unroll 1
+            for (int s0 = 32; s0 < a.t.n_seq; s0 += 32) { const SeqWork x = work(s0 + lane); n += x.units * pieces_of(x.tiles, per); }
+            n = __reduce_add_sync(0xffffffffu, n);
+            if (n <= p.slots) break;
+            per = i ? total / (p.slots - units) + 1 : (int)((float)per * (float)n / (float)p.slots) + 1;
+        }
+    }
+    *per_out = per;
+    if (blockIdx.x == 0 && lane == 0) p.plan[0] = per;
+    int before = 0, shares = 0;
+    int4 found = make_int4(-1, 0, 0, -1);
+#pragma unroll 1
+    for (int s0 = 0; s0 < a.t.n_seq; s0 += 32) {
+        const SeqWork x = s0 ? work(s0 + lane) : mine;
+        const int k = pieces_of(x.tiles, per), sum = warp_scan(x.units * k, lane), cut = k > 1 ? x.units * k : 0, cuts = warp_scan(cut, lane);
+        if (blockIdx.x == 0 && s0 + lane < a.t.n_seq) p.plan[1 + s0 + lane] = shares + cuts - cut;
+        const unsigned int in = __ballot_sync(0xffffffffu, (int)blockIdx.x < before + sum);
+        if (in && found.x < 0) {
+            const int l = __ffs(in) - 1, kl = __shfl_sync(0xffffffffu, k, l), at = (int)blockIdx.x - before - __shfl_sync(0xffffffffu, sum - x.units * k, l), unit = at / kl;
+            found = make_int4(s0 + l, unit, at - unit * kl, kl > 1 ? shares + __shfl_sync(0xffffffffu, cuts - cut, l) + unit * kl : -1);
+            if (blockIdx.x) break;
+        }
+        before += __shfl_sync(0xffffffffu, sum, 31);
+        shares += __shfl_sync(0xffffffffu, cuts, 31);
+    }
+    return found;
+}
+__device__ __forceinline__ void piece_load(const TreeAttnArgs& a, const Share& p, int4 found, int per, Piece& x) {
+    x.s = found.x;
+    const SeqWork y = seq_work(a, p, x.s, &x.q, &x.w);
+    const int per_head = y.units / a.n_kv, k = pieces_of(y.tiles, per), least = y.tiles / k, more = y.tiles - least * k;
+    x.kvh = found.y / per_head;                      // a K/V head's row tiles follow each other: their keys are in L2
+    x.f0 = (found.y - x.kvh * per_head) * p.tile_rows;
+    x.tile = found.z * least + min(found.z, more);
+    x.tiles = least + (found.z < more ? 1 : 0);
+    x.share = found.w < 0 ? -1 : found.w + found.z;
+}
 
 template <typename T> __device__ __forceinline__ T out_of(float x);
 template <> __device__ __forceinline__ float out_of<float>(float x) { return x; }
 template <> __device__ __forceinline__ __nv_bfloat16 out_of<__nv_bfloat16>(float x) { return __float2bfloat16_rn(x); }      // the one rounding of the result
 
+// What a finished segment's row becomes: its share, or the result, which is out = o / l with the sink's part in l.
+__device__ __forceinline__ float tree_inverse(const TreeAttnArgs& a, int h, float m, float l) {
+    if (!a.sinks) return l > 0.0f ? 1.0f / l : l;    // (undefined stays undefined)
+    const float sink = a.sinks[h] * kLog2e, top = fmaxf(m, sink), c = m == -INFINITY ? 0.0f : exp2f(m - top);
+    const float sum = l * c + exp2f(sink - top);
+    return sum > 0.0f ? c / sum : sum;
+}
+
 // ---- products on CUDA cores, in 32 bits: an f32 cache
-// CTA = chunk x (K/V head, 32 query rows) x sequence; 8 warps of 4 query rows.  32 keys at a time lie in shared memory as f32: a lane multiplies its key with
-// the warp's four rows, and then four (two) dimensions of the values with their weights.
+// A unit has 32 query rows; 8 warps of 4 query rows.  32 keys at a time lie in shared memory as f32: a lane multiplies its key with the warp's four rows, and
+// then four (two) dimensions of the values with their weights.
 constexpr int kRowsTile = 32, kRowsKeys = 32;
 template <int HD>
-constexpr int rows_smem() { return (kRowsTile * HD + kRowsKeys * (HD + 4) + kRowsKeys * HD + kRowsTile * kRowsKeys) * 4 + (int)sizeof(TreeNodes); }
+constexpr int rows_smem() { return (kRowsTile * HD + kRowsKeys * (HD + 4) + kRowsKeys * HD + kRowsTile * kRowsKeys) * 4 + 32 + (int)sizeof(TreeNodes); }
 
 template <int HD>
-__global__ void __launch_bounds__(256) attn_tree_rows(const TreeAttnArgs a, const Part part) {
+__global__ void __launch_bounds__(256) attn_tree_rows(const TreeAttnArgs a, const Share part) {
     extern __shared__ __align__(16) unsigned char smem[];
     float* s_q = (float*)smem;                       // [32][HD]
     float* s_k = s_q + kRowsTile * HD;               // [32][HD + 4]
     float* s_v = s_k + kRowsKeys * (HD + 4);         // [32][HD]
     float* s_p = s_v + kRowsKeys * HD;               // [32 rows][32 keys]
-    TreeNodes& tree = *(TreeNodes*)(s_p + kRowsTile * kRowsKeys);
+    int* s_piece = (int*)(s_p + kRowsTile * kRowsKeys);
+    TreeNodes& tree = *(TreeNodes*)(s_piece + 8);
     constexpr int DPL = HD / 32;
-    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, chunk = blockIdx.x, s = blockIdx.z, G = a.n_q / a.n_kv;
-    const int kvh = blockIdx.y % a.n_kv, f0 = blockIdx.y / a.n_kv * kRowsTile;
-    TreeSeq q;
-    if (!tree_seq(a.t, &a.m, s, &q, a.status) || f0 >= q.n * G) return;
-    const TreeWork w = tree_work(q.prefix, q.n, a.window);
-    if (chunk * part.tiles >= w.n_tiles) return;
-    tree_load(tree, a.t, q, a.window, tid, 256, 0, a.status);
-    for (int x = tid; x < kRowsTile * HD / 4; x += 256) {
-        const int r = x / (HD / 4), c = x % (HD / 4) * 4, f = f0 + r;
-        float4 v = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-        if (f < q.n * G) v = *(const float4*)((const float*)a.q + (size_t)(q.r0 + f / G) * a.q_stride + ((size_t)kvh * G + f % G) * HD + c);
-        *(float4*)(s_q + r * HD + c) = v;
+    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, G = a.n_q / a.n_kv;
+    if (warp == 0) {
+        int per;
+        const int4 found = piece_find(a, part, lane, &per);
+        if (lane == 0) { *(int4*)s_piece = found; s_piece[4] = per; }
     }
+    __syncthreads();
+    if (s_piece[0] < 0) return;
+    Piece x;
+    piece_load(a, part, *(int4*)s_piece, s_piece[4], x);
     const float scale = a.scale * kLog2e;
-    float o[4][DPL], mx[4], l[4];
-    int node[4];
-#pragma unroll
-    for (int r = 0; r < 4; r++) {
-        mx[r] = -INFINITY; l[r] = 0.0f;
-        const int f = f0 + warp * 4 + r;
-        node[r] = f < q.n * G ? f / G : -1;
-#pragma unroll
-        for (int i = 0; i < DPL; i++) o[r][i] = 0.0f;
-    }
-    const int j_first = (w.t_lo + chunk * part.tiles) * kTileKeys, j_end = min(w.n_keys, j_first + part.tiles * kTileKeys);
-#pragma unroll 1
-    for (int j0 = j_first; j0 < j_end; j0 += kRowsKeys) {
-        __syncthreads();                             // (the tree and the queries are there; the tile before has been read)
-        for (int x = tid; x < kRowsKeys * HD / 4; x += 256) {
-            const int r = x / (HD / 4), c = x % (HD / 4) * 4, j = j0 + r;
-            float4 kf = make_float4(0.0f, 0.0f, 0.0f, 0.0f), vf = kf;
-            const long long at = j >= w.low && j < j_end ? tree_row(a.m, q.slot, j, a.status) : -1;
-            if (at >= 0) {
-                const size_t off = (size_t)at * a.kv_stride + (size_t)kvh * HD + c;
-                kf = *(const float4*)((const float*)a.k + off);
-                vf = *(const float4*)((const float*)a.v + off);
-            }
-            *(float4*)(s_k + r * (HD + 4) + c) = kf;
-            *(float4*)(s_v + r * HD + c) = vf;
+    {
+        const TreeSeq& q = x.q;
+        const TreeWork& w = x.w;
+        tree_load(tree, a.t, q, a.window, tid, 256, 0, a.status);
+        for (int e = tid; e < kRowsTile * HD / 4; e += 256) {
+            const int r = e / (HD / 4), c = e % (HD / 4) * 4, f = x.f0 + r;
+            float4 v = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+            if (f < q.n * G) v = *(const float4*)((const float*)a.q + (size_t)(q.r0 + f / G) * a.q_stride + ((size_t)x.kvh * G + f % G) * HD + c);
+            *(float4*)(s_q + r * HD + c) = v;
         }
-        __syncthreads();
-        float x[4] = {0.0f, 0.0f, 0.0f, 0.0f};
-        const float* qr = s_q + warp * 4 * HD;
-#pragma unroll 8
-        for (int c = 0; c < HD; c += 4) {
-            const float4 k4 = *(const float4*)(s_k + lane * (HD + 4) + c);
-#pragma unroll
-            for (int r = 0; r < 4; r++) {
-                const float4 q4 = *(const float4*)(qr + r * HD + c);
-                x[r] = fmaf(q4.x, k4.x, fmaf(q4.y, k4.y, fmaf(q4.z, k4.z, fmaf(q4.w, k4.w, x[r]))));
-            }
-        }
-        const int j = j0 + lane;
-        const bool live = j >= w.low && j < j_end;
-        unsigned int vis[4], all = 0xffffffffu;
+        float o[4][DPL], mx[4], l[4];
+        int node[4];
 #pragma unroll
         for (int r = 0; r < 4; r++) {
-            const bool see = live && node[r] >= 0 && tree_sees(tree, q, a.window, node[r], j);
-            vis[r] = __ballot_sync(0xffffffffu, see);
-            all &= vis[r];
-            const float y = see ? x[r] * scale : -INFINITY;
-            float top = y;
+            mx[r] = -INFINITY; l[r] = 0.0f;
+            const int f = x.f0 + warp * 4 + r;
+            node[r] = f < q.n * G ? f / G : -1;
 #pragma unroll
-            for (int i = 16; i > 0; i >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, i));
-            const float mn = fmaxf(mx[r], top);
-            const float p = see ? exp2f(y - (mn == -INFINITY ? 0.0f : mn)) : 0.0f;
-            const float corr = mx[r] == mn ? 1.0f : exp2f(mx[r] - mn);
-            l[r] = l[r] * corr + p;
-            mx[r] = mn;
-#pragma unroll
-            for (int i = 0; i < DPL; i++) o[r][i] *= corr;
-            s_p[(warp * 4 + r) * kRowsKeys + lane] = p;
+            for (int i = 0; i < DPL; i++) o[r][i] = 0.0f;
         }
-        __syncwarp();
-        // a key that a row does not see adds nothing to it, whatever its value holds (0 times infinity is no zero)
-#pragma unroll 4
-        for (int key = 0; key < kRowsKeys; key++) {
-            float v[DPL];
+        const int j_first = (w.t_lo + x.tile) * kTileKeys, j_end = min(w.n_keys, j_first + x.tiles * kTileKeys);
+#pragma unroll 1
+        for (int j0 = j_first; j0 < j_end; j0 += kRowsKeys) {
+            __syncthreads();                         // (the tree and the queries are there; the tile before has been read)
+            for (int e = tid; e < kRowsKeys * HD / 4; e += 256) {
+                const int r = e / (HD / 4), c = e % (HD / 4) * 4, j = j0 + r;
+                float4 kf = make_float4(0.0f, 0.0f, 0.0f, 0.0f), vf = kf;
+                const long long at = j >= w.low && j < j_end ? tree_row(a.m, q.slot, j, a.status) : -1;
+                if (at >= 0) {
+                    const size_t off = (size_t)at * a.kv_stride + (size_t)x.kvh * HD + c;
+                    kf = *(const float4*)((const float*)a.k + off);
+                    vf = *(const float4*)((const float*)a.v + off);
+                }
+                *(float4*)(s_k + r * (HD + 4) + c) = kf;
+                *(float4*)(s_v + r * HD + c) = vf;
+            }
+            __syncthreads();
+            float y[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+            const float* qr = s_q + warp * 4 * HD;
+#pragma unroll 8
+            for (int c = 0; c < HD; c += 4) {
+                const float4 k4 = *(const float4*)(s_k + lane * (HD + 4) + c);
 #pragma unroll
-            for (int i = 0; i < DPL; i++) v[i] = s_v[key * HD + lane * DPL + i];
-#pragma unroll
-            for (int r = 0; r < 4; r++) {
-                if (all == 0xffffffffu || (vis[r] >> key & 1u)) {
-                    const float p = s_p[(warp * 4 + r) * kRowsKeys + key];
-#pragma unroll
-                    for (int i = 0; i < DPL; i++) o[r][i] = fmaf(p, v[i], o[r][i]);
+                for (int r = 0; r < 4; r++) {
+                    const float4 q4 = *(const float4*)(qr + r * HD + c);
+                    y[r] = fmaf(q4.x, k4.x, fmaf(q4.y, k4.y, fmaf(q4.z, k4.z, fmaf(q4.w, k4.w, y[r]))));
                 }
             }
-        }
-        __syncwarp();
-    }
+            const int j = j0 + lane;
+            const bool live = j >= w.low && j < j_end;
+            unsigned int vis[4], all = 0xffffffffu;
 #pragma unroll
-    for (int r = 0; r < 4; r++) {
-        if (node[r] < 0) continue;
-        const int f = f0 + warp * 4 + r, row = q.r0 + node[r], h = kvh * G + f % G;
-        float sum = warp_sum(l[r]);
-        if (part.chunks == 1) {
-            float top = mx[r], c = 1.0f;
-            if (a.sinks) {
-                const float sink = a.sinks[h] * kLog2e;
-                top = fmaxf(top, sink);
-                c = mx[r] == -INFINITY ? 0.0f : exp2f(mx[r] - top);
-                sum = sum * c + exp2f(sink - top);
+            for (int r = 0; r < 4; r++) {
+                const bool see = live && node[r] >= 0 && tree_sees(tree, q, a.window, node[r], j);
+                vis[r] = __ballot_sync(0xffffffffu, see);
+                all &= vis[r];
+                const float z = see ? y[r] * scale : -INFINITY;
+                float top = z;
+#pragma unroll
+                for (int i = 16; i > 0; i >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, i));
+                const float mn = fmaxf(mx[r], top);
+                const float p = see ? exp2f(z - (mn == -INFINITY ? 0.0f : mn)) : 0.0f;
+                const float corr = mx[r] == mn ? 1.0f : exp2f(mx[r] - mn);
+                l[r] = l[r] * corr + p;
+                mx[r] = mn;
+#pragma unroll
+                for (int i = 0; i < DPL; i++) o[r][i] *= corr;
+                s_p[(warp * 4 + r) * kRowsKeys + lane] = p;
             }
-            const float inv = sum > 0.0f ? c / sum : sum;      // (undefined stays undefined)
-            float* dst = (float*)a.out + (size_t)row * a.out_stride + (size_t)h * HD + lane * DPL;
+            __syncwarp();
+            // a key that a row does not see adds nothing to it, whatever its value holds (0 times infinity is no zero)
+#pragma unroll 4
+            for (int key = 0; key < kRowsKeys; key++) {
+                float v[DPL];
 #pragma unroll
-            for (int i = 0; i < DPL; i++) dst[i] = o[r][i] * inv;
-        } else {
-            const size_t at = part_at(a, chunk, row, h);
+                for (int i = 0; i < DPL; i++) v[i] = s_v[key * HD + lane * DPL + i];
 #pragma unroll
-            for (int i = 0; i < DPL; i++) part.o[at * HD + lane * DPL + i] = o[r][i];
-            if (lane == 0) { part.ml[2 * at] = mx[r]; part.ml[2 * at + 1] = sum; }
+                for (int r = 0; r < 4; r++) {
+                    if (all == 0xffffffffu || (vis[r] >> key & 1u)) {
+                        const float p = s_p[(warp * 4 + r) * kRowsKeys + key];
+#pragma unroll
+                        for (int i = 0; i < DPL; i++) o[r][i] = fmaf(p, v[i], o[r][i]);
+                    }
+                }
+            }
+            __syncwarp();
+        }
+#pragma unroll
+        for (int r = 0; r < 4; r++) {
+            if (node[r] < 0) continue;
+            const int row = q.r0 + node[r], h = x.kvh * G + (x.f0 + warp * 4 + r) % G;
+            const float sum = warp_sum(l[r]);
+            if (x.share >= 0) {
+                const size_t at = share_at(part, x.share, warp * 4 + r);
+#pragma unroll
+                for (int i = 0; i < DPL; i++) part.o[at * HD + lane * DPL + i] = o[r][i];
+                if (lane == 0) { part.ml[2 * at] = mx[r]; part.ml[2 * at + 1] = sum; }
+            } else {
+                const float inv = tree_inverse(a, h, mx[r], sum);
+                float* dst = (float*)a.out + (size_t)row * a.out_stride + (size_t)h * HD + lane * DPL;
+#pragma unroll
+                for (int i = 0; i < DPL; i++) dst[i] = o[r][i] * inv;
+            }
         }
     }
 }
@@ -221,13 +314,13 @@ __global__ void __launch_bounds__(256) attn_tree_rows(const TreeAttnArgs a, cons
 // A key that a row does not see has weight 0, but 0 times infinity is no zero: rows of V behind the last node or before the window are zeroed, and a row whose
 // result is not finite is computed again by tree_row_plain, key by key.
 constexpr int kTcThreads = 224;                     // four softmax warps, K, products, V
-constexpr int kTcGroup = 128 * 16 + 16;              // Q: 16-byte column groups of 128 rows, the next one 16 bytes further on (banks)
+constexpr int kTcGroup = 128 * 16 + 16;              // f32 queries' terms: 16-byte column groups of 128 rows, the next one 16 bytes further on (banks)
 template <int HD, bool F32>
 struct TcShape {
     static constexpr int q_terms = F32 ? 3 : 1, p_terms = F32 ? 3 : 2;
     static constexpr int tile = kTileKeys * HD * 2;  // bytes of K (or V)
-    static constexpr int q_bytes = HD / 8 * kTcGroup;
-    static constexpr int off_k = 0, off_v = 2 * tile, off_q = 4 * tile, off_misc = off_q + q_terms * q_bytes, off_tree = off_misc + 128 + 32 * 4;
+    static constexpr int q_bytes = F32 ? HD / 8 * kTcGroup : 128 * HD * 2;
+    static constexpr int off_k = 0, off_v = 2 * tile, off_q = 4 * tile, off_misc = off_q + q_terms * q_bytes, off_tree = off_misc + 144;
     static constexpr int smem = off_tree + (int)sizeof(TreeNodes);
     static constexpr int ctas = F32 && HD == 128 ? 1 : 2;                 // per SM
     static constexpr int cols = F32 && HD == 128 ? 512 : 256;             // tensor memory: scores 2 x 64, O, third terms 2 x 32
@@ -241,22 +334,30 @@ __device__ __forceinline__ void tc_mma_ts(uint32_t d, uint32_t a, uint64_t b, ui
     asm volatile("{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\ttcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}" ::"r"(d), "r"(a), "l"(b), "r"(idesc), "r"(accumulate) : "memory");
 }
 __device__ __forceinline__ uint64_t tc_desc_sw128(uint32_t addr, uint32_t lbo, uint32_t sbo) { return umma_smem_desc(addr, lbo, sbo) | (2ull << 61); }
-__device__ __forceinline__ void tc_ld32(uint32_t at, uint32_t* v) {
-    asm volatile("tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31}, [%32];"
-                 : "=r"(v[0]), "=r"(v[1]), "=r"(v[2]), "=r"(v[3]), "=r"(v[4]), "=r"(v[5]), "=r"(v[6]), "=r"(v[7]), "=r"(v[8]), "=r"(v[9]), "=r"(v[10]), "=r"(v[11]),
-                   "=r"(v[12]), "=r"(v[13]), "=r"(v[14]), "=r"(v[15]), "=r"(v[16]), "=r"(v[17]), "=r"(v[18]), "=r"(v[19]), "=r"(v[20]), "=r"(v[21]), "=r"(v[22]), "=r"(v[23]),
-                   "=r"(v[24]), "=r"(v[25]), "=r"(v[26]), "=r"(v[27]), "=r"(v[28]), "=r"(v[29]), "=r"(v[30]), "=r"(v[31])
+// N consecutive 32-bit columns of this thread's lane of tensor memory, by a whole warp
+template <int N> __device__ __forceinline__ void tc_ld(uint32_t at, uint32_t* v);
+template <int N> __device__ __forceinline__ void tc_st(uint32_t at, const uint32_t* v);
+template <> __device__ __forceinline__ void tc_ld<16>(uint32_t at, uint32_t* v) {
+    asm volatile("tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%16];"
+                 : "=r"(v[0]), "=r"(v[1]), "=r"(v[2]), "=r"(v[3]), "=r"(v[4]), "=r"(v[5]), "=r"(v[6]), "=r"(v[7]), "=r"(v[8]), "=r"(v[9]), "=r"(v[10]), "=r"(v[11]), "=r"(v[12]), "=r"(v[13]), "=r"(v[14]), "=r"(v[15])
                  : "r"(at) : "memory");
 }
-__device__ __forceinline__ void tc_st32(uint32_t at, const uint32_t* v) {
-    asm volatile("tcgen05.st.sync.aligned.32x32b.x32.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31,%32};"
-                 ::"r"(at), "r"(v[0]), "r"(v[1]), "r"(v[2]), "r"(v[3]), "r"(v[4]), "r"(v[5]), "r"(v[6]), "r"(v[7]), "r"(v[8]), "r"(v[9]), "r"(v[10]), "r"(v[11]),
-                 "r"(v[12]), "r"(v[13]), "r"(v[14]), "r"(v[15]), "r"(v[16]), "r"(v[17]), "r"(v[18]), "r"(v[19]), "r"(v[20]), "r"(v[21]), "r"(v[22]), "r"(v[23]),
-                 "r"(v[24]), "r"(v[25]), "r"(v[26]), "r"(v[27]), "r"(v[28]), "r"(v[29]), "r"(v[30]), "r"(v[31]) : "memory");
+template <> __device__ __forceinline__ void tc_ld<32>(uint32_t at, uint32_t* v) {
+    asm volatile("tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31}, [%32];"
+                 : "=r"(v[0]), "=r"(v[1]), "=r"(v[2]), "=r"(v[3]), "=r"(v[4]), "=r"(v[5]), "=r"(v[6]), "=r"(v[7]), "=r"(v[8]), "=r"(v[9]), "=r"(v[10]), "=r"(v[11]), "=r"(v[12]), "=r"(v[13]), "=r"(v[14]), "=r"(v[15]), "=r"(v[16]), "=r"(v[17]), "=r"(v[18]), "=r"(v[19]), "=r"(v[20]), "=r"(v[21]), "=r"(v[22]), "=r"(v[23]), "=r"(v[24]), "=r"(v[25]), "=r"(v[26]), "=r"(v[27]), "=r"(v[28]), "=r"(v[29]), "=r"(v[30]), "=r"(v[31])
+                 : "r"(at) : "memory");
 }
-__device__ __forceinline__ void tc_st16(uint32_t at, const uint32_t* v) {
-    asm volatile("tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16};" ::"r"(at), "r"(v[0]), "r"(v[1]), "r"(v[2]), "r"(v[3]),
-                 "r"(v[4]), "r"(v[5]), "r"(v[6]), "r"(v[7]), "r"(v[8]), "r"(v[9]), "r"(v[10]), "r"(v[11]), "r"(v[12]), "r"(v[13]), "r"(v[14]), "r"(v[15]) : "memory");
+template <> __device__ __forceinline__ void tc_st<8>(uint32_t at, const uint32_t* v) {
+    asm volatile("tcgen05.st.sync.aligned.32x32b.x8.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8};" ::"r"(at), "r"(v[0]), "r"(v[1]), "r"(v[2]), "r"(v[3]), "r"(v[4]), "r"(v[5]), "r"(v[6]), "r"(v[7])
+                 : "memory");
+}
+template <> __device__ __forceinline__ void tc_st<16>(uint32_t at, const uint32_t* v) {
+    asm volatile("tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16};" ::"r"(at), "r"(v[0]), "r"(v[1]), "r"(v[2]), "r"(v[3]), "r"(v[4]), "r"(v[5]), "r"(v[6]), "r"(v[7]), "r"(v[8]), "r"(v[9]), "r"(v[10]), "r"(v[11]), "r"(v[12]), "r"(v[13]), "r"(v[14]), "r"(v[15])
+                 : "memory");
+}
+template <> __device__ __forceinline__ void tc_st<32>(uint32_t at, const uint32_t* v) {
+    asm volatile("tcgen05.st.sync.aligned.32x32b.x32.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31,%32};" ::"r"(at), "r"(v[0]), "r"(v[1]), "r"(v[2]), "r"(v[3]), "r"(v[4]), "r"(v[5]), "r"(v[6]), "r"(v[7]), "r"(v[8]), "r"(v[9]), "r"(v[10]), "r"(v[11]), "r"(v[12]), "r"(v[13]), "r"(v[14]), "r"(v[15]), "r"(v[16]), "r"(v[17]), "r"(v[18]), "r"(v[19]), "r"(v[20]), "r"(v[21]), "r"(v[22]), "r"(v[23]), "r"(v[24]), "r"(v[25]), "r"(v[26]), "r"(v[27]), "r"(v[28]), "r"(v[29]), "r"(v[30]), "r"(v[31])
+                 : "memory");
 }
 __device__ __forceinline__ void tc_st_wait() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
 __device__ __forceinline__ float tc_ex2(float x) { float y; asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x)); return y; }
@@ -283,6 +384,11 @@ __device__ __forceinline__ uint32_t tc_term(float* x0, float* x1) {
 }
 __device__ __forceinline__ void tma_box(uint32_t dst, const CUtensorMap* map, int row, int col, uint32_t bar) {
     asm volatile("cp.async.bulk.tensor.3d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4}], [%5];" ::"r"(dst), "l"(map), "r"(0), "r"(row), "r"(col), "r"(bar) : "memory");
+}
+
+__device__ __forceinline__ void tma_queries(uint32_t dst, const CUtensorMap* map, int head, int row, int half, uint32_t bar) {
+    asm volatile("cp.async.bulk.tensor.4d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4, %5}], [%6];" ::"r"(dst), "l"(map), "r"(0), "r"(head), "r"(row), "r"(half),
+                 "r"(bar) : "memory");
 }
 
 // One query row (f of its K/V head) over cache rows [j0, j1) by a warp, in f32 and key by key: (m, l) in every lane, out[i] = dimension lane * HD / 32 + i.
@@ -314,30 +420,20 @@ __device__ __noinline__ void tree_row_plain(const TreeAttnArgs& a, const TreeNod
 #pragma unroll
     for (int i = 0; i < DPL; i++) out[i] = o[i];
 }
-// A finished row of a call with one chunk: 1 / l and the sink's share.
-__device__ __forceinline__ float tree_inverse(const TreeAttnArgs& a, int h, float m, float l) {
-    if (!a.sinks) return l > 0.0f ? 1.0f / l : l;    // (undefined stays undefined)
-    const float sink = a.sinks[h] * kLog2e, top = fmaxf(m, sink), c = m == -INFINITY ? 0.0f : exp2f(m - top);
-    const float sum = l * c + exp2f(sink - top);
-    return sum > 0.0f ? c / sum : sum;
-}
-
-template <int HD, bool F32>
-__global__ void __launch_bounds__(kTcThreads, TcShape<HD, F32>::ctas) attn_tree_tc(const __grid_constant__ TreeAttnArgs a, const Part part, const __grid_constant__ CUtensorMap map_k,
-                                                                                   const __grid_constant__ CUtensorMap map_v, int box_rows) {
+template <int HD, bool F32, int DUP>
+__global__ void __launch_bounds__(kTcThreads, TcShape<HD, F32>::ctas) attn_tree_tc(const __grid_constant__ TreeAttnArgs a, const __grid_constant__ Share part, const __grid_constant__ CUtensorMap map_q,
+                                                                                   const __grid_constant__ CUtensorMap map_k, const __grid_constant__ CUtensorMap map_v, int box_rows) {
     using S = TcShape<HD, F32>;
     using TQ = typename std::conditional<F32, float, __nv_bfloat16>::type;
     extern __shared__ __align__(1024) unsigned char tc_smem[];
-    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, chunk = blockIdx.x, s = blockIdx.z, G = a.n_q / a.n_kv;
-    const int kvh = blockIdx.y % a.n_kv, f0 = blockIdx.y / a.n_kv * 128;
+    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, G = a.n_q / a.n_kv;
     const uint32_t base = smem_u32(tc_smem), misc = base + S::off_misc;
-    const uint32_t bar_k = misc, bar_v = misc + 16, bar_s = misc + 32, bar_p = misc + 48, bar_o = misc + 64;      // two of each: tile t uses number t % 2
-    volatile int* gave_up = (volatile int*)(tc_smem + S::off_misc + 88);
-    unsigned int* s_odd = (unsigned int*)(tc_smem + S::off_misc + 96);       // [4]: rows whose result is not finite
+    const uint32_t bar_k = misc, bar_v = misc + 16, bar_s = misc + 32, bar_p = misc + 48, bar_o = misc + 64, bar_q = misc + 80;      // two of each (queries: one): tile t uses number t % 2
+    volatile int* gave_up = (volatile int*)(tc_smem + S::off_misc + 104);
+    int* s_piece = (int*)(tc_smem + S::off_misc + 112);
     TreeNodes& tree = *(TreeNodes*)(tc_smem + S::off_tree);
-    if (part.chunks > 1) pdl_launch_dependents();    // (tree_combine waits for this kernel's end)
-    TreeSeq q = tree_seq_load(a.t, s);               // on its way while the CTA sets itself up
-    if (tid == 0) {
+    pdl_launch_dependents();                         // (tree_combine waits for this kernel's end)
+    if (tid == 32) {
         for (int i = 0; i < 2; i++) {
             mbar_init(bar_k + 8 * i, 1);             // K(t) has landed
             mbar_init(bar_v + 8 * i, 1);             // V(t)
@@ -345,25 +441,29 @@ __global__ void __launch_bounds__(kTcThreads, TcShape<HD, F32>::ctas) attn_tree_
             mbar_init(bar_p + 8 * i, 4);             // P(t) is stored, O may be added to
             mbar_init(bar_o + 8 * i, 1);             // O holds tile t, V(t) is no longer read
         }
+        mbar_init(bar_q, F32 ? 4 : 1);               // the queries are there
         mbar_fence_init();
         *gave_up = 0;
     }
-    if (tid < 4) s_odd[tid] = 0u;
-    if (warp == 5) tmem_alloc(misc + 80, S::cols);
+    if (warp == 0) {
+        int per;
+        const int4 found = piece_find(a, part, lane, &per);
+        if (lane == 0) { *(int4*)s_piece = found; s_piece[4] = per; }
+    }
+    if (warp == 5) tmem_alloc(misc + 96, S::cols);
     tc_fence_before_sync();
     __syncthreads();
     tc_fence_after_sync();
-    const uint32_t tmem = *(volatile uint32_t*)(tc_smem + S::off_misc + 80);
-    const bool ok = tree_seq_ok(a.t, &a.m, &q, a.status);
-    const TreeWork w = tree_work(q.prefix, q.n, a.window);
-    const int t_first = w.t_lo + chunk * part.tiles, n_tiles = min(part.tiles, w.t_lo + w.n_tiles - t_first);
-    if (!ok || f0 >= q.n * G || n_tiles <= 0) {
+    const uint32_t tmem = *(volatile uint32_t*)(tc_smem + S::off_misc + 96);
+    if (s_piece[0] < 0) {
         if (warp == 5) tmem_dealloc(tmem, S::cols);
         return;
     }
-    const int live_rows = min(128, q.n * G - f0);
-    const uint32_t magic = 0xffffffffu / (uint32_t)G + 1u;               // f / G = f magic / 2^32 for f < 2^18, 2 <= G <= 2^10
-    auto node_of = [&](int f) { return G == 1 ? f : (int)__umulhi((uint32_t)f, magic); };
+    Piece x;
+    piece_load(a, part, *(int4*)s_piece, s_piece[4], x);
+    const TreeSeq q = x.q;
+    const TreeWork w = x.w;
+    const int t_first = w.t_lo + x.tile, n_tiles = x.tiles, kvh = x.kvh, f0 = x.f0;
 
     // A wait that runs out of its budget is remembered; what follows hardly waits and multiplies no more, but meets every barrier.
     auto wait = [&](uint32_t bar, int t) {
@@ -372,175 +472,177 @@ __global__ void __launch_bounds__(kTcThreads, TcShape<HD, F32>::ctas) attn_tree_
         if (!mbar_wait_abortable(at, parity, gave_up)) *gave_up = 1;
     };
     constexpr int kHalves = HD / 64;
-    // Where this lane's box of tile t starts in the cache (a lane per box); one page-table entry on its way while the tile before is waited for.
-    auto box_row = [&](int t) {
-        const int j = (t_first + t) * kTileKeys + lane * box_rows;
-        if (t >= n_tiles || lane >= kTileKeys / box_rows || j >= w.n_keys || j + box_rows <= w.low) return (int)a.m.rows;     // outside the tensor: zeros
-        const long long row = tree_row(a.m, q.slot, j, a.status);
-        return (int)(row < 0 ? a.m.rows : row);
-    };
-    auto load = [&](const CUtensorMap* map, int t, int row, uint32_t dst, uint32_t full) {
-        const uint32_t bar = full + 8u * (t & 1);
-        dst += (uint32_t)(t & 1) * S::tile;
-        if (lane == 0) mbar_arrive_expect_tx(bar, S::tile);
-        __syncwarp();
-        // a box holds its halves of 64 dimensions one behind the other; a whole tile's are kTileKeys rows apart
-        if (box_rows == kTileKeys) { if (elect_one()) tma_box(dst, map, row, kvh * kHalves, bar); }
-        else if (lane < kTileKeys / box_rows)
-#pragma unroll
-            for (int h = 0; h < kHalves; h++) tma_box(dst + h * (kTileKeys * 128) + lane * box_rows * 128, map, row, kvh * kHalves + h, bar);
-    };
-    const bool loads_k = warp == 4, loads = loads_k || warp == 6;
-    int next_row = 0;
-    if (loads) {
-        const int first = box_row(0);
-        const int second = box_row(1);
-        next_row = box_row(2);
-        load(loads_k ? &map_k : &map_v, 0, first, base + (loads_k ? S::off_k : S::off_v), loads_k ? bar_k : bar_v);
-        if (n_tiles > 1) load(loads_k ? &map_k : &map_v, 1, second, base + (loads_k ? S::off_k : S::off_v), loads_k ? bar_k : bar_v);
-    }
-    // ---- the tree, by the warps that then only issue; the queries, by the others
-    if (loads) {
-        tree_load(tree, a.t, q, a.window, (warp == 6 ? 32 : 0) + lane, 64, 1, a.status);
-        named_arrive(3, 192);
-    } else if (warp < 4) {
-        // (rows beyond the last query are left as they are: nobody reads what they make)
-        constexpr int kPieces = HD / 8, kStep = 128 / kPieces, kAhead = F32 ? 2 : 4;
-        const int c = tid % kPieces;
-        for (int r0 = tid / kPieces; r0 < live_rows; r0 += kStep * kAhead) {
-            uint4 raw[kAhead][F32 ? 2 : 1];
-#pragma unroll
-            for (int u = 0; u < kAhead; u++) {
-                const int f = f0 + min(r0 + u * kStep, live_rows - 1), node = node_of(f);
-                const uint4* src = (const uint4*)((const TQ*)a.q + (size_t)(q.r0 + node) * a.q_stride + ((size_t)kvh * G + f - node * G) * HD + c * 8);
-#pragma unroll
-                for (int e = 0; e < (F32 ? 2 : 1); e++) raw[u][e] = src[e];
-            }
-#pragma unroll
-            for (int u = 0; u < kAhead; u++) {
-                const int r = r0 + u * kStep;
-                if (r >= live_rows) break;
-                unsigned char* dst = tc_smem + S::off_q + c * kTcGroup + r * 16;
-                if constexpr (F32) {
-                    float* y = (float*)raw[u];
-#pragma unroll
-                    for (int e = 0; e < 3; e++) *(uint4*)(dst + e * S::q_bytes) = make_uint4(tc_term(y, y + 1), tc_term(y + 2, y + 3), tc_term(y + 4, y + 5), tc_term(y + 6, y + 7));
-                } else *(uint4*)dst = raw[u][0];
-            }
-        }
-        fence_proxy_async_smem();
-        named_arrive(2, 160);
-    } else named_sync(2, 160);                       // (the queries are there)
-
-    float m_run = -INFINITY, l_run = 0.0f;
-    float o[F32 ? HD : 1];
-    const uint32_t mine = tmem + ((uint32_t)((warp & 3) * 32) << 16);
-    const int row = warp * 32 + lane, f = f0 + row, node = row < live_rows && warp < 4 ? node_of(f) : -1;
-    if (loads) {
-        // K(t + 2) goes out when S(t) is there, V(t + 2) when O holds tile t
-        const CUtensorMap* map = loads_k ? &map_k : &map_v;
-        const uint32_t dst = base + (loads_k ? S::off_k : S::off_v), full = loads_k ? bar_k : bar_v, used = loads_k ? bar_s : bar_o;
-        int last = min(n_tiles, 2) - 1;
-        for (int t = 2; t < n_tiles; t++) {
-            const int row = next_row;
-            next_row = box_row(t + 1);
-            wait(used, t - 2);
+    if (warp == 4 || warp == 6) {
+        // ---- keys (warp 4) or values (warp 6): K(t + 2) goes out when S(t) is there, V(t + 2) when O holds tile t
+        const bool keys = warp == 4;
+        const CUtensorMap* map = keys ? &map_k : &map_v;
+        const uint32_t dst0 = base + (keys ? S::off_k : S::off_v), full = keys ? bar_k : bar_v, used = keys ? bar_s : bar_o;
+        int last = -1;
+        // Where this lane's box of tile t starts in the cache (a lane per box); a page-table entry is on its way while the tile before is waited for.
+        auto box_row = [&](int t) {
+            const int j = (t_first + t) * kTileKeys + lane * box_rows;
+            if (t >= n_tiles || lane >= kTileKeys / box_rows || j >= w.n_keys || j + box_rows <= w.low) return (int)a.m.rows;     // outside the tensor: zeros
+            const long long row = tree_row(a.m, q.slot, j, a.status);
+            return (int)(row < 0 ? a.m.rows : row);
+        };
+        int next = box_row(0);
+        for (int t = 0; t < n_tiles; t++) {
+            const int row = next;
+            next = box_row(t + 1);
+            if (t > 1) wait(used, t - 2);
             if (__any_sync(0xffffffffu, *gave_up)) break;
-            load(map, last = t, row, dst, full);
+            const uint32_t bar = full + 8u * (t & 1), dst = dst0 + (uint32_t)(t & 1) * S::tile;
+            if (lane == 0) mbar_arrive_expect_tx(bar, S::tile);
+            __syncwarp();
+            // a box holds its halves of 64 dimensions one behind the other; a whole tile's are kTileKeys rows apart
+            if (box_rows == kTileKeys) { if (elect_one()) tma_box(dst, map, row, kvh * kHalves, bar); }
+            else if (lane < kTileKeys / box_rows)
+#pragma unroll
+                for (int h = 0; h < kHalves; h++) tma_box(dst + h * (kTileKeys * 128) + lane * box_rows * 128, map, row, kvh * kHalves + h, bar);
+            last = t;
         }
         // no copy is on its way when the CTA ends (they have landed long ago, unless a wait was given up)
         for (int t = max(last - 1, 0); t <= last; t++) mbar_wait(full + 8u * (t & 1), (uint32_t)(t >> 1) & 1u);
     } else if (warp == 5) {
+        // ---- the products (and the copy of bf16 queries: the unit's nodes, their heads of this K/V head, in the order of the operand's rows)
         constexpr uint32_t id_s = tc_idesc(kTileKeys, false), id_o = tc_idesc(HD, true);
         if (elect_one()) {
+            if constexpr (!F32) {
+                mbar_arrive_expect_tx(bar_q, (uint32_t)part.tile_rows * 128u * kHalves * DUP);
+#pragma unroll
+                for (int h = 0; h < kHalves; h++)
+#pragma unroll
+                    for (int d = 0; d < DUP; d++) tma_queries(base + S::off_q + h * (128 * 128) + d * (128 / DUP * 128), &map_q, kvh * G, q.r0 + f0 / G, h, bar_q);
+            }
+            wait(bar_q, 0);
 #pragma unroll 1
             for (int t = 0; t <= n_tiles; t++) {
                 if (t < n_tiles) {
+                    const int b = t & 1;
                     wait(bar_k, t);
                     if (*gave_up) break;
                     tc_fence_after_sync();
-                    const uint32_t kb = base + S::off_k + (t & 1) * S::tile, d = tmem + (uint32_t)(t & 1) * 64u;
+                    const uint32_t kb = base + S::off_k + b * S::tile, d = tmem + (uint32_t)b * 64u;
 #pragma unroll
                     for (int e = S::q_terms - 1; e >= 0; e--)
 #pragma unroll
                         for (int ks = 0; ks < HD / 16; ks++)
-                            tc_mma(d, umma_smem_desc(base + S::off_q + e * S::q_bytes + ks * 2 * kTcGroup, kTcGroup, 128), tc_desc_sw128(kb + (ks >> 2) * (kTileKeys * 128) + (ks & 3) * 32, 16, 1024),
-                                   id_s, e != S::q_terms - 1 || ks ? 1u : 0u);
-                    umma_commit(bar_s + 8u * (t & 1));
+                            tc_mma(d, F32 ? umma_smem_desc(base + S::off_q + e * S::q_bytes + ks * 2 * kTcGroup, kTcGroup, 128) : tc_desc_sw128(base + S::off_q + (ks >> 2) * (128 * 128) + (ks & 3) * 32, 16, 1024),
+                                   tc_desc_sw128(kb + (ks >> 2) * (kTileKeys * 128) + (ks & 3) * 32, 16, 1024), id_s, e != S::q_terms - 1 || ks ? 1u : 0u);
+                    umma_commit(bar_s + 8u * b);
                 }
                 if (t > 0) {
-                    const int u = t - 1;
+                    const int u = t - 1, b = u & 1;
                     wait(bar_v, u);
                     wait(bar_p, u);
                     if (*gave_up) break;
                     tc_fence_after_sync();
-                    const uint32_t vb = base + S::off_v + (u & 1) * S::tile, p = tmem + (uint32_t)(u & 1) * 64u, px = tmem + S::col_x + (uint32_t)(u & 1) * 32u, d = tmem + S::col_o;
+                    const uint32_t vb = base + S::off_v + b * S::tile, p = tmem + (uint32_t)b * 64u, px = tmem + S::col_x + (uint32_t)b * 32u, d = tmem + S::col_o;
 #pragma unroll
                     for (int e = S::p_terms - 1; e >= 0; e--)
 #pragma unroll
                         for (int ks = 0; ks < kTileKeys / 16; ks++)
                             tc_mma_ts(d, (e == 2 ? px : p + e * 32u) + ks * 8u, tc_desc_sw128(vb + ks * 2048, kTileKeys * 128, 1024), id_o, (!F32 && u) || e != S::p_terms - 1 || ks ? 1u : 0u);
-                    umma_commit(bar_o + 8u * (u & 1));
+                    umma_commit(bar_o + 8u * b);
                 }
             }
+            if constexpr (!F32) mbar_wait(bar_q, 0);     // (landed long ago, unless a wait was given up)
         }
         __syncwarp();
     } else {
+        // ---- softmax
+        constexpr int KPT = kTileKeys / DUP;         // keys per thread and tile
+        const float scale = a.scale * kLog2e;
+        const uint32_t mine = tmem + ((uint32_t)(warp * 32) << 16);
+        const uint32_t magic = 0xffffffffu / (uint32_t)G + 1u;           // f / G = f magic / 2^32 for f < 2^18, 2 <= G <= 2^10
+        auto node_of = [&](int f) { return G == 1 ? f : (int)__umulhi((uint32_t)f, magic); };
+        const int live_rows = min(part.tile_rows, q.n * G - f0);
+        if constexpr (F32) {                         // three terms of the queries (rows beyond the last one are left as they are: nobody reads what they make)
+            constexpr int kPieces = HD / 8, kStep = 128 / kPieces, kAhead = 4;
+            const int c = tid % kPieces;
+            for (int r0 = tid / kPieces; r0 < live_rows; r0 += kStep * kAhead) {
+                uint4 raw[kAhead][2];
+#pragma unroll
+                for (int u = 0; u < kAhead; u++) {
+                    const int f = f0 + min(r0 + u * kStep, live_rows - 1), node = node_of(f);
+                    const uint4* src = (const uint4*)((const float*)a.q + (size_t)(q.r0 + node) * a.q_stride + ((size_t)kvh * G + f - node * G) * HD + c * 8);
+                    raw[u][0] = src[0]; raw[u][1] = src[1];
+                }
+#pragma unroll
+                for (int u = 0; u < kAhead; u++) {
+                    const int r = r0 + u * kStep;
+                    if (r >= live_rows) break;
+                    float* y = (float*)raw[u];
+#pragma unroll
+                    for (int e = 0; e < 3; e++) {
+                        const uint4 t = make_uint4(tc_term(y, y + 1), tc_term(y + 2, y + 3), tc_term(y + 4, y + 5), tc_term(y + 6, y + 7));
+#pragma unroll
+                        for (int d = 0; d < DUP; d++) *(uint4*)(tc_smem + S::off_q + e * S::q_bytes + c * kTcGroup + (d * (128 / DUP) + r) * 16) = t;
+                    }
+                }
+            }
+            fence_proxy_async_smem();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(bar_q);
+        }
+        // the tree, where the piece reaches it (with a window every tile may be cut)
+        if (a.window > 0 || (t_first + n_tiles) * kTileKeys > q.prefix) {
+            tree_load(tree, a.t, q, a.window, tid, 128, 1, a.status);
+            named_sync(1, 128);
+        }
+        const int grp = warp / (4 / DUP), warp_row = warp % (4 / DUP) * 32, row = warp_row + lane, f = f0 + row, node = row < live_rows ? node_of(f) : -1;
+        const bool live = warp_row < live_rows;      // a warp without live rows leaves its rows of P as they are: nobody reads what they make
+        float m_run = -INFINITY, l_run = 0.0f;
+        float o[F32 ? HD : 1];
         if constexpr (F32)
 #pragma unroll
             for (int i = 0; i < HD; i++) o[i] = 0.0f;
-        const float scale = a.scale * kLog2e;
-        auto zero_v = [&](int t) {                   // rows of V(t) that no query row may see
-            const int j0 = (t_first + t) * kTileKeys;
-            if (j0 >= w.low && j0 + kTileKeys <= w.n_keys) return;
-            wait(bar_v, t);
-            unsigned char* vb = tc_smem + S::off_v + (t & 1) * S::tile;
-            for (int x = tid; x < kTileKeys * (HD / 8); x += 128) {
-                const int j = x / (HD / 8), c = x % (HD / 8);
-                if (j0 + j < w.low || j0 + j >= w.n_keys) *(uint4*)(vb + (c >> 3) * (kTileKeys * 128) + j * 128 + (c & 7) * 16) = make_uint4(0u, 0u, 0u, 0u);
-            }
-            fence_proxy_async_smem();
-        };
 #pragma unroll 1
         for (int t = 0; t < n_tiles; t++) {
+            const int b = t & 1, j0 = (t_first + t) * kTileKeys;
             if (t > 1) wait(bar_o, t - 2);           // (long there: every phase of bar_o is seen, and V(t - 2) has been used)
-            zero_v(t);
+            if (j0 < w.low || j0 + kTileKeys > w.n_keys) {           // rows of V that no query row may see
+                wait(bar_v, t);
+                unsigned char* vb = tc_smem + S::off_v + b * S::tile;
+                for (int e = tid; e < kTileKeys * (HD / 8); e += 128) {
+                    const int j = e / (HD / 8), c = e % (HD / 8);
+                    if (j0 + j < w.low || j0 + j >= w.n_keys) *(uint4*)(vb + (c >> 3) * (kTileKeys * 128) + j * 128 + (c & 7) * 16) = make_uint4(0u, 0u, 0u, 0u);
+                }
+                fence_proxy_async_smem();
+            }
             wait(bar_s, t);
             tc_fence_after_sync();
-            if (t == 0) named_sync(3, 192);          // (the tree is there)
-            if (warp * 32 < live_rows) {             // (a warp without live rows leaves its rows of P as they are: nobody reads what they make)
-                const uint32_t sc = mine + (uint32_t)(t & 1) * 64u;
-                float v[64];
-                tc_ld32(sc, (uint32_t*)v);
-                tc_ld32(sc + 32u, (uint32_t*)v + 32);
+            if (live) {
+                const uint32_t sc = mine + (uint32_t)b * 64u;
+                float v[KPT];
+#pragma unroll
+                for (int c = 0; c < KPT; c += KPT < 32 ? KPT : 32) tc_ld<(KPT < 32 ? KPT : 32)>(sc + grp * KPT + c, (uint32_t*)v + c);
                 tmem_ld_wait();
-                const int j0 = (t_first + t) * kTileKeys;
-                if (j0 + kTileKeys > q.prefix || a.window > 0) {         // some key may be out of some row's sight
+                if (j0 + kTileKeys > q.prefix || a.window > 0) {     // some key may be out of some row's sight
                     unsigned long long see = 0ull;
                     if (node >= 0) {
-                        const int cached = q.prefix - j0;                // keys of the tile before the tree
+                        const int cached = q.prefix - j0;            // keys of the tile before the tree
                         see = cached >= 64 ? ~0ull : cached > 0 ? (1ull << cached) - 1 : 0ull;
                         const int first = q.prefix + tree.depth[node] - a.window + 1 - j0;
                         if (a.window > 0 && first > 0) see = first >= 64 ? 0ull : see & (~0ull << first);
 #pragma unroll
-                        for (int k = 0; k < kTreeWords; k++) {           // nodes 32 k .. 32 k + 31 are the keys from 32 k + cached on
+                        for (int k = 0; k < kTreeWords; k++) {       // nodes 32 k .. 32 k + 31 are the keys from 32 k + cached on
                             const int at = 32 * k + cached;
                             if (32 * k < q.n && at < 64 && at > -32) see |= at >= 0 ? (unsigned long long)tree.anc[node][k] << at : (unsigned long long)(tree.anc[node][k] >> -at);
                         }
                     }
+                    see >>= grp * KPT;
 #pragma unroll
-                    for (int i = 0; i < 32; i++) {
-                        if (!((uint32_t)see >> i & 1u)) v[i] = -INFINITY;
-                        if (!((uint32_t)(see >> 32) >> i & 1u)) v[32 + i] = -INFINITY;
-                    }
+                    for (int i = 0; i < KPT; i++)
+                        if (!((i < 32 ? (uint32_t)see : (uint32_t)(see >> 32)) >> (i & 31) & 1u)) v[i] = -INFINITY;
                 }
                 float top[4] = {v[0], v[1], v[2], v[3]};
 #pragma unroll
-                for (int i = 4; i < 60; i += 8)
+                for (int i = 4; i < KPT - 4; i += 8)
 #pragma unroll
                     for (int e = 0; e < 4; e++) top[e] = fmaxf(top[e], fmaxf(v[i + e], v[i + 4 + e]));
 #pragma unroll
-                for (int e = 0; e < 4; e++) top[e] = fmaxf(top[e], v[60 + e]);
+                for (int e = 0; e < 4; e++) top[e] = fmaxf(top[e], v[KPT - 4 + e]);
                 const float tm = node >= 0 ? fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3])) * scale : -INFINITY;
                 // the reference of the exponents: kept while nothing is more than 2^8 times it
                 const bool grows = tm > m_run + (F32 ? 0.0f : 8.0f) || m_run == -INFINITY;
@@ -550,39 +652,38 @@ __global__ void __launch_bounds__(kTcThreads, TcShape<HD, F32>::ctas) attn_tree_
                 const float off = m_new == -INFINITY ? 0.0f : -m_new;
                 float2 sum[2] = {};
 #pragma unroll
-                for (int i = 0; i < 64; i += 2) {
-                    const float2 x = fma2(make_float2(v[i], v[i + 1]), make_float2(scale, scale), make_float2(off, off));
-                    v[i] = tc_ex2(x.x); v[i + 1] = tc_ex2(x.y);
+                for (int i = 0; i < KPT; i += 2) {
+                    const float2 y = fma2(make_float2(v[i], v[i + 1]), make_float2(scale, scale), make_float2(off, off));
+                    v[i] = tc_ex2(y.x); v[i + 1] = tc_ex2(y.y);
                     sum[i >> 1 & 1] = add2(sum[i >> 1 & 1], make_float2(v[i], v[i + 1]));
                 }
                 l_run = l_run * alpha + ((sum[0].x + sum[0].y) + (sum[1].x + sum[1].y));
-                if constexpr (F32) {
-                    uint32_t pk[16];
+                // the weights' terms over the scores (the third one beside them), zeros where the keys are another row's
+                constexpr int kCols = KPT / 2 < 16 ? KPT / 2 : 16;
 #pragma unroll
-                    for (int h = 0; h < 2; h++)
+                for (int e = 0; e < S::p_terms; e++)
 #pragma unroll
-                        for (int e = 0; e < 3; e++) {
+                    for (int c = 0; c < KPT / 2; c += kCols) {
+                        uint32_t pk[kCols];
 #pragma unroll
-                            for (int i = 0; i < 16; i++) pk[i] = tc_term(&v[h * 32 + 2 * i], &v[h * 32 + 2 * i + 1]);
-                            tc_st16(e == 2 ? mine + S::col_x + (uint32_t)(t & 1) * 32u + h * 16u : sc + e * 32u + h * 16u, pk);
+                        for (int i = 0; i < kCols; i++) pk[i] = tc_term(&v[2 * (c + i)], &v[2 * (c + i) + 1]);
+                        const uint32_t to = e == 2 ? mine + S::col_x + (uint32_t)b * 32u : sc + e * 32u;
+#pragma unroll
+                        for (int d = 0; d < DUP; d++) {
+                            uint32_t out[kCols];
+#pragma unroll
+                            for (int i = 0; i < kCols; i++) out[i] = d == grp ? pk[i] : 0u;
+                            tc_st<kCols>(to + d * (KPT / 2) + c, out);
                         }
-                } else {
-                    uint32_t pk[32];
-#pragma unroll
-                    for (int e = 0; e < 2; e++) {
-#pragma unroll
-                        for (int i = 0; i < 32; i++) pk[i] = tc_term(&v[2 * i], &v[2 * i + 1]);
-                        tc_st32(sc + e * 32u, pk);
                     }
-                }
                 if (t > 0) {
-                    if constexpr (F32) {             // O(t - 1) comes out before O(t) is made
+                    if constexpr (F32) {         // O(t - 1) comes out before O(t) is made
                         wait(bar_o, t - 1);
                         tc_fence_after_sync();
 #pragma unroll
                         for (int c = 0; c < HD / 32; c++) {
                             uint32_t y[32];
-                            tc_ld32(mine + S::col_o + c * 32u, y);
+                            tc_ld<32>(mine + S::col_o + c * 32u, y);
                             tmem_ld_wait();
 #pragma unroll
                             for (int i = 0; i < 32; i++) o[c * 32 + i] = (o[c * 32 + i] + __uint_as_float(y[i])) * alpha;
@@ -593,11 +694,11 @@ __global__ void __launch_bounds__(kTcThreads, TcShape<HD, F32>::ctas) attn_tree_
 #pragma unroll 1
                         for (int c = 0; c < HD / 32; c++) {
                             uint32_t y[32];
-                            tc_ld32(mine + S::col_o + c * 32u, y);
+                            tc_ld<32>(mine + S::col_o + c * 32u, y);
                             tmem_ld_wait();
 #pragma unroll
                             for (int i = 0; i < 32; i++) y[i] = __float_as_uint(__uint_as_float(y[i]) * alpha);
-                            tc_st32(mine + S::col_o + c * 32u, y);
+                            tc_st<32>(mine + S::col_o + c * 32u, y);
                         }
                     }
                 }
@@ -605,31 +706,74 @@ __global__ void __launch_bounds__(kTcThreads, TcShape<HD, F32>::ctas) attn_tree_
             }
             tc_fence_before_sync();
             __syncwarp();
-            if (lane == 0) mbar_arrive(bar_p + 8u * (t & 1));
+            if (lane == 0) mbar_arrive(bar_p + 8u * b);
         }
         if (n_tiles > 1) wait(bar_o, n_tiles - 2);
         wait(bar_o, n_tiles - 1);
         tc_fence_after_sync();
-        // ---- out = O / l, or this chunk's share
-        if (warp * 32 < live_rows) {
+        // ---- the row's other copies: (maximum, sum, outputs) of their keys, through the room of the tiles (all of them have been used)
+        constexpr int kLd = HD + 4;
+        float* s_o = (float*)tc_smem;                // [copy - 1][row][kLd]
+        float* s_ml = (float*)(tc_smem + 2 * S::tile + 2 * S::tile) - 2 * 128;
+        static_assert(DUP == 1 || (DUP - 1) * (128 / DUP) * kLd * 4 + 1024 <= 4 * S::tile, "fits");
+        float f_own = 1.0f, f_other[DUP > 1 ? DUP - 1 : 1];
+        if constexpr (DUP > 1) {
+            if (live && grp > 0) {
+                s_ml[2 * (grp * (128 / DUP) + row)] = m_run; s_ml[2 * (grp * (128 / DUP) + row) + 1] = l_run;
+#pragma unroll
+                for (int c = 0; c < HD / 32; c++) {
+                    uint32_t y[32];
+                    tc_ld<32>(mine + S::col_o + c * 32u, y);
+                    tmem_ld_wait();
+#pragma unroll
+                    for (int i = 0; i < 32; i += 4) {
+                        float4 z = make_float4(__uint_as_float(y[i]), __uint_as_float(y[i + 1]), __uint_as_float(y[i + 2]), __uint_as_float(y[i + 3]));
+                        if constexpr (F32) { z.x += o[c * 32 + i]; z.y += o[c * 32 + i + 1]; z.z += o[c * 32 + i + 2]; z.w += o[c * 32 + i + 3]; }
+                        *(float4*)(s_o + ((grp - 1) * (128 / DUP) + row) * kLd + c * 32 + i) = z;
+                    }
+                }
+            }
+            named_sync(1, 128);
+            if (live && grp == 0) {
+                float top = m_run, m_g[DUP - 1], l_g[DUP - 1];
+#pragma unroll
+                for (int g = 0; g < DUP - 1; g++) {
+                    m_g[g] = s_ml[2 * ((g + 1) * (128 / DUP) + row)]; l_g[g] = s_ml[2 * ((g + 1) * (128 / DUP) + row) + 1];
+                    top = fmaxf(top, m_g[g]);
+                }
+                f_own = m_run == top ? 1.0f : exp2f(m_run - top);
+                l_run *= f_own;
+#pragma unroll
+                for (int g = 0; g < DUP - 1; g++) { f_other[g] = m_g[g] == top ? 1.0f : exp2f(m_g[g] - top); l_run = fmaf(l_g[g], f_other[g], l_run); }
+                m_run = top;
+            }
+        }
+        // ---- out = O / l, or this piece's share
+        const bool share = x.share >= 0;
+        if (live && grp == 0) {
             const int h = kvh * G + (node >= 0 ? f - node * G : 0), out_row = q.r0 + max(node, 0);
-            const float inv = part.chunks == 1 && node >= 0 ? tree_inverse(a, h, m_run, l_run) : 1.0f;
-            float odd = l_run * 0.0f;                // 0, or NaN where something is not finite
-            const size_t at = part_at(a, chunk, out_row, h);
+            const float inv = !share && node >= 0 ? tree_inverse(a, h, m_run, l_run) : 1.0f;
+            float odd = l_run * 0.0f;            // 0, or NaN where something is not finite
+            const size_t at = share_at(part, max(x.share, 0), row);
 #pragma unroll
             for (int c = 0; c < HD / 32; c++) {
                 uint32_t y[32];
-                tc_ld32(mine + S::col_o + c * 32u, y);
+                tc_ld<32>(mine + S::col_o + c * 32u, y);
                 tmem_ld_wait();
 #pragma unroll
                 for (int i = 0; i < 32; i++) {
-                    float x = __uint_as_float(y[i]);
-                    if constexpr (F32) x += o[c * 32 + i];
-                    odd = fmaf(x, 0.0f, odd);
-                    y[i] = __float_as_uint(x * inv);
+                    float z = __uint_as_float(y[i]);
+                    if constexpr (F32) z += o[c * 32 + i];
+                    if constexpr (DUP > 1) {
+                        z *= f_own;
+#pragma unroll
+                        for (int g = 0; g < DUP - 1; g++) z = fmaf(s_o[(g * (128 / DUP) + row) * kLd + c * 32 + i], f_other[g], z);
+                    }
+                    odd = fmaf(z, 0.0f, odd);
+                    y[i] = __float_as_uint(z * inv);
                 }
                 if (node >= 0) {
-                    if (part.chunks > 1) {
+                    if (share) {
 #pragma unroll
                         for (int i = 0; i < 32; i += 4) *(uint4*)(part.o + at * HD + c * 32 + i) = make_uint4(y[i], y[i + 1], y[i + 2], y[i + 3]);
                     } else {
@@ -640,82 +784,104 @@ __global__ void __launch_bounds__(kTcThreads, TcShape<HD, F32>::ctas) attn_tree_
                         } else {
 #pragma unroll
                             for (int i = 0; i < 32; i += 8) {
-                                uint32_t b[4];
+                                uint32_t r[4];
 #pragma unroll
-                                for (int e = 0; e < 4; e++) {            // the one rounding of the result
-                                    const __nv_bfloat162 r = __floats2bfloat162_rn(__uint_as_float(y[i + 2 * e]), __uint_as_float(y[i + 2 * e + 1]));
-                                    b[e] = *(const uint32_t*)&r;
+                                for (int e = 0; e < 4; e++) {        // the one rounding of the result
+                                    const __nv_bfloat162 z = __floats2bfloat162_rn(__uint_as_float(y[i + 2 * e]), __uint_as_float(y[i + 2 * e + 1]));
+                                    r[e] = *(const uint32_t*)&z;
                                 }
-                                *(uint4*)(dst + i) = make_uint4(b[0], b[1], b[2], b[3]);
+                                *(uint4*)(dst + i) = make_uint4(r[0], r[1], r[2], r[3]);
                             }
                         }
                     }
                 }
             }
-            if (part.chunks > 1 && node >= 0) { part.ml[2 * at] = m_run; part.ml[2 * at + 1] = l_run; }
-            const unsigned int bad = __ballot_sync(0xffffffffu, node >= 0 && odd != 0.0f);
-            if (lane == 0) s_odd[warp] = bad;
+            if (share && node >= 0) { part.ml[2 * at] = m_run; part.ml[2 * at + 1] = l_run; }
+            // rows that are not finite, once more and key by key
+            unsigned int bad = __ballot_sync(0xffffffffu, node >= 0 && odd != 0.0f && !*gave_up);
+            const int j_first = max(t_first * kTileKeys, w.low), j_end = min(w.n_keys, (t_first + n_tiles) * kTileKeys);
+            for (; bad; bad &= bad - 1) {
+                const int r = warp_row + __ffs(bad) - 1, fr = f0 + r, nr = node_of(fr), hr = kvh * G + fr - nr * G;
+                float m, l, z[HD / 32];
+                tree_row_plain<HD, TQ>(a, tree, q, kvh, fr, j_first, j_end, lane, &m, &l, z);
+                if (share) {
+                    const size_t to = share_at(part, x.share, r);
+                    for (int i = 0; i < HD / 32; i++) part.o[to * HD + lane * (HD / 32) + i] = z[i];
+                    if (lane == 0) { part.ml[2 * to] = m; part.ml[2 * to + 1] = l; }
+                } else {
+                    const float c = tree_inverse(a, hr, m, l);
+                    TQ* dst = (TQ*)a.out + (size_t)(q.r0 + nr) * a.out_stride + (size_t)hr * HD + lane * (HD / 32);
+                    for (int i = 0; i < HD / 32; i++) dst[i] = out_of<TQ>(z[i] * c);
+                }
+            }
         }
         tc_fence_before_sync();
     }
     __syncthreads();
     if (warp == 5) tmem_dealloc(tmem, S::cols);
-    if (*gave_up) {
-        if (tid == 0) atomicOr(a.status, LUM_ST_WAIT_TMEM);
-        return;
-    }
-    // rows that are not finite, once more and key by key
-    const int j_first = max(t_first * kTileKeys, w.low), j_end = min(w.n_keys, (t_first + n_tiles) * kTileKeys);
-    for (int r = warp; r < live_rows; r += kTcThreads / 32) {
-        if (!(s_odd[r >> 5] >> (r & 31) & 1u)) continue;
-        const int fr = f0 + r, h = kvh * G + fr % G, out_row = q.r0 + fr / G;
-        float m, l, x[HD / 32];
-        tree_row_plain<HD, TQ>(a, tree, q, kvh, fr, j_first, j_end, lane, &m, &l, x);
-        if (part.chunks > 1) {
-            const size_t at = part_at(a, chunk, out_row, h);
-            for (int i = 0; i < HD / 32; i++) part.o[at * HD + lane * (HD / 32) + i] = x[i];
-            if (lane == 0) { part.ml[2 * at] = m; part.ml[2 * at + 1] = l; }
-        } else {
-            const float inv = tree_inverse(a, h, m, l);
-            TQ* dst = (TQ*)a.out + (size_t)out_row * a.out_stride + (size_t)h * HD + lane * (HD / 32);
-            for (int i = 0; i < HD / 32; i++) dst[i] = out_of<TQ>(x[i] * inv);
-        }
-    }
+    if (tid == 0 && *gave_up) atomicOr(a.status, LUM_ST_WAIT_TMEM);
 }
 
-// ---- joins the chunks: a warp per (row, head); o = sum_c 2^(m_c - M) o_c / (sum_c 2^(m_c - M) l_c + 2^(sink - M))
+// ---- joins the shares of units that were cut: a warp per (row, head); o = sum_c 2^(m_c - M) o_c / (sum_c 2^(m_c - M) l_c + 2^(sink - M))
 template <int HD, typename TQ>
-__global__ void __launch_bounds__(256) tree_combine(const TreeAttnArgs a, const Part part) {
+__global__ void __launch_bounds__(256) tree_combine(const TreeAttnArgs a, const Share part) {
     constexpr int DPL = HD / 32;
-    pdl_grid_wait();
-    const int lane = threadIdx.x & 31;
+    const int lane = threadIdx.x & 31, G = a.n_q / a.n_kv;
     const long long item = (long long)blockIdx.x * 8 + (threadIdx.x >> 5);
-    if (item >= (long long)a.t.n_rows * a.n_q) return;
+    if (item >= (long long)a.t.n_rows * a.n_q) { pdl_grid_wait(); return; }
     const int row = (int)(item / a.n_q), h = (int)(item % a.n_q);
     // the row's sequence: the last one that starts at or before it
-    int lo = 0, hi = a.t.n_seq - 1;
-    while (lo < hi) {
-        const int mid = (lo + hi + 1) >> 1;
-        if (__ldg(a.t.row_start + mid) <= row) lo = mid; else hi = mid - 1;
+    Piece x;
+    int hi = a.t.n_seq - 1;
+    x.s = 0;
+    while (x.s < hi) {
+        const int mid = (x.s + hi + 1) >> 1;
+        if (__ldg(a.t.row_start + mid) <= row) x.s = mid; else hi = mid - 1;
     }
-    TreeSeq q;
-    if (!tree_seq(a.t, &a.m, lo, &q, nullptr) || row < q.r0 || row >= q.r0 + q.n) return;
-    const int n_tiles = tree_work(q.prefix, q.n, a.window).n_tiles, chunks = (n_tiles + part.tiles - 1) / part.tiles;
-    float top = a.sinks ? a.sinks[h] * kLog2e : -INFINITY;
-    for (int c = lane; c < chunks; c += 32) top = fmaxf(top, part.ml[2 * part_at(a, c, row, h)]);
-#pragma unroll
-    for (int i = 16; i > 0; i >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, i));
-    float sum = a.sinks ? exp2f(a.sinks[h] * kLog2e - top) : 0.0f, o[DPL];
+    const bool mine = tree_seq(a.t, &a.m, x.s, &x.q, nullptr) && row >= x.q.r0 && row < x.q.r0 + x.q.n;
+    pdl_grid_wait();                                 // (what comes before does not depend on the kernel before; every warp waits, so that this kernel ends behind that one)
+    if (!mine) return;
+    x.w = tree_work(x.q.prefix, x.q.n, a.window);
+    const int f = (row - x.q.r0) * G + h % G, R = part.tile_rows, unit = h / G * ((x.q.n * G + R - 1) / R) + f / R, r = f % R;
+    const int shares = pieces_of(x.w.n_tiles, __ldcg(part.plan)), first = __ldcg(part.plan + 1 + x.s) + unit * shares;
+    if (shares == 1) return;                         // finished by its CTA
+    const float sink = a.sinks ? a.sinks[h] * kLog2e : -INFINITY;
+    float top = sink, sum = a.sinks ? 1.0f : 0.0f, o[DPL];
 #pragma unroll
     for (int i = 0; i < DPL; i++) o[i] = 0.0f;
-    for (int c = 0; c < chunks; c++) {
-        const size_t at = part_at(a, c, row, h);
-        const float m = part.ml[2 * at], l = part.ml[2 * at + 1];
-        if (m == -INFINITY && l == 0.0f) continue;   // the chunk holds no key that this row sees
-        const float f = m == top ? 1.0f : exp2f(m - top);
-        sum = fmaf(l, f, sum);
+    // 32 shares at a time: a lane has the factor of one, all have their dimensions of each, eight on their way
+    for (int c0 = 0; c0 < shares; c0 += 32) {
+        float m = -INFINITY, l = 0.0f;
+        if (c0 + lane < shares) {
+            const float2 v = __ldcg((const float2*)part.ml + share_at(part, first + c0 + lane, r));
+            m = v.x; l = v.y;
+        }
+        float t = fmaxf(top, m);
 #pragma unroll
-        for (int i = 0; i < DPL; i++) o[i] = fmaf(part.o[at * HD + lane * DPL + i], f, o[i]);
+        for (int i = 16; i > 0; i >>= 1) t = fmaxf(t, __shfl_xor_sync(0xffffffffu, t, i));
+        const float before = top == t ? 1.0f : exp2f(top - t);
+        // negative: a share without a key that this row sees; undefined sums stay undefined
+        const float factor = m == -INFINITY && l == 0.0f ? -1.0f : m == t || l != l ? 1.0f : exp2f(m - t);
+        sum = sum * before + warp_sum(factor >= 0.0f ? l * factor : 0.0f);
+        top = t;
+#pragma unroll
+        for (int i = 0; i < DPL; i++) o[i] *= before;
+        const int n = min(32, shares - c0);
+        for (int c = 0; c < n; c += 8) {
+            float y[8][DPL], g[8];
+#pragma unroll
+            for (int u = 0; u < 8; u++) {
+                g[u] = __shfl_sync(0xffffffffu, factor, min(c + u, 31));
+                const bool in = c + u < n && g[u] >= 0.0f;
+                const float* src = part.o + share_at(part, first + min(c0 + c + u, shares - 1), r) * HD + lane * DPL;
+#pragma unroll
+                for (int i = 0; i < DPL; i++) y[u][i] = in ? __ldcg(src + i) : 0.0f;
+            }
+#pragma unroll
+            for (int u = 0; u < 8; u++)
+#pragma unroll
+                for (int i = 0; i < DPL; i++) o[i] = fmaf(y[u][i], fmaxf(g[u], 0.0f), o[i]);
+        }
     }
     const float inv = sum > 0.0f ? 1.0f / sum : sum;
     TQ* dst = (TQ*)a.out + (size_t)row * a.out_stride + (size_t)h * HD + lane * DPL;
@@ -723,31 +889,55 @@ __global__ void __launch_bounds__(256) tree_combine(const TreeAttnArgs a, const 
     for (int i = 0; i < DPL; i++) dst[i] = out_of<TQ>(o[i] * inv);
 }
 
-// Chunks of keys: as many as give every SM work, from what the call knows on the host (the longest sequence).
-Part plan(const TreeAttnArgs& a, int sm_count, int rows_tile, int per_sm) {
-    Part p{};
+// Copies of the query rows in a tile of 128 (see attn_tree_tc): as many as there is room for.
+int copies_of(const TreeAttnArgs& a) {
+    const int rows = a.t.max_rows * (a.n_q / a.n_kv);
+    return rows <= 32 ? 4 : rows <= 64 ? 2 : 1;
+}
+// What the call knows on the host: the CTAs that run at once, and bounds of the units and pieces the batch can have.
+struct Bounds { long long units, tiles; };
+Bounds bounds_of(const TreeAttnArgs& a, int tile_rows) {
     const int G = a.n_q / a.n_kv;
-    int tiles = (int)(((long long)a.t.max_prefix + a.t.max_rows + kTileKeys - 1) / kTileKeys);
-    if (a.window > 0) {
-        const long long seen = ((long long)a.window + a.t.max_rows) / kTileKeys + 2;
-        if (seen < tiles) tiles = (int)seen;
-    }
-    const long long units = (long long)a.t.n_seq * a.n_kv * ((a.t.max_rows * G + rows_tile - 1) / rows_tile), slots = (long long)sm_count * per_sm;
-    long long want = (slots + units - 1) / units;
-    if (want > tiles) want = tiles;
-    if (want < 1) want = 1;
-    p.tiles = (int)((tiles + want - 1) / want);
-    p.chunks = (tiles + p.tiles - 1) / p.tiles;
+    long long tiles = ((long long)a.t.max_prefix + a.t.max_rows + kTileKeys - 1) / kTileKeys;
+    if (a.window > 0) tiles = std::min(tiles, ((long long)a.window + a.t.max_rows) / kTileKeys + 2);
+    return {(long long)a.t.n_seq * a.n_kv * ((a.t.max_rows * G + tile_rows - 1) / tile_rows), tiles};
+}
+Share share_of(const TreeAttnArgs& a, int sm_count) {
+    Share p{};
+    const int G = a.n_q / a.n_kv;
+    p.copies = a.kv_bf16 ? copies_of(a) : 1;
+    p.tile_rows = a.kv_bf16 ? 128 / p.copies / G * G : kRowsTile;
+    p.rows = std::min(p.tile_rows, a.t.max_rows * G);
+    p.slots = sm_count * (a.kv_bf16 && !a.q_bf16 && a.hd == 128 ? 1 : 2);
+    const Bounds b = bounds_of(a, p.tile_rows);
+    // pieces: at most slots of them where there are fewer units, else at most units + tiles / (2 tiles / slots), with two for every cut
+    p.grid = (int)std::min(b.units * b.tiles, b.units < p.slots ? (long long)p.slots : b.units + p.slots / 2);
+    p.shares = b.tiles == 1 ? 0 : std::min(p.grid, p.slots);
     return p;
 }
-size_t part_bytes(const TreeAttnArgs& a, const Part& p) { return p.chunks > 1 ? (size_t)p.chunks * a.t.n_rows * a.n_q * (a.hd + 2) * 4 : 0; }
+size_t plan_bytes(const TreeAttnArgs& a) { return ((size_t)a.t.n_seq + 1 + 3) / 4 * 16; }
+size_t share_bytes(const TreeAttnArgs& a, const Share& p) { return plan_bytes(a) + (size_t)p.shares * p.rows * (a.hd + 2) * 4; }
 
-Part plan_of(const TreeAttnArgs& a, int sm_count) { return a.kv_bf16 ? plan(a, sm_count, 128, !a.q_bf16 && a.hd == 128 ? 1 : 2) : plan(a, sm_count, kRowsTile, 2); }
+template <int HD, typename TQ>
+cudaError_t combine(const TreeAttnArgs& a, const Share& p, cudaStream_t st) {
+    if (!p.shares) return cudaSuccess;               // nothing is cut
+    const long long items = (long long)a.t.n_rows * a.n_q;
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3((unsigned)((items + 7) / 8));
+    cfg.blockDim = dim3(256);
+    cfg.stream = st;
+    cudaLaunchAttribute at[1];
+    at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;      // its CTAs are there when the last share is
+    at[0].val.programmaticStreamSerializationAllowed = 1;
+    cfg.attrs = at;
+    cfg.numAttrs = 1;
+    return cudaLaunchKernelEx(&cfg, tree_combine<HD, TQ>, a, p);
+}
 
 // A cache as a tensor [dimension groups of 64][row][64]: one copy brings both halves of a head of 128.
 using EncodeTiled = CUresult (*)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*, const cuuint64_t*, const cuuint32_t*, const cuuint32_t*, CUtensorMapInterleave,
                                  CUtensorMapSwizzle, CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
-cudaError_t tensor_map(CUtensorMap* map, const TreeAttnArgs& a, const void* cache, int box_rows) {
+cudaError_t encode_bf16(CUtensorMap* map, const void* p, int rank, const cuuint64_t* dims, const cuuint64_t* strides, const cuuint32_t* box) {
     static std::atomic<EncodeTiled> found{nullptr};
     EncodeTiled encode = found.load(std::memory_order_acquire);
     if (!encode) {
@@ -758,59 +948,65 @@ cudaError_t tensor_map(CUtensorMap* map, const TreeAttnArgs& a, const void* cach
         encode = (EncodeTiled)fn;
         found.store(encode, std::memory_order_release);
     }
-    const cuuint64_t dims[3] = {64, (cuuint64_t)a.m.rows, (cuuint64_t)a.n_kv * a.hd / 64}, strides[2] = {(cuuint64_t)a.kv_stride * 2, 128};
-    const cuuint32_t box[3] = {64, (cuuint32_t)box_rows, box_rows == kTileKeys ? (cuuint32_t)a.hd / 64 : 1u}, step[3] = {1, 1, 1};
-    return encode(map, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 3, const_cast<void*>(cache), dims, strides, box, step, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
+    const cuuint32_t step[4] = {1, 1, 1, 1};
+    return encode(map, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, (cuuint32_t)rank, const_cast<void*>(p), dims, strides, box, step, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
                   CU_TENSOR_MAP_L2_PROMOTION_L2_128B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS ? cudaSuccess : cudaErrorInvalidValue;
 }
-
-template <int HD, typename TQ>
-cudaError_t combine(const TreeAttnArgs& a, const Part& p, cudaStream_t st) {
-    const long long items = (long long)a.t.n_rows * a.n_q;
-    cudaLaunchConfig_t cfg = {};
-    cfg.gridDim = dim3((unsigned)((items + 7) / 8));
-    cfg.blockDim = dim3(256);
-    cfg.stream = st;
-    cudaLaunchAttribute at[1];
-    at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;      // its CTAs are there when the last chunk ends
-    at[0].val.programmaticStreamSerializationAllowed = 1;
-    cfg.attrs = at;
-    cfg.numAttrs = 1;
-    return cudaLaunchKernelEx(&cfg, tree_combine<HD, TQ>, a, p);
+// A cache as a tensor [groups of 64 dimensions][row][64]: one copy brings both halves of a head of 128.
+cudaError_t map_cache(CUtensorMap* map, const TreeAttnArgs& a, const void* cache, int box_rows) {
+    const cuuint64_t dims[3] = {64, (cuuint64_t)a.m.rows, (cuuint64_t)a.n_kv * a.hd / 64}, strides[2] = {(cuuint64_t)a.kv_stride * 2, 128};
+    const cuuint32_t box[3] = {64, (cuuint32_t)box_rows, box_rows == kTileKeys ? (cuuint32_t)a.hd / 64 : 1u};
+    return encode_bf16(map, cache, 3, dims, strides, box);
+}
+// The queries as a tensor [half][row][head][64]: a box is the heads of a K/V head for the nodes of a unit.
+cudaError_t map_queries(CUtensorMap* map, const TreeAttnArgs& a, int tile_rows) {
+    const int G = a.n_q / a.n_kv;
+    const cuuint64_t dims[4] = {64, (cuuint64_t)a.n_q, (cuuint64_t)a.t.n_rows, (cuuint64_t)a.hd / 64}, strides[3] = {(cuuint64_t)a.hd * 2, (cuuint64_t)a.q_stride * 2, 128};
+    const cuuint32_t box[4] = {64, (cuuint32_t)G, (cuuint32_t)(tile_rows / G), 1};
+    return encode_bf16(map, a.q, 4, dims, strides, box);
 }
 template <int HD>
-cudaError_t rows_launch(const TreeAttnArgs& a, const Part& p, cudaStream_t st) {
+cudaError_t rows_launch(const TreeAttnArgs& a, const Share& p, cudaStream_t st) {
     static std::atomic<uint64_t> raised{0};
     if (const cudaError_t e = allow_smem(raised, (const void*)attn_tree_rows<HD>, rows_smem<HD>())) return e;
-    const int G = a.n_q / a.n_kv;
-    attn_tree_rows<HD><<<dim3(p.chunks, a.n_kv * ((a.t.max_rows * G + kRowsTile - 1) / kRowsTile), a.t.n_seq), 256, rows_smem<HD>(), st>>>(a, p);
+    attn_tree_rows<HD><<<p.grid, 256, rows_smem<HD>(), st>>>(a, p);
     const cudaError_t e = cudaGetLastError();
-    return e != cudaSuccess || p.chunks == 1 ? e : combine<HD, float>(a, p, st);
+    return e != cudaSuccess ? e : combine<HD, float>(a, p, st);
 }
-
-template <int HD, bool F32>
-cudaError_t tc_launch(const TreeAttnArgs& a, const Part& p, cudaStream_t st) {
+template <int HD, bool F32, int DUP>
+cudaError_t tc_launch_copies(const TreeAttnArgs& a, const Share& p, cudaStream_t st) {
     using S = TcShape<HD, F32>;
     static std::atomic<uint64_t> raised{0};
-    if (const cudaError_t e = allow_smem(raised, (const void*)attn_tree_tc<HD, F32>, S::smem, true)) return e;
-    const int G = a.n_q / a.n_kv, box_rows = a.m.lg >= 0 && 1 << a.m.lg < kTileKeys ? 1 << a.m.lg : kTileKeys;
-    CUtensorMap map_k, map_v;
-    if (const cudaError_t e = tensor_map(&map_k, a, a.k, box_rows)) return e;
-    if (const cudaError_t e = tensor_map(&map_v, a, a.v, box_rows)) return e;
-    attn_tree_tc<HD, F32><<<dim3(p.chunks, a.n_kv * ((a.t.max_rows * G + 127) / 128), a.t.n_seq), kTcThreads, S::smem, st>>>(a, p, map_k, map_v, box_rows);
+    if (const cudaError_t e = allow_smem(raised, (const void*)attn_tree_tc<HD, F32, DUP>, S::smem, true)) return e;
+    const int box_rows = a.m.lg >= 0 && 1 << a.m.lg < kTileKeys ? 1 << a.m.lg : kTileKeys;
+    CUtensorMap map_q{}, map_k, map_v;
+    if constexpr (!F32) if (const cudaError_t e = map_queries(&map_q, a, p.tile_rows)) return e;
+    if (const cudaError_t e = map_cache(&map_k, a, a.k, box_rows)) return e;
+    if (const cudaError_t e = map_cache(&map_v, a, a.v, box_rows)) return e;
+    attn_tree_tc<HD, F32, DUP><<<p.grid, kTcThreads, S::smem, st>>>(a, p, map_q, map_k, map_v, box_rows);
     const cudaError_t e = cudaGetLastError();
-    return e != cudaSuccess || p.chunks == 1 ? e : combine<HD, typename std::conditional<F32, float, __nv_bfloat16>::type>(a, p, st);
+    return e != cudaSuccess ? e : combine<HD, typename std::conditional<F32, float, __nv_bfloat16>::type>(a, p, st);
+}
+template <int HD, bool F32>
+cudaError_t tc_launch(const TreeAttnArgs& a, const Share& p, cudaStream_t st) {
+    return p.copies == 4 ? tc_launch_copies<HD, F32, 4>(a, p, st) : p.copies == 2 ? tc_launch_copies<HD, F32, 2>(a, p, st) : tc_launch_copies<HD, F32, 1>(a, p, st);
 }
 
 }  // namespace
 
-size_t tree_attn_workspace(const TreeAttnArgs& a, int sm_count) { return part_bytes(a, plan_of(a, sm_count)); }
+bool tree_attn_supported(const TreeAttnArgs& a) {
+    if (a.kv_bf16 && a.n_q / a.n_kv > 128) return false;
+    const Bounds b = bounds_of(a, a.kv_bf16 ? 128 / copies_of(a) / (a.n_q / a.n_kv) * (a.n_q / a.n_kv) : kRowsTile);
+    return b.units < 0x40000000ll && b.units * b.tiles < 0x7fffffffll;       // tiles are counted in 32 bits
+}
+size_t tree_attn_workspace(const TreeAttnArgs& a, int sm_count) { return share_bytes(a, share_of(a, sm_count)); }
 
 cudaError_t launch_tree_attn(const TreeAttnArgs& a, int sm_count, cudaStream_t st) {
-    Part p = plan_of(a, sm_count);
-    if (part_bytes(a, p) > a.ws_bytes) return cudaErrorInvalidValue;
-    p.o = (float*)a.ws;
-    p.ml = p.o + (size_t)p.chunks * a.t.n_rows * a.n_q * a.hd;
+    Share p = share_of(a, sm_count);
+    if (share_bytes(a, p) > a.ws_bytes) return cudaErrorInvalidValue;
+    p.plan = (int*)a.ws;
+    p.o = (float*)((char*)a.ws + plan_bytes(a));
+    p.ml = p.o + (size_t)p.shares * p.rows * a.hd;
     if (!a.kv_bf16) return a.hd == 128 ? rows_launch<128>(a, p, st) : rows_launch<64>(a, p, st);
     if (a.hd == 128) return a.q_bf16 ? tc_launch<128, false>(a, p, st) : tc_launch<128, true>(a, p, st);
     return a.q_bf16 ? tc_launch<64, false>(a, p, st) : tc_launch<64, true>(a, p, st);
