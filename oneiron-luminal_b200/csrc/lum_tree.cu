@@ -14,55 +14,155 @@ namespace {
 __device__ uint32_t g_tree_status;                   // status word of these operators: part of the library, so that no call allocates
 
 // ---------------------------------------------------------------------------------------------------- accepted nodes
-// A pick as a key: order-preserving bits of the logit (NaN as -inf, -0 as 0), then its index, so that the largest key is the last maximum.
+// pick(i) = arg-max of the logits of node i (the last maximum); node 0 stands, and the first child of a node that carries its pick stands next.  What it costs is
+// reading logits.  Two ways:
+//   tree_picks, tree_follow   every row's arg-max at once, spread over all SMs, then the walk through numbers;
+//   tree_walk                 row by row along the path: rows of nodes that do not stand are not read, but each one waits for the one before.  A cluster per
+//                             sequence shares a row and exchanges its maxima through distributed shared memory, one barrier a step.
+// Both use 16-byte loads and as many of them in flight as a thread has.
+
+// A pick as a key: order-preserving bits of the logit, then its index, so that the largest key is the last maximum (-0 as 0).
 __device__ __forceinline__ unsigned long long pick_key(float v, int i) {
-    v = v != v ? -INFINITY : v + 0.0f;
-    const uint32_t b = __float_as_uint(v);
+    const uint32_t b = __float_as_uint(v + 0.0f);
     return ((unsigned long long)(b & 0x80000000u ? ~b : b | 0x80000000u) << 32) | (uint32_t)i;
 }
 __device__ __forceinline__ unsigned long long key_max(unsigned long long a, unsigned long long b) { return a > b ? a : b; }
+__device__ __forceinline__ unsigned long long warp_key(unsigned long long k) {
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) k = key_max(k, __shfl_xor_sync(0xffffffffu, k, o));
+    return k;
+}
+// The best of row[i0 .. i1) among `threads` threads (every thread its own; 0: it has none).  NaN counts as -inf.
+__device__ __forceinline__ unsigned long long pick_range(const float* row, int i0, int i1, int tid, int threads) {
+    float v[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+    int at[4] = {-1, -1, -1, -1};
+    auto take = [&](int u, float x, int i) {
+        x = fmaxf(x, -INFINITY);
+        if (x >= v[u]) { v[u] = x; at[u] = i; }      // (a thread's indices grow)
+    };
+    const int head = min(i1 - i0, (int)(-((uintptr_t)(row + i0) >> 2) & 3)), n4 = (i1 - i0 - head) >> 2, tail = i0 + head + 4 * n4;
+    if (tid < head) take(0, __ldcg(row + i0 + tid), i0 + tid);
+    const float4* p = (const float4*)(row + i0 + head);
+    constexpr int U = 8;
+    for (int x0 = tid; x0 < n4; x0 += threads * U) {
+        float4 y[U];
+#pragma unroll
+        for (int u = 0; u < U; u++) if (x0 + u * threads < n4) y[u] = __ldcg(p + x0 + u * threads);
+#pragma unroll
+        for (int u = 0; u < U; u++)
+            if (x0 + u * threads < n4) {
+                const int i = i0 + head + 4 * (x0 + u * threads);
+                take(0, y[u].x, i); take(1, y[u].y, i + 1); take(2, y[u].z, i + 2); take(3, y[u].w, i + 3);
+            }
+    }
+    if (tid < i1 - tail) take(0, __ldcg(row + tail + tid), tail + tid);
+    unsigned long long k = 0ull;
+#pragma unroll
+    for (int u = 0; u < 4; u++) if (at[u] >= 0) k = key_max(k, pick_key(v[u], at[u]));
+    return k;
+}
 
-// One CTA per sequence: the row of logits of the node it stands at, its arg-max, the child that carries it.  Rows of nodes that do not stand are not read.
-__global__ void __launch_bounds__(1024) tree_walk(const TreeAcceptArgs a) {
-    __shared__ unsigned long long s_key[32];
-    __shared__ int s_tok[kTreeMax], s_parent[kTreeMax], s_child;
-    const int s = blockIdx.x, tid = threadIdx.x;
-    TreeSeq q;
-    if (!tree_seq(a.t, nullptr, s, &q, a.status)) return;
-    for (int i = tid; i < q.n; i += 1024) {
-        s_tok[i] = a.tokens[q.r0 + i];
+// The tree of a sequence in shared memory; parents that are no earlier node count as none.
+struct WalkTree { int token[kTreeMax]; short parent[kTreeMax]; };
+__device__ __forceinline__ void walk_load(WalkTree& w, const TreeAcceptArgs& a, const TreeSeq& q, int tid, int threads, bool report) {
+    for (int i = tid; i < q.n; i += threads) {
+        w.token[i] = a.tokens[q.r0 + i];
         int p = __ldg(a.t.parent + q.r0 + i);
-        if (p < -1 || p >= i) { p = -1; atomicOr(a.status, LUM_ST_BAD_TREE); }
-        s_parent[i] = p;
+        if (p < -1 || p >= i) { p = -1; if (report) atomicOr(a.status, LUM_ST_BAD_TREE); }
+        w.parent[i] = (short)p;
     }
-    int* path = a.path + (size_t)s * a.path_len;
-    for (int i = tid; i < a.path_len; i += 1024) path[i] = -1;
+}
+// The first child of `node` that carries `pick`, by a warp (kTreeMax: none).
+__device__ __forceinline__ int walk_child(const WalkTree& w, int n, int node, int pick, int lane) {
+    for (int i0 = node + 1; i0 < n; i0 += 32) {
+        const unsigned int m = __ballot_sync(0xffffffffu, i0 + lane < n && w.parent[i0 + lane] == node && w.token[i0 + lane] == pick);
+        if (m) return i0 + __ffs(m) - 1;
+    }
+    return kTreeMax;
+}
+
+constexpr int kPickThreads = 256;
+__global__ void __launch_bounds__(kPickThreads) tree_picks(const TreeAcceptArgs a, int chunks, unsigned long long* keys) {
+    __shared__ unsigned long long s_key[kPickThreads / 32];
+    pdl_launch_dependents();
+    const int row = blockIdx.x / chunks, c = blockIdx.x - row * chunks, per = (a.vocab + chunks - 1) / chunks, i0 = min(a.vocab, c * per), i1 = min(a.vocab, i0 + per);
+    unsigned long long k = warp_key(pick_range(a.logits + (size_t)row * a.ld, i0, i1, threadIdx.x, kPickThreads));
+    if ((threadIdx.x & 31) == 0) s_key[threadIdx.x >> 5] = k;
     __syncthreads();
-    int node = q.n > 0 ? 0 : -1, count = 0, pick = -1;
-    while (node >= 0) {
-        if (tid == 0) { path[count] = node; s_child = q.n; }
-        count++;
-        if (a.picks) pick = a.picks[q.r0 + node];
-        else {
-            const float* row = a.logits + (size_t)(q.r0 + node) * a.ld;
-            unsigned long long k = 0ull;
-            for (int i = tid; i < a.vocab; i += 1024) k = key_max(k, pick_key(row[i], i));
+    if (threadIdx.x == 0) {
 #pragma unroll
-            for (int o = 16; o > 0; o >>= 1) k = key_max(k, __shfl_xor_sync(0xffffffffu, k, o));
-            if ((tid & 31) == 0) s_key[tid >> 5] = k;
-            __syncthreads();
-            k = s_key[tid & 31];
-#pragma unroll
-            for (int o = 16; o > 0; o >>= 1) k = key_max(k, __shfl_xor_sync(0xffffffffu, k, o));
-            pick = (int)(uint32_t)k;
-        }
-        __syncthreads();
-        for (int i = node + 1 + tid; i < q.n; i += 1024) if (s_parent[i] == node && s_tok[i] == pick) atomicMin(&s_child, i);
-        __syncthreads();
-        node = s_child < q.n ? s_child : -1;
-        __syncthreads();
+        for (int i = 1; i < kPickThreads / 32; i++) k = key_max(k, s_key[i]);
+        keys[blockIdx.x] = k;
     }
-    if (tid == 0) { a.n_accepted[s] = count; a.next[s] = pick; }
+}
+// One CTA per sequence: the picks of its rows (from their chunks' keys, or given), then the walk by one warp.
+__global__ void __launch_bounds__(256) tree_follow(const TreeAcceptArgs a, int chunks, const unsigned long long* keys) {
+    __shared__ WalkTree w;
+    __shared__ int s_pick[kTreeMax];
+    const int s = blockIdx.x, tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+    TreeSeq q;
+    const bool ok = tree_seq(a.t, nullptr, s, &q, a.status);
+    int* path = a.path + (size_t)s * a.path_len;
+    if (ok) {
+        walk_load(w, a, q, tid, 256, true);
+        if (!keys) for (int i = tid; i < q.n; i += 256) s_pick[i] = a.picks[q.r0 + i];
+    }
+    pdl_grid_wait();                                 // (what comes before does not depend on the kernel before)
+    if (!ok) return;
+    if (keys)
+        for (int i = warp; i < q.n; i += 8) {
+            unsigned long long k = 0ull;
+            for (int c = lane; c < chunks; c += 32) k = key_max(k, __ldcg(keys + (size_t)(q.r0 + i) * chunks + c));
+            k = warp_key(k);
+            if (lane == 0) s_pick[i] = (int)(uint32_t)k;
+        }
+    __syncthreads();
+    if (warp == 0) {
+        int node = q.n > 0 ? 0 : kTreeMax, count = 0, pick = -1;
+        while (node < kTreeMax) {
+            if (lane == 0) path[count] = node;
+            count++;
+            pick = s_pick[node];
+            node = walk_child(w, q.n, node, pick, lane);
+        }
+        for (int i = count + lane; i < a.path_len; i += 32) path[i] = -1;
+        if (lane == 0) { a.n_accepted[s] = count; a.next[s] = pick; }
+    }
+}
+
+constexpr int kWalkThreads = 512, kWalkMax = 8;      // CTAs of a (portable) cluster
+__global__ void __launch_bounds__(kWalkThreads) tree_walk(const TreeAcceptArgs a) {
+    __shared__ WalkTree w;
+    __shared__ unsigned long long s_key[kWalkThreads / 32], s_all[2][kWalkMax];
+    const int C = gridDim.x, c = blockIdx.x, s = blockIdx.y, tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+    TreeSeq q;
+    if (!tree_seq(a.t, nullptr, s, &q, a.status)) return;                      // (the whole cluster)
+    walk_load(w, a, q, tid, kWalkThreads, c == 0);
+    int* path = a.path + (size_t)s * a.path_len;
+    const int per = ((a.vocab + C - 1) / C + 3) & ~3, i0 = min(a.vocab, c * per), i1 = min(a.vocab, i0 + per);
+    int node = q.n > 0 ? 0 : kTreeMax, count = 0, pick = -1;
+    cluster_arrive_release();                        // nobody writes into a CTA that has not begun
+    cluster_wait_acquire();
+    while (node < kTreeMax) {
+        if (c == 0 && tid == 0) path[count] = node;
+        unsigned long long k = warp_key(pick_range(a.logits + (size_t)(q.r0 + node) * a.ld, i0, i1, tid, kWalkThreads));
+        if (lane == 0) s_key[warp] = k;
+        __syncthreads();                             // (also: the tree is there)
+        if (warp == 0) {
+            k = warp_key(lane < kWalkThreads / 32 ? s_key[lane] : 0ull);
+            if (lane < C) asm volatile("st.shared::cluster.u64 [%0], %1;" ::"r"(cluster_map(smem_u32(&s_all[count & 1][c]), (uint32_t)lane)), "l"(k) : "memory");
+        }
+        cluster_arrive_release();
+        cluster_wait_acquire();
+        k = warp_key(lane < C ? s_all[count & 1][lane] : 0ull);
+        pick = (int)(uint32_t)k;
+        node = walk_child(w, q.n, node, pick, lane);
+        count++;
+    }
+    if (c == 0) {
+        for (int i = count + tid; i < a.path_len; i += kWalkThreads) path[i] = -1;
+        if (tid == 0) { a.n_accepted[s] = count; a.next[s] = pick; }
+    }
 }
 
 // ---------------------------------------------------------------------------------------------------- cache rows
@@ -130,11 +230,45 @@ __global__ void __launch_bounds__(kCopyThreads) kv_copy(const KvPlane* planes, l
 
 }  // namespace
 
-size_t tree_accept_workspace(const TreeBatch&, int, int) { return 0; }
+// Every row at once where that is little to read, else along the paths.  Measured from HBM, us, all rows / along paths of 4 nodes, vocabulary 128256: 1 x 8 nodes (4 MB)
+// 11.4 / 18.5, 4 x 16 (33 MB) 18.2 / 19.1, 1 x 64 (33 MB) 21.3 / 18.1, 8 x 16 (66 MB) 27.0 / 20.2, 32 x 64 (1051 MB) 180 / 26.8.
+static bool picks_all(const TreeBatch& t, int vocab) { return (long long)t.n_rows * vocab <= (8ll << 20); }
+static int pick_chunks(const TreeBatch& t, int vocab, int sm_count) {          // four CTAs per SM, each with at least a load per thread
+    const long long want = (4ll * sm_count + t.n_rows - 1) / t.n_rows, most = (vocab + 4 * kPickThreads - 1) / (4 * kPickThreads);
+    return (int)(want < most ? want : most);
+}
+size_t tree_accept_workspace(const TreeBatch& t, int vocab, int sm_count) { return picks_all(t, vocab) ? (size_t)t.n_rows * pick_chunks(t, vocab, sm_count) * 8 : 0; }
 
-cudaError_t launch_tree_accept(const TreeAcceptArgs& a, int, cudaStream_t st) {
-    tree_walk<<<a.t.n_seq, 1024, 0, st>>>(a);
-    return cudaGetLastError();
+cudaError_t launch_tree_accept(const TreeAcceptArgs& a, int sm_count, cudaStream_t st) {
+    cudaLaunchConfig_t cfg = {};
+    cudaLaunchAttribute at[1];
+    cfg.stream = st;
+    cfg.attrs = at;
+    if (a.logits && !picks_all(a.t, a.vocab)) {
+        // two CTAs per SM in all, at least one per sequence
+        int C = 1;
+        while (C < kWalkMax && 2 * C * a.t.n_seq <= 2 * sm_count) C *= 2;
+        cfg.gridDim = dim3(C, a.t.n_seq);
+        cfg.blockDim = dim3(kWalkThreads);
+        at[0].id = cudaLaunchAttributeClusterDimension;
+        at[0].val.clusterDim.x = (unsigned)C; at[0].val.clusterDim.y = 1; at[0].val.clusterDim.z = 1;
+        cfg.numAttrs = 1;
+        return cudaLaunchKernelEx(&cfg, tree_walk, a);
+    }
+    int chunks = 0;
+    unsigned long long* keys = nullptr;
+    if (a.logits) {
+        chunks = pick_chunks(a.t, a.vocab, sm_count);
+        keys = (unsigned long long*)a.ws;
+        tree_picks<<<(unsigned)(a.t.n_rows * chunks), kPickThreads, 0, st>>>(a, chunks, keys);
+        if (const cudaError_t e = cudaGetLastError()) return e;
+    }
+    cfg.gridDim = dim3(a.t.n_seq);
+    cfg.blockDim = dim3(256);
+    at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    at[0].val.programmaticStreamSerializationAllowed = 1;
+    cfg.numAttrs = a.logits ? 1 : 0;                 // (without tree_picks before it, it waits for whatever wrote the picks)
+    return cudaLaunchKernelEx(&cfg, tree_follow, a, chunks, (const unsigned long long*)keys);
 }
 cudaError_t launch_kv_compact(const KvPlane* planes, int n_planes, const TreeMap& m, const TreeBatch& t, const int* path, int path_len, const int* n_accepted, uint32_t* status,
                               int, cudaStream_t st) {
@@ -159,8 +293,15 @@ using namespace lum;
 
 // the status word of the current device (null: it cannot be had); lum_op_status reads it too
 uint32_t* lum_tree_status_word() {
-    void* p = nullptr;
-    return cudaGetSymbolAddress(&p, g_tree_status) == cudaSuccess ? (uint32_t*)p : nullptr;
+    static std::atomic<void*> known[64] = {};        // its address per device: asking takes longer than a launch
+    int dev = 0;
+    if (cudaGetDevice(&dev) != cudaSuccess) return nullptr;
+    void* p = dev >= 0 && dev < 64 ? known[dev].load(std::memory_order_acquire) : nullptr;
+    if (!p) {
+        if (cudaGetSymbolAddress(&p, g_tree_status) != cudaSuccess) return nullptr;
+        if (dev >= 0 && dev < 64) known[dev].store(p, std::memory_order_release);
+    }
+    return (uint32_t*)p;
 }
 
 namespace {

@@ -24,9 +24,23 @@ _F32, _BF16 = 0, 2
 _INVALID = -1
 
 
-def _torch():
-    import torch       # the package itself does not need it
-    return torch
+torch = None               # the package itself does not need it: imported by the first tensor
+
+
+def _use_torch():
+    global torch
+    if torch is None:
+        import torch as t
+        torch = t
+
+
+_TYPES = {}
+
+
+def _types():
+    if not _TYPES:
+        _TYPES.update({torch.float32: _F32, torch.bfloat16: _BF16})
+    return _TYPES
 
 
 def _bad(why: str):
@@ -37,7 +51,8 @@ def _ints(name, t, device, dims=1, optional=False):
     """Address of a contiguous int32 tensor on ``device``."""
     if t is None and optional:
         return None
-    torch = _torch()
+    if torch is None:
+        _use_torch()
     if not isinstance(t, torch.Tensor) or t.dtype != torch.int32 or t.dim() != dims or not t.is_contiguous() or t.device != device or not t.is_cuda:
         _bad(f"{name}: a contiguous {dims}-d int32 tensor on {device} is wanted")
     return t.data_ptr()
@@ -48,24 +63,26 @@ def _check(rc: int) -> None:
         raise LumError(rc, load_library().lum_last_error(None).decode())
 
 
-class _On:
-    """Makes the tensors' device the current one for a call and hands out its current stream."""
+def _stream(index: int) -> int:
+    return torch._C._cuda_getCurrentRawStream(index)       # what torch.cuda.current_stream(index).cuda_stream is, at a tenth of its time
+
+
+class _Here:
+    """Makes the tensors' device the current one for a call, where it is not."""
 
     __slots__ = ("index", "before")
 
-    def __init__(self, device):
-        self.index = device.index
+    def __init__(self, index):
+        self.index = index
 
     def __enter__(self):
-        cuda = _torch().cuda
-        self.before = cuda.current_device()
+        self.before = torch.cuda.current_device()
         if self.before != self.index:
-            cuda.set_device(self.index)
-        return cuda.current_stream().cuda_stream
+            torch.cuda.set_device(self.index)
 
     def __exit__(self, *exc):
         if self.before != self.index:
-            _torch().cuda.set_device(self.before)
+            torch.cuda.set_device(self.before)
 
 
 class DraftTree:
@@ -75,9 +92,9 @@ class DraftTree:
     def __init__(self, row_start, prefix, parent, *, max_rows: int, max_prefix: int, slot=None):
         device = getattr(parent, "device", None)
         n_seq = prefix.numel()
-        self.device, self.tensors = device, (row_start, prefix, parent, slot)
+        self.device, self.n_seq, self.n_rows, self.max_rows, self.tensors = device, n_seq, parent.numel(), max_rows, (row_start, prefix, parent, slot)
         self.desc = DraftTreeDesc(_ints("row_start", row_start, device), _ints("prefix", prefix, device), _ints("parent", parent, device),
-                                  _ints("slot", slot, device, optional=True), n_seq, parent.numel(), max_rows, max_prefix)
+                                  _ints("slot", slot, device, optional=True), n_seq, self.n_rows, max_rows, max_prefix)
         if row_start.numel() != n_seq + 1 or (slot is not None and slot.numel() != n_seq):
             _bad(f"row_start has {row_start.numel()} entries, slot {n_seq if slot is None else slot.numel()}, for {n_seq} sequences")
 
@@ -98,8 +115,11 @@ class KvMap:
 
 def _rows_of(name, t, device, width, rows):
     """(address, row stride) of a tensor whose rows are ``width`` elements, dense in a row."""
-    if t.device != device or t.dim() < 2 or t.shape[0] != rows:
-        _bad(f"{name}: {rows} rows on {device} are wanted, got {tuple(t.shape)} on {t.device}")
+    shape = t.shape
+    if t.device != device or len(shape) < 2 or shape[0] != rows:
+        _bad(f"{name}: {rows} rows on {device} are wanted, got {tuple(shape)} on {t.device}")
+    if t.is_contiguous() and t.numel() == rows * width:
+        return t.data_ptr(), width
     inner = 1
     for size, stride in zip(reversed(t.shape[1:]), reversed(t.stride()[1:])):
         if size != 1 and stride != inner:
@@ -117,12 +137,13 @@ def attn_tree(q, k, v, tree: DraftTree, cache: KvMap, *, n_kv_heads: int, head_d
     queries; rows may be strided.  ``scale`` 0: 1 / sqrt(head_dim).  ``window``: a node sees only what is fewer than so many places before its own.  ``sinks``
     [heads] f32: a logit per head that joins the softmax's denominator.  Returns ``out`` (like q; rows of no sequence are left as they were; without ``out``
     given they are not set).  ``workspace``: scratch to use, a uint8 tensor of at least :func:`attn_tree_workspace` bytes (None: taken from torch)."""
-    torch = _torch()
-    device, types = q.device, {torch.float32: _F32, torch.bfloat16: _BF16}
-    if device != tree.device or q.dtype not in types or k.dtype not in types or v.dtype != k.dtype:
+    device, q_type, k_type = q.device, _types().get(q.dtype), _types().get(k.dtype)
+    if device != tree.device or q_type is None or k_type is None or v.dtype != k.dtype:
         _bad(f"attn_tree: q {q.dtype} on {device}, tree on {tree.device}, k {k.dtype}, v {v.dtype}: bf16 or f32 on one device are wanted")
-    rows = tree.desc.n_rows
-    width = q[0].numel() if rows else q.shape[1] if q.dim() > 1 else 0
+    rows = tree.n_rows
+    width = 1
+    for size in q.shape[1:]:
+        width *= size
     if out is None:
         out = torch.empty_like(q, memory_format=torch.contiguous_format)
     elif out.dtype != q.dtype:
@@ -138,16 +159,16 @@ def attn_tree(q, k, v, tree: DraftTree, cache: KvMap, *, n_kv_heads: int, head_d
         if sinks.device != device or sinks.dtype != torch.float32 or not sinks.is_contiguous() or sinks.numel() != width // head_dim:
             _bad(f"attn_tree: sinks must be {width // head_dim} contiguous f32 values on {device}")
         s_at = sinks.data_ptr()
-    desc = TreeAttnDesc(types[q.dtype], types[k.dtype], width // head_dim, n_kv_heads, head_dim, window, scale, 0, q_stride, k_stride, o_stride)
+    desc = TreeAttnDesc(q_type, k_type, width // head_dim, n_kv_heads, head_dim, window, scale, 0, q_stride, k_stride, o_stride)
     lib = load_library()
-    with _On(device) as stream:
+    with _Here(device.index):
         need = lib.lum_op_attn_tree_workspace(desc, tree.desc, cache.desc)
         if need == C.c_size_t(-1).value:
             _check(_INVALID)
         if need and workspace is None:
             workspace = torch.empty(need, dtype=torch.uint8, device=device)
         w_at, w_bytes = (workspace.data_ptr(), workspace.numel() * workspace.element_size()) if workspace is not None else (None, 0)
-        _check(lib.lum_op_attn_tree(desc, tree.desc, cache.desc, q_at, k_at, v_at, s_at, o_at, w_at, w_bytes, stream))
+        _check(lib.lum_op_attn_tree(desc, tree.desc, cache.desc, q_at, k_at, v_at, s_at, o_at, w_at, w_bytes, _stream(device.index)))
     return out
 
 
@@ -157,9 +178,8 @@ def tree_accept(tree: DraftTree, tokens, *, logits=None, picks=None, path_len: i
     Node 0 stands; at a node the model picks the arg-max of its row of ``logits`` [rows, vocab] f32 (the last maximum, as the greedy sample does) or
     ``picks`` [rows] (what a sampler drew); the first child whose token (``tokens`` [rows]) is the pick stands next.  ``path`` has -1 behind the nodes that stand;
     ``next_token`` is the pick at the last of them."""
-    torch = _torch()
-    device, n, rows = tree.device, tree.desc.n_seq, tree.desc.n_rows
-    path_len = path_len or tree.desc.max_rows
+    device, n, rows = tree.device, tree.n_seq, tree.n_rows
+    path_len = path_len or tree.max_rows
     t_at, p_at = _ints("tokens", tokens, device), _ints("picks", picks, device, optional=True)
     if tokens.numel() != rows or (picks is not None and picks.numel() != rows):
         _bad(f"tree_accept: {tokens.numel()} tokens for {rows} rows")
@@ -171,7 +191,7 @@ def tree_accept(tree: DraftTree, tokens, *, logits=None, picks=None, path_len: i
     path = torch.empty((n, path_len), dtype=torch.int32, device=device)
     count, after = torch.empty((2, n), dtype=torch.int32, device=device).unbind(0)
     lib = load_library()
-    with _On(device) as stream:
+    with _Here(device.index):
         w_at, need = None, 0
         if logits is not None:
             need = lib.lum_op_tree_accept_workspace(tree.desc, vocab)
@@ -180,12 +200,13 @@ def tree_accept(tree: DraftTree, tokens, *, logits=None, picks=None, path_len: i
             if need:
                 workspace = torch.empty(need, dtype=torch.uint8, device=device)
                 w_at = workspace.data_ptr()
-        _check(lib.lum_op_tree_accept(tree.desc, t_at, l_at, vocab, ld, p_at, path.data_ptr(), path_len, count.data_ptr(), after.data_ptr(), w_at, need, stream))
+        _check(lib.lum_op_tree_accept(tree.desc, t_at, l_at, vocab, ld, p_at, path.data_ptr(), path_len, count.data_ptr(), after.data_ptr(), w_at, need, _stream(device.index)))
     return path, count, after
 
 
 def _planes(planes):
-    torch = _torch()
+    if torch is None:
+        _use_torch()
     if planes.dtype != torch.int64 or planes.dim() != 2 or planes.shape[1] != 2 or not planes.is_contiguous() or not planes.is_cuda:
         _bad("planes: a contiguous [planes, 2] int64 tensor on the GPU is wanted (address and bytes of a row)")
     return planes.data_ptr(), planes.shape[0]
@@ -194,7 +215,7 @@ def _planes(planes):
 def kv_planes(tensors):
     """The table of planes that :func:`kv_compact` and :func:`kv_copy` take, of 2-d (or 3-d: one plane per first index) cache tensors whose rows follow each
     other.  Made once for a cache; the tensors have to outlive it."""
-    torch = _torch()
+    _use_torch()
     entries, device = [], None
     for t in tensors:
         for p in (t.unbind(0) if t.dim() == 3 else [t]):
@@ -215,10 +236,10 @@ def kv_compact(planes, cache: KvMap, tree: DraftTree, path, n_accepted) -> None:
     p_at, n = _planes(planes)
     device = planes.device
     path_at, n_at = _ints("path", path, device, dims=2), _ints("n_accepted", n_accepted, device)
-    if device != tree.device or path.shape[0] != tree.desc.n_seq or n_accepted.numel() != tree.desc.n_seq:
-        _bad(f"kv_compact: paths of {path.shape[0]} and counts of {n_accepted.numel()} sequences for {tree.desc.n_seq}")
-    with _On(device) as stream:
-        _check(load_library().lum_op_kv_compact(p_at, n, cache.desc, tree.desc, path_at, path.shape[1], n_at, stream))
+    if device != tree.device or path.shape[0] != tree.n_seq or n_accepted.numel() != tree.n_seq:
+        _bad(f"kv_compact: paths of {path.shape[0]} and counts of {n_accepted.numel()} sequences for {tree.n_seq}")
+    with _Here(device.index):
+        _check(load_library().lum_op_kv_compact(p_at, n, cache.desc, tree.desc, path_at, path.shape[1], n_at, _stream(device.index)))
 
 
 def kv_copy(planes, rows: int, spans, *, max_rows: int) -> None:
@@ -228,12 +249,14 @@ def kv_copy(planes, rows: int, spans, *, max_rows: int) -> None:
     s_at = _ints("spans", spans, planes.device, dims=2)
     if spans.shape[1] != 3:
         _bad("kv_copy: spans are [n, 3]")
-    with _On(planes.device) as stream:
-        _check(load_library().lum_op_kv_copy(p_at, n, rows, s_at, spans.shape[0], max_rows, stream))
+    with _Here(planes.device.index):
+        _check(load_library().lum_op_kv_copy(p_at, n, rows, s_at, spans.shape[0], max_rows, _stream(planes.device.index)))
 
 
 def status(device=None) -> None:
     """Waits for the current stream of ``device`` and raises what a kernel of these operators found wrong since the last call."""
-    torch = _torch()
-    with _On(torch.device("cuda", torch.cuda.current_device()) if device is None else torch.device(device)) as stream:
-        _check(load_library().lum_op_status(stream))
+    _use_torch()
+    index = torch.device("cuda" if device is None else device).index
+    index = torch.cuda.current_device() if index is None else index
+    with _Here(index):
+        _check(load_library().lum_op_status(_stream(index)))
