@@ -371,6 +371,20 @@ int32_t lum_batch_begin_slots(lum_rt* rt, int32_t n_seq, const int32_t* slots, c
 int32_t lum_batch_decode(lum_rt* rt, int32_t n_steps);
 int32_t lum_batch_get_decoded(lum_rt* rt, int32_t* host_out, size_t n_steps);
 int32_t lum_batch_get_logits(lum_rt* rt, int32_t seq, float* host_out, size_t n);
+/* Speculative decoding (no counterpart in the reference, whose loop runs one token per step): one pass of the model over a tree of drafted
+ * tokens per sequence (the operators of lum_tree.h, in every layer), which says how many of them the model would have produced itself.
+ * Sequence s works on cache slot slots[s] (NULL: s), has positions[s] rows cached, and its nodes are row_start[s] .. row_start[s + 1] - 1 of
+ * `tokens` and `parents` (host arrays): node 0 is the token that comes next at positions[s] — what the step before ended with — with parent -1,
+ * every other node is a guess that follows its parent, an earlier node of the same tree (at most LUM_TREE_MAX_NODES).  A node's token stands
+ * if its parent stands and the sample there — greedy, or the draw of lum_set_sampling at that position — is this token: what comes out is
+ * what decoding token by token gives, up to rounding.  Asynchronous.  lum_draft_get waits and reads, per sequence, how many tokens
+ * follow node 0 (counts[s] >= 1: the guesses that stand and the sample behind them) and which (tokens_out [n_seq][len], len at least the
+ * nodes of the largest tree); the cache then holds positions[s] + counts[s] rows of the sequence (pages behind them have gone back), and the last
+ * token is node 0 of the next step.  The selected sequence's single-token steps (lum_decode_greedy) go on from there.
+ * Needs what lum_batch_begin needs, with max_batch 1 too. */
+int32_t lum_draft_verify(lum_rt* rt, int32_t n_seq, const int32_t* slots, const int32_t* positions, const int32_t* row_start, const int32_t* tokens,
+                         const int32_t* parents);
+int32_t lum_draft_get(lum_rt* rt, int32_t* counts, int32_t* tokens_out, size_t len);
 
 /* `Runtime::profile` (src/op.rs:18-23): time `trials` decode steps with CUDA events on the
  * runtime's stream (state is restored afterwards); returns mean microseconds per step and a

@@ -50,8 +50,8 @@ __global__ void __launch_bounds__(256) rope_append_rows(const RopeRowsArgs a) {
     const int per_row = (heads + 7) / 8, m = blockIdx.x / per_row, h = (blockIdx.x - m * per_row) * 8 + (tid >> 5);
     if (a.use_pdl) { pdl_launch_dependents(); pdl_grid_wait(); }
     const int pos = a.row_pos[m];
-    const int seq = a.row_seq ? a.row_seq[m] : a.seq0;
-    if (pos < 0 || pos >= a.max_seq || seq < 0 || seq >= a.max_batch) {
+    const int seq = a.row_seq ? a.row_seq[m] : a.seq0, at = a.row_at ? a.row_at[m] : pos;
+    if (pos < 0 || pos >= a.max_seq || at < 0 || at >= a.max_seq || seq < 0 || seq >= a.max_batch) {
         if (h == 0 && lane == 0) atomicOr(a.status, LUM_ST_BAD_POS);
         return;                                          // (the whole CTA: its warps share a row)
     }
@@ -110,7 +110,7 @@ __global__ void __launch_bounds__(256) rope_append_rows(const RopeRowsArgs a) {
     }
     const bool is_k = h < nq + nkv;
     void* cache = is_k ? a.k_cache : a.v_cache;
-    const size_t off = kv_phys_row(a.pg, seq, a.max_seq, pos) * ((size_t)nkv * HD) + (size_t)(h - nq - (is_k ? 0 : nkv)) * HD + lane;
+    const size_t off = kv_phys_row(a.pg, seq, a.max_seq, at) * ((size_t)nkv * HD) + (size_t)(h - nq - (is_k ? 0 : nkv)) * HD + lane;
 #pragma unroll
     for (int i = 0; i < N; i++) {
         if (a.kv_bf16) ((__nv_bfloat16*)cache)[off + 32 * i] = __float2bfloat16_rn(x[i]);

@@ -44,6 +44,7 @@ struct RopeRowsArgs {
     const int* row_pos;        // [M]
     const int* row_seq;        // [M] or null: every row belongs to sequence seq0
     int seq0;
+    const int* row_at;         // [M] or null: the cache row that row m is appended at, where that is not its position (drafted trees)
     float* q_rot;              // [M][n_q * hd]: rotated queries
     void* k_cache; void* v_cache;   // [max_batch][max_seq][n_kv * hd], or a pool of pages (pg)
     KvPages pg;

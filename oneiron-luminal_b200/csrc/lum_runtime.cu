@@ -29,6 +29,7 @@
 #include "lum_rows.cuh"
 #include "lum_moe.cuh"
 #include "lum_sample.cuh"
+#include "lum_tree.cuh"
 #include "lum_dense.cuh"
 
 using namespace lum;
@@ -227,6 +228,17 @@ struct lum_rt {
         RowOperand rec_hi{}, rec_lo{};                               // block_kind 2: operands of a recurrence's gates
         float *sub = nullptr, *u = nullptr, *rec_u = nullptr, *gates = nullptr;      // a sublayer's output, sum of the streams, convolved inputs, gates
     } rows;
+    // Drafted trees (lum_draft_verify): the last step's numbers on the host, its arrays on the device
+    struct Drafts {
+        int n_seq = 0;                    // sequences whose results are to be read
+        std::vector<int32_t> tokens, row_start, slot, position;
+        int* ints = nullptr; size_t ints_cap = 0;        // row_start, prefix, slot, then per row token, parent, place, cache row, slot, draw, pick
+        int* found = nullptr; size_t found_cap = 0;      // n_accepted, next, path
+        float* logits = nullptr; size_t logits_cap = 0;
+        char* ws = nullptr; size_t ws_cap = 0;
+    } drafts;
+    KvPlane* d_planes = nullptr;          // every layer run's K and V cache, for the kernels that move rows of all of them
+    int* d_span = nullptr;                // {source row, destination row, rows}
     float* yarn_inv = nullptr;        // rope_style 2: inverse-frequency table [head_dim / 2] on the device
     float yarn_factor_cs = 1.0f;      // ... and the factor on cos / sin
     float *moe_xf = nullptr, *moe_sw = nullptr, *moe_recv = nullptr, *moe_part = nullptr, *moe_comb = nullptr;   // MoE scratch (slots, gated activations, exchanges)
@@ -363,6 +375,7 @@ void free_model(lum_rt* rt) {
     if (rt->g_batch) cudaGraphExecDestroy(rt->g_batch);
     rt->g_batch = nullptr; rt->g_batch_n = 0; rt->batch_n = 0; rt->cur_seq = 0;
     rt->rows = lum_rt::Rows();
+    rt->drafts = lum_rt::Drafts(); rt->d_planes = nullptr; rt->d_span = nullptr;
     rt->b_step = nullptr; rt->b_log = nullptr;
     rt->v_first = nullptr; rt->pos_freq = nullptr; rt->u = nullptr; rt->n_streams = 0; rt->seq_state_bytes = 0; rt->seq_pos.clear();
     rt->want.clear(); rt->want_n = 0; rt->want_logits = nullptr; rt->want_cap = 0; rt->want_idx = nullptr; rt->want_idx_cap = 0;
@@ -499,6 +512,7 @@ int slot_layer_for_id(const lum_rt* rt, int slot, int layer) {
     return (slot == LUM_S_EMBED || slot == LUM_S_FINAL_NORM || slot == LUM_S_LM_HEAD || slot == LUM_S_FINAL_NORM_BIAS) ? rt->d.n_layers : layer;
 }
 
+__global__ void draft_state_kernel(DecodeState* st, int pos, int tok) { st->pos = pos; st->tok = tok; st->last_tok = tok; }
 __global__ void set_state_kernel(DecodeState* st, int pos, int tok, int log, int set_pos_tok, int reset_step) {
     if (set_pos_tok) { st->pos = pos; st->tok = tok; }
     if (log >= 0) st->log = log;
@@ -1063,6 +1077,40 @@ size_t kv_row_elems(const LayerW& w, int kind) { return kind ? w.v_elems : w.k_e
 size_t kv_row_bytes(const lum_rt* rt, const LayerW& w, int kind) { return kv_row_elems(w, kind) * (rt->d.kv_dtype == LUM_BF16 ? 2 : 4); }
 size_t kv_rows_total(const lum_rt* rt) { return rt->page_rows ? (size_t)rt->pool_pages * rt->page_rows : (size_t)rt->d.max_batch * rt->d.max_seq; }
 
+// Every layer run's K and V cache, as the kernels that move rows of all of them take them.
+bool kv_movable(const lum_rt* rt) {
+    for (const LayerW& w : rt->L)
+        if (kv_row_bytes(rt, w, 0) % 16 || kv_row_bytes(rt, w, 1) % 16 || (((uintptr_t)w.kc | (uintptr_t)w.vc) & 15)) return false;
+    return !rt->L.empty() && kv_rows_total(rt) <= 0x7fffffff && 2 * rt->L.size() <= 65535;
+}
+int kv_planes(lum_rt* rt) {
+    if (rt->d_planes) return 0;
+    std::vector<KvPlane> h;
+    for (const LayerW& w : rt->L) { h.push_back({w.kc, kv_row_bytes(rt, w, 0)}); h.push_back({w.vc, kv_row_bytes(rt, w, 1)}); }
+    KvPlane* d = nullptr;
+    if (!rt->d_span) if (int r = dev_alloc(rt, (void**)&rt->d_span, 3 * sizeof(int))) return r;
+    if (int r = dev_alloc(rt, (void**)&d, h.size() * sizeof(KvPlane))) return r;
+    CU(rt, cudaMemcpyAsync(d, h.data(), h.size() * sizeof(KvPlane), cudaMemcpyHostToDevice, rt->stream));     // pageable source: staged before the call returns
+    rt->d_planes = d;
+    return 0;
+}
+// n rows from row `src` of the caches (of the pool) to row `dst`, in every layer: one launch, where two copies a layer were queued one by one
+int kv_move(lum_rt* rt, size_t src, size_t dst, int n) {
+    if (!kv_movable(rt)) {
+        for (const LayerW& w : rt->L) {
+            const size_t kb = kv_row_bytes(rt, w, 0), vb = kv_row_bytes(rt, w, 1);
+            CU(rt, cudaMemcpyAsync((char*)w.kc + dst * kb, (const char*)w.kc + src * kb, n * kb, cudaMemcpyDeviceToDevice, rt->stream));
+            CU(rt, cudaMemcpyAsync((char*)w.vc + dst * vb, (const char*)w.vc + src * vb, n * vb, cudaMemcpyDeviceToDevice, rt->stream));
+        }
+        return 0;
+    }
+    if (int r = kv_planes(rt)) return r;
+    const int span[3] = {(int)src, (int)dst, n};
+    CU(rt, cudaMemcpyAsync(rt->d_span, span, sizeof span, cudaMemcpyHostToDevice, rt->stream));
+    CU(rt, launch_kv_copy(rt->d_planes, 2 * (int)rt->L.size(), (long long)kv_rows_total(rt), rt->d_span, 1, n, rt->status, rt->sm_count, rt->stream));
+    return 0;
+}
+
 int kv_page_upload(lum_rt* rt, int seq, int lp) {
     const size_t i = (size_t)seq * rt->pages_per_seq + lp;
     const int v = rt->h_page_table[i] < 0 ? 0 : rt->h_page_table[i];
@@ -1090,11 +1138,7 @@ int kv_ensure(lum_rt* rt, int seq, int from, int to) {
         int fresh = -1;
         if (int r = kv_page_take(rt, &fresh)) return r;
         if (e >= 0) {      // shared: copy what it holds, then let go of it
-            for (const LayerW& w : rt->L) {
-                const size_t kb = rt->page_rows * kv_row_bytes(rt, w, 0), vb = rt->page_rows * kv_row_bytes(rt, w, 1);
-                CU(rt, cudaMemcpyAsync((char*)w.kc + fresh * kb, (const char*)w.kc + e * kb, kb, cudaMemcpyDeviceToDevice, rt->stream));
-                CU(rt, cudaMemcpyAsync((char*)w.vc + fresh * vb, (const char*)w.vc + e * vb, vb, cudaMemcpyDeviceToDevice, rt->stream));
-            }
+            if (int r = kv_move(rt, (size_t)e * rt->page_rows, (size_t)fresh * rt->page_rows, rt->page_rows)) { kv_page_unref(rt, fresh); return r; }
             kv_page_unref(rt, e);
         }
         e = fresh;
@@ -1104,6 +1148,15 @@ int kv_ensure(lum_rt* rt, int seq, int from, int to) {
 }
 void kv_release_seq(lum_rt* rt, int seq) {
     for (int lp = 0; lp < rt->pages_per_seq; lp++) {
+        int& e = rt->h_page_table[(size_t)seq * rt->pages_per_seq + lp];
+        kv_page_unref(rt, e);
+        e = -1;
+    }
+}
+// The pages behind the first `rows` rows go back to the pool.
+void kv_trim_seq(lum_rt* rt, int seq, int rows) {
+    if (!rt->page_rows) return;
+    for (int lp = (rows + rt->page_rows - 1) >> rt->page_lg; lp < rt->pages_per_seq; lp++) {
         int& e = rt->h_page_table[(size_t)seq * rt->pages_per_seq + lp];
         kv_page_unref(rt, e);
         e = -1;
@@ -1392,10 +1445,28 @@ int run_rows_sequential(lum_rt* rt, int M, int* d_tok, int* d_pos, const int* d_
     return 0;
 }
 
+// room for `want` elements of a buffer of the drafted-tree steps, which grows
+template <typename T>
+int draft_room(lum_rt* rt, T** p, size_t* cap, size_t want) {
+    if (want <= *cap) return 0;
+    const size_t n = want + want / 2;
+    *cap = 0;
+    if (int r = dev_alloc(rt, (void**)p, n * sizeof(T))) return r;
+    *cap = n;
+    return 0;
+}
 // One pass of M rows through every layer.  d_tok / d_pos: device arrays [M]; d_seq: device array [M], or null when every row
 // belongs to sequence seq0.  head: 0 none (the rows only fill the cache), 1 vocabulary projection + greedy sample of the LAST row
-// into the decode state (the end of a prompt), 2 of every row into the batch state (batched decode).
-int run_rows(lum_rt* rt, int M, int* d_tok, int* d_pos, const int* d_seq, int seq0, int head) {
+// into the decode state (the end of a prompt), 2 of every row into the batch state (batched decode), 3 vocabulary projection of every row into
+// tree->logits (planes of *tree->parts K ranges).  tree: the rows are drafted trees; they lie at cache rows tree->at and attend as lum_op_attn_tree does.
+struct TreeRows { TreeBatch t; TreeMap m; const int* at; float* logits; void* ws; size_t ws_bytes; int parts; };
+TreeAttnArgs tree_attn_args(const lum_rt* rt, const TreeRows& tree) {
+    TreeAttnArgs a{};
+    a.t = tree.t; a.m = tree.m; a.n_q = rt->nq_l; a.n_kv = rt->nkv_l; a.hd = rt->d.head_dim; a.q_bf16 = 0; a.kv_bf16 = rt->d.kv_dtype == LUM_BF16; a.scale = 1.0f / sqrtf((float)rt->d.head_dim);
+    a.q_stride = a.out_stride = (long long)rt->nq_l * a.hd; a.kv_stride = (long long)rt->nkv_l * a.hd; a.ws = tree.ws; a.ws_bytes = tree.ws_bytes; a.status = rt->status;
+    return a;
+}
+int run_rows(lum_rt* rt, int M, int* d_tok, int* d_pos, const int* d_seq, int seq0, int head, TreeRows* tree = nullptr) {
     if (rt->d.block_kind == 1) return run_rows_blocks(rt, M, d_tok, d_pos, d_seq, seq0, head);
     if (rt->d.block_kind == 2) return run_rows_sequential(rt, M, d_tok, d_pos, d_seq, seq0, head);
     const lum_model_desc& d = rt->d;
@@ -1406,7 +1477,7 @@ int run_rows(lum_rt* rt, int M, int* d_tok, int* d_pos, const int* d_seq, int se
     const GemmShape g_qkv = gemm_shape(W, M, H, sms), g_o = gemm_shape(H, M, qd, sms), g_gu = gemm_shape(2 * F, M, H, sms), g_dn = gemm_shape(H, M, F, sms);
     // Up to five rows: the products on integer levels (lum_few.cu), where every K is one they take and the planes' buffers (of at least 32 rows) hold their K ranges
     const int r_h = few_ranges(H, sms), r_q = few_ranges(qd, sms), r_f = few_ranges(F, sms);
-    const bool few = M <= kFewMax && r_h && r_q && r_f && W % 8 == 0 && (head != 2 || (r_h == 1 && rt->lm_head.kc));
+    const bool few = M <= kFewMax && r_h && r_q && r_f && W % 8 == 0 && (head < 2 || (r_h == 1 && rt->lm_head.kc));
     const int ks_qkv = few ? r_h : g_qkv.ks, ks_o = few ? r_q : g_o.ks, ks_gu = few ? r_h : g_gu.ks, ks_dn = few ? r_f : g_dn.ks;
     b.down_parts = ks_dn;
     CU(rt, launch_embed_rows(rt->embed.w, rt->embed.kind, H, d.vocab, d_tok, b.xr, M, rt->status, st));
@@ -1448,6 +1519,7 @@ int run_rows(lum_rt* rt, int M, int* d_tok, int* d_pos, const int* d_seq, int se
         {
             RopeRowsArgs t{};
             t.qkv = b.qkv; t.n_parts = ks_qkv; t.part_stride = (size_t)M * W; t.row_pos = d_pos; t.row_seq = d_seq; t.seq0 = seq0;
+            t.row_at = tree ? tree->at : nullptr;
             t.q_rot = b.q_rot; t.k_cache = w.kc; t.v_cache = w.vc; t.pg = kv_pages(rt);
             t.q_gain = d.qk_norm ? w.q_norm.w : nullptr; t.k_gain = d.qk_norm ? w.k_norm.w : nullptr; t.gain_kind = gk; t.qk_eps = d.rms_eps;
             t.M = M; t.n_q = rt->nq_l; t.n_kv = rt->nkv_l; t.hd = hd; t.kv_bf16 = d.kv_dtype == LUM_BF16; t.rope_style = d.rope_style;
@@ -1461,7 +1533,11 @@ int run_rows(lum_rt* rt, int M, int* d_tok, int* d_pos, const int* d_seq, int se
             a.status = rt->status; a.use_pdl = pdl;
             // many rows of one sequence (a prompt): the tensor-core kernel; few rows, or rows of different sequences: one CTA per row
             static const int env_tc = [] { const char* e = getenv("LUM_ATTN_TC"); return e ? atoi(e) : 1; }();
-            if (env_tc && M >= 16 && attn_prompt_tc_supported(a)) CU(rt, launch_attn_prompt_tc(a, st));
+            if (tree) {
+                TreeAttnArgs x = tree_attn_args(rt, *tree);
+                x.q = b.q_rot; x.k = w.kc; x.v = w.vc; x.out = b.attn;
+                CU(rt, launch_tree_attn(x, sms, st));
+            } else if (env_tc && M >= 16 && attn_prompt_tc_supported(a)) CU(rt, launch_attn_prompt_tc(a, st));
             else CU(rt, launch_attn_rows(a, sms, st));
             launches += 2;
         }
@@ -1514,7 +1590,7 @@ int run_rows(lum_rt* rt, int M, int* d_tok, int* d_pos, const int* d_seq, int se
             CU(rt, launch_sample_rows(sa, st));
             launches++;
         }
-    } else if (head == 2) {
+    } else if (head >= 2) {
         RowsArgs r{};
         r.a = b.down; r.n_parts = ks_dn; r.part_stride = (size_t)M * H; r.ld = H; r.resid = b.xr; r.resid_ld = H; r.out = b.xr; r.out_ld = H;
         r.gain = rt->final_norm.w; r.gain_kind = gk; r.eps = rt->eps6;
@@ -1523,8 +1599,9 @@ int run_rows(lum_rt* rt, int M, int* d_tok, int* d_pos, const int* d_seq, int se
         CU(rt, quant(r, H, g_v));
         GemmArgs g{};
         g.nseg = 1; g.seg[0] = {(const unsigned char*)rt->lm_head.w, V, 0};
-        CU(rt, gemm(g, H, g_v, b.logits, V));
-        if (int r2 = batch_sample(rt, M, d_tok, d_pos, d_seq, few ? r_h : g_v.ks, &launches)) return r2;
+        CU(rt, gemm(g, H, g_v, tree ? tree->logits : b.logits, V));
+        if (tree) tree->parts = few ? r_h : g_v.ks;
+        else if (int r2 = batch_sample(rt, M, d_tok, d_pos, d_seq, few ? r_h : g_v.ks, &launches)) return r2;
     }
     rt->n_launches += launches;
     return 0;
@@ -2494,21 +2571,11 @@ int32_t lum_kv_copy(lum_rt* rt, int32_t src_seq, int32_t dst_seq, int32_t rows) 
         if (rest) {
             if (int r = kv_ensure(rt, dst_seq, full * rt->page_rows, rows)) return r;
             const int se = rt->h_page_table[(size_t)src_seq * rt->pages_per_seq + full], de = rt->h_page_table[(size_t)dst_seq * rt->pages_per_seq + full];
-            for (const LayerW& w : rt->L) {
-                const size_t kb = kv_row_bytes(rt, w, 0), vb = kv_row_bytes(rt, w, 1), pr = rt->page_rows;
-                CU(rt, cudaMemcpyAsync((char*)w.kc + de * pr * kb, (const char*)w.kc + se * pr * kb, rest * kb, cudaMemcpyDeviceToDevice, rt->stream));
-                CU(rt, cudaMemcpyAsync((char*)w.vc + de * pr * vb, (const char*)w.vc + se * pr * vb, rest * vb, cudaMemcpyDeviceToDevice, rt->stream));
-            }
+            if (int r = kv_move(rt, (size_t)se * rt->page_rows, (size_t)de * rt->page_rows, rest)) return r;
         }
         return 0;
     }
-    const size_t ms = (size_t)rt->d.max_seq;
-    for (const LayerW& w : rt->L) {
-        const size_t kb = kv_row_bytes(rt, w, 0), vb = kv_row_bytes(rt, w, 1);
-        CU(rt, cudaMemcpyAsync((char*)w.kc + dst_seq * ms * kb, (const char*)w.kc + src_seq * ms * kb, rows * kb, cudaMemcpyDeviceToDevice, rt->stream));
-        CU(rt, cudaMemcpyAsync((char*)w.vc + dst_seq * ms * vb, (const char*)w.vc + src_seq * ms * vb, rows * vb, cudaMemcpyDeviceToDevice, rt->stream));
-    }
-    return 0;
+    return kv_move(rt, (size_t)src_seq * rt->d.max_seq, (size_t)dst_seq * rt->d.max_seq, rows);
 }
 
 int32_t lum_kv_release(lum_rt* rt, int32_t seq) {
@@ -2705,6 +2772,128 @@ int32_t lum_batch_get_logits(lum_rt* rt, int32_t seq, float* host_out, size_t n)
     CU(rt, cudaMemcpyAsync(host_out, rt->rows.logits + (size_t)seq * rt->vocab_l, n * 4, cudaMemcpyDeviceToHost, rt->stream));
     CU(rt, cudaStreamSynchronize(rt->stream));
     return check_status(rt);
+}
+
+// ---- drafted trees -------------------------------------------------------------------------------------------------------
+
+int32_t lum_draft_verify(lum_rt* rt, int32_t n_seq, const int32_t* slots, const int32_t* positions, const int32_t* row_start, const int32_t* tokens, const int32_t* parents) {
+    if (!rt || !rt->has_model || !positions || !row_start || !tokens || !parents) return fail(rt, LUM_E_INVALID, "draft_verify: no model or null argument");
+    if (rt->d.block_kind != 0 || !rows_supported(rt) || rt->d.tied_head || !rt->lm_head.kc || (rt->mega_ok && rt->use_mega))
+        return fail(rt, LUM_E_UNSUPPORTED, "draft_verify needs packed Q8_0 weights with a Q8_0 vocabulary projection on one GPU, and an executor of one kernel per operation");
+    if (n_seq < 1 || n_seq > rt->max_batch) return fail(rt, LUM_E_INVALID, "draft_verify: %d sequences, the model was loaded with max_batch %d", n_seq, rt->max_batch);
+    if (row_start[0] != 0) return fail(rt, LUM_E_INVALID, "draft_verify: the first sequence's rows start at %d, not 0", row_start[0]);
+    std::vector<char> taken((size_t)rt->max_batch, 0);
+    lum_rt::Drafts& w = rt->drafts;
+    w.n_seq = 0;
+    std::vector<int32_t> place, at, seq, draw, slot((size_t)n_seq);
+    int max_rows = 1, max_prefix = 0;
+    for (int s = 0; s < n_seq; s++) {
+        const int n = row_start[s + 1] - row_start[s], p = positions[s], sl = slots ? slots[s] : s;
+        if (n < 1 || n > kTreeMax) return fail(rt, LUM_E_INVALID, "draft_verify: %d nodes for sequence %d (1 .. %d)", n, s, kTreeMax);
+        if (sl < 0 || sl >= rt->max_batch || taken[(size_t)sl]) return fail(rt, LUM_E_INVALID, "draft_verify: cache slot %d is outside max_batch %d or named twice", sl, rt->max_batch);
+        if (p < 0 || p > rt->d.max_seq - n) return fail(rt, LUM_E_INVALID, "draft_verify: %d nodes behind position %d pass the cache capacity %d", n, p, rt->d.max_seq);
+        taken[(size_t)sl] = 1;
+        slot[(size_t)s] = sl;
+        if (n > max_rows) max_rows = n;
+        if (p > max_prefix) max_prefix = p;
+        for (int i = 0; i < n; i++) {
+            const int t = tokens[row_start[s] + i], up = parents[row_start[s] + i];
+            if (t < 0 || t >= rt->d.vocab) return fail(rt, LUM_E_INVALID, "draft_verify: token id %d outside the vocabulary", t);
+            if (i == 0 ? up != -1 : up < 0 || up >= i) return fail(rt, LUM_E_INVALID, "draft_verify: node %d of sequence %d has the parent %d (node 0 has -1, the others an earlier node)", i, s, up);
+            place.push_back(i ? place[(size_t)(row_start[s] + up)] + 1 : p);
+            at.push_back(p + i);
+            seq.push_back(sl);
+            draw.push_back(place.back() + 1);
+        }
+    }
+    const int M = row_start[n_seq];
+    CU(rt, cudaSetDevice(rt->cfg.device));
+    if (int r = ensure_rows(rt, 1)) return r;
+    if (M > rt->rows.cap) return fail(rt, LUM_E_INVALID, "draft_verify: %d nodes in all, a pass takes %d", M, rt->rows.cap);
+    if (!kv_movable(rt)) return fail(rt, LUM_E_UNSUPPORTED, "draft_verify: cache rows that are no multiple of 16 bytes, or 2^31 of them");
+    if (int r = kv_planes(rt)) return r;
+    for (int s = 0; s < n_seq; s++) if (int r = kv_ensure(rt, slot[(size_t)s], positions[s], positions[s] + row_start[s + 1] - row_start[s])) return r;
+    // one upload: row_start, prefix, slot, then per row token, parent, place, cache row, slot, position of the token drawn there (and room for the picks)
+    const size_t n = (size_t)n_seq, R = (size_t)M;
+    std::vector<int32_t> up(row_start, row_start + n + 1);
+    up.insert(up.end(), positions, positions + n);
+    up.insert(up.end(), slot.begin(), slot.end());
+    const size_t rows0 = up.size();
+    up.insert(up.end(), tokens, tokens + R);
+    up.insert(up.end(), parents, parents + R);
+    for (const std::vector<int32_t>* v : {&place, &at, &seq, &draw}) up.insert(up.end(), v->begin(), v->end());
+    if (int r = draft_room(rt, &w.ints, &w.ints_cap, up.size() + R)) return r;
+    CU(rt, cudaMemcpyAsync(w.ints, up.data(), up.size() * 4, cudaMemcpyHostToDevice, rt->stream));            // pageable source: staged before the call returns
+    int *d_tok = w.ints + rows0, *d_parent = d_tok + R, *d_place = d_parent + R, *d_at = d_place + R, *d_seq = d_at + R, *d_draw = d_seq + R, *d_pick = d_draw + R;
+    TreeRows tree{};
+    tree.t = {w.ints, w.ints + n + 1, d_parent, w.ints + 2 * n + 1, n_seq, M, max_rows, max_prefix};
+    tree.m = {rt->page_rows ? rt->d_page_table : nullptr, (long long)kv_rows_total(rt), rt->max_batch, rt->d.max_seq, rt->page_rows ? rt->page_lg : -1, rt->pages_per_seq};
+    tree.at = d_at;
+    const TreeAttnArgs probe = tree_attn_args(rt, tree);
+    const size_t attn_ws = tree_attn_workspace(probe, rt->sm_count), accept_ws = tree_accept_workspace(tree.t, rt->vocab_l, rt->sm_count);
+    if (int r = draft_room(rt, &w.ws, &w.ws_cap, attn_ws > accept_ws ? attn_ws : accept_ws)) return r;
+    if (int r = draft_room(rt, &w.found, &w.found_cap, 2 * n + n * (size_t)max_rows)) return r;
+    if (int r = draft_room(rt, &w.logits, &w.logits_cap, rows_parts_floats(rt, rt->vocab_l, rt->d.hidden, M))) return r;
+    tree.ws = w.ws; tree.ws_bytes = w.ws_cap; tree.logits = w.logits;
+    if (int r = run_rows(rt, M, d_tok, d_place, d_seq, 0, 3, &tree)) return r;
+    TreeAcceptArgs a{};
+    a.t = tree.t; a.tokens = d_tok; a.vocab = rt->vocab_l; a.ld = rt->vocab_l; a.path = w.found + 2 * n; a.path_len = max_rows; a.n_accepted = w.found; a.next = w.found + n;
+    a.ws = w.ws; a.ws_bytes = w.ws_cap; a.status = rt->status;
+    if (tree.parts > 1 || rt->sampling) {                // the planes are added up and the greedy picks come with it; a sampler draws from the sums
+        ArgmaxRowsArgs x{};
+        x.logits = w.logits; x.n_parts = tree.parts; x.part_stride = R * rt->vocab_l; x.M = M; x.vocab = rt->vocab_l; x.best = d_pick; x.use_pdl = rt->rows_pdl;
+        CU(rt, launch_argmax_rows(x, rt->stream));
+        rt->n_launches++;
+        if (rt->sampling) {
+            SampleArgs sa{};
+            sa.logits = w.logits; sa.row_stride = (size_t)rt->vocab_l; sa.M = M; sa.vocab = rt->vocab_l; sa.params = rt->d_sample; sa.row_seq = d_seq; sa.draw_pos = d_draw; sa.out = d_pick;
+            CU(rt, launch_sample_rows(sa, rt->stream));
+            rt->n_launches++;
+        }
+        a.picks = d_pick;
+    } else a.logits = w.logits;
+    CU(rt, launch_tree_accept(a, rt->sm_count, rt->stream));
+    CU(rt, launch_kv_compact(rt->d_planes, 2 * (int)rt->L.size(), tree.m, tree.t, a.path, a.path_len, a.n_accepted, rt->status, rt->sm_count, rt->stream));
+    rt->n_launches += 2;
+    rt->n_tokens_run += R;
+    w.tokens.assign(tokens, tokens + R);
+    w.row_start.assign(row_start, row_start + n + 1);
+    w.position.assign(positions, positions + n);
+    w.slot = slot;
+    w.n_seq = n_seq;
+    return 0;
+}
+
+int32_t lum_draft_get(lum_rt* rt, int32_t* counts, int32_t* tokens_out, size_t len) {
+    if (!rt || !rt->has_model || !counts || !tokens_out) return fail(rt, LUM_E_INVALID, "draft_get: no model or null output");
+    lum_rt::Drafts& w = rt->drafts;
+    if (!w.n_seq) return fail(rt, LUM_E_INVALID, "draft_get: call lum_draft_verify first (its results are read once)");
+    const size_t n = (size_t)w.n_seq;
+    int max_rows = 1;
+    for (size_t s = 0; s < n; s++) if (w.row_start[s + 1] - w.row_start[s] > max_rows) max_rows = w.row_start[s + 1] - w.row_start[s];
+    if (len < (size_t)max_rows) return fail(rt, LUM_E_INVALID, "draft_get: room for %zu tokens per sequence, up to %d may follow", len, max_rows);
+    CU(rt, cudaSetDevice(rt->cfg.device));
+    std::vector<int32_t> got(2 * n + n * (size_t)max_rows);
+    CU(rt, cudaMemcpyAsync(got.data(), w.found, got.size() * 4, cudaMemcpyDeviceToHost, rt->stream));
+    CU(rt, cudaStreamSynchronize(rt->stream));
+    w.n_seq = 0;
+    if (int r = check_status(rt)) return r;
+    for (size_t s = 0; s < n; s++) {
+        const int k = got[s], next = got[n + s];
+        const int32_t* path = got.data() + 2 * n + s * (size_t)max_rows;
+        if (k < 1 || k > max_rows) return fail(rt, LUM_E_DEVICE, "draft_get: %d nodes of sequence %zu stand", k, s);
+        counts[s] = k;
+        for (int i = 1; i < k; i++) tokens_out[s * len + (size_t)i - 1] = w.tokens[(size_t)(w.row_start[s] + path[i])];
+        tokens_out[s * len + (size_t)k - 1] = next;
+        const int rows = w.position[s] + k;
+        kv_trim_seq(rt, w.slot[s], rows);
+        if (w.slot[s] == rt->cur_seq) {                  // single-token steps go on from here
+            draft_state_kernel<<<1, 1, 0, rt->stream>>>(rt->state, rows, next);
+            CU(rt, cudaGetLastError());
+            rt->h_next_pos = rows;
+        }
+    }
+    return 0;
 }
 
 // Test hook: makes a bounded wait run out.  Runs layer 0's q | k | v projection with one extra partial vector that never

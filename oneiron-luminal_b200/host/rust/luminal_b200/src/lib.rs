@@ -21,6 +21,7 @@
 pub mod ffi;
 pub mod ops;
 pub mod runtime;
+pub mod tree;
 pub mod wire;
 
 pub use runtime::{B200Arg, B200Error, B200Runtime};

@@ -299,6 +299,8 @@ def load_library() -> C.CDLL:
         "lum_batch_decode": (i32, [vp, i32]),
         "lum_batch_get_decoded": (i32, [vp, P(i32), sz]),
         "lum_batch_get_logits": (i32, [vp, i32, P(C.c_float), sz]),
+        "lum_draft_verify": (i32, [vp, i32, P(i32), P(i32), P(i32), P(i32), P(i32)]),
+        "lum_draft_get": (i32, [vp, P(i32), P(i32), sz]),
         "lum_profile": (i32, [vp, i32, P(C.c_double), C.c_char_p, sz]),
         "lum_launches_per_step": (i32, [vp, P(i32)]),
         "lum_stream": (vp, [vp]),
@@ -811,6 +813,26 @@ class B200Runtime:
         out = np.empty(self.desc.vocab, dtype=np.float32)
         self._ck(self._lib.lum_batch_get_logits(self._h, seq, out.ctypes.data_as(C.POINTER(C.c_float)), out.size))
         return out
+
+    def draft_verify(self, trees, positions: Sequence[int], slots: Optional[Sequence[int]] = None) -> List[List[int]]:
+        """One pass of the model over a tree of drafted tokens per sequence: ``trees[s]`` = (tokens, parents), node 0 the token that comes next at
+        ``positions[s]`` (parent -1), the others guesses that follow an earlier node.  Returns the tokens that follow node 0 of every sequence, at
+        least one: the guesses the model would have sampled itself and the sample behind them.  The cache keeps their rows (all but the last token's)."""
+        ints = lambda v: (C.c_int32 * max(1, len(v)))(*[int(x) for x in v])  # noqa: E731
+        start, tokens, parents = [0], [], []
+        for t, p in trees:
+            if len(t) != len(p):
+                raise LumError(-1, f"draft_verify: {len(t)} tokens and {len(p)} parents")
+            tokens += list(t)
+            parents += list(p)
+            start.append(len(tokens))
+        n, most = len(start) - 1, max([len(t) for t, _ in trees], default=1)
+        if len(positions) != n or (slots is not None and len(slots) != n):
+            raise LumError(-1, f"draft_verify: {n} trees, {len(positions)} positions, {n if slots is None else len(slots)} slots")
+        self._ck(self._lib.lum_draft_verify(self._h, n, None if slots is None else ints(slots), ints(positions), ints(start), ints(tokens), ints(parents)))
+        counts, out = (C.c_int32 * n)(), (C.c_int32 * (n * most))()
+        self._ck(self._lib.lum_draft_get(self._h, counts, out, most))
+        return [[int(out[s * most + i]) for i in range(counts[s])] for s in range(n)]
 
     def profile(self, trials: int = 16):
         us = C.c_double()

@@ -9,6 +9,10 @@ a new request's slot on the device instead of being recomputed.  With a paged ca
 the pool can hold its whole life (prompt and every token it may generate) next to what is already promised, and gives a
 finished request's pages back.
 
+With a ``drafter`` the steps are speculative: every live sequence brings a tree of guesses of what follows its last token, one pass of
+the model verifies them all (``draft_verify``), and a sequence moves on by as many tokens as it guessed right, plus one — the tokens are
+those of plain decoding.  :class:`PromptLookup` is a drafter that needs no second model.
+
 Everything here is host-side bookkeeping over four calls of the runtime: ``seq_select`` + ``execute`` (admission),
 ``kv_copy`` (prefix reuse), ``batch_begin_slots`` + ``batch_decode`` (the steps).  The runtime object only needs those methods
 plus ``set_data``, ``get_token``, ``batch_get_decoded`` and ``desc.max_batch`` / ``desc.max_seq`` / ``desc.max_new_tokens``.
@@ -40,13 +44,54 @@ class Request:
         return self.tokens[-1]
 
 
+class PromptLookup:
+    """Guesses that the text goes on as it did before: where the last ``match`` tokens (or fewer, down to one) occurred earlier in a sequence, what
+    followed them there, up to ``length`` tokens.  The ``places`` most recent such places are branches of the tree; what they have in common is one
+    path of it."""
+
+    def __init__(self, length: int = 8, match: int = 3, places: int = 2):
+        if length < 1 or match < 1 or places < 1:
+            raise ValueError("length, match and places must be at least 1")
+        self.length, self.match, self.places = length, match, places
+
+    def __call__(self, text: Sequence[int], room: int) -> Tuple[List[int], List[int]]:
+        text, room = list(text), min(room, self.length * self.places)
+        tokens: List[int] = []
+        parents: List[int] = []
+        for n in range(min(self.match, len(text) - 1), 0, -1):
+            tail, found = text[-n:], 0
+            for i in range(len(text) - n - 1, -1, -1):
+                if text[i:i + n] != tail:
+                    continue
+                at = 0                                   # node 0 is the last token of the text
+                for t in text[i + n:i + n + self.length]:
+                    known = [j + 1 for j in range(len(tokens)) if parents[j] == at and tokens[j] == t]
+                    if known:
+                        at = known[0]
+                    elif len(tokens) < room:
+                        tokens.append(t)
+                        parents.append(at)
+                        at = len(tokens)
+                    else:
+                        break
+                found += 1
+                if found == self.places:
+                    break
+            if tokens:
+                break
+        return tokens, parents
+
+
 class ContinuousBatcher:
     """Keeps up to ``max_batch`` (minus parked prefixes) sequences decoding together and refills slots as requests end."""
 
-    def __init__(self, rt, steps_per_round: int = 8):
+    def __init__(self, rt, steps_per_round: int = 8, drafter=None):
+        """``drafter(text, room)``: at most ``room`` guesses of what follows the tokens ``text``, as (tokens, parents) with parent 0 = the last
+        token of the text and parent k = the k-th guess, which comes before its children (None: plain steps)."""
         if steps_per_round < 1:
             raise ValueError("steps_per_round must be at least 1")
         self.rt = rt
+        self.drafter = drafter
         self.steps_per_round = steps_per_round
         self.free: List[int] = list(range(rt.desc.max_batch))[::-1]      # pop() hands out slot 0 first
         self.queue: Deque[Request] = deque()
@@ -66,7 +111,9 @@ class ContinuousBatcher:
         self.promised = 0           # pages promised to live requests and parked prefixes
         self.rounds = 0
         self.steps_run = 0          # batched steps issued
-        self.rows_run = 0           # rows those steps carried (sum of live sequences per step)
+        self.rows_run = 0           # rows those steps carried (sum of live sequences per step; with a drafter, of nodes)
+        self.drafted = 0            # guesses made, and those that stood
+        self.stood = 0
 
     # ---- requests ------------------------------------------------------------------------------------------------
     def submit(self, prompt: Sequence[int], max_new: int, eos: Optional[Iterable[int]] = None) -> int:
@@ -147,7 +194,11 @@ class ContinuousBatcher:
             if self.page_rows and self.promised + self._pages_for(len(nxt.prompt) + nxt.max_new) > self.pool_pages:
                 break                                    # first come, first served: it waits for pages, nobody overtakes it
             self._admit(self.queue.popleft(), self.free.pop())
-        if self.live:
+        if self.live and self.drafter is not None:
+            for _ in range(self.steps_per_round):
+                if self.live and not self._speculate():
+                    break
+        elif self.live:
             slots = sorted(self.live)
             reqs = [self.live[s] for s in slots]
             n = min(self.steps_per_round, self.rt.desc.max_new_tokens, min(r.max_new - len(r.tokens) for r in reqs))
@@ -166,11 +217,40 @@ class ContinuousBatcher:
         self.rounds += 1
         return [self.finished[i] for i in sorted(set(self.finished) - before)]
 
+    def _speculate(self) -> bool:
+        """One speculative step of every live sequence.  False: a request has ended, its slot can be filled."""
+        slots = sorted(self.live)
+        reqs = [self.live[s] for s in slots]
+        trees = []
+        for r in reqs:
+            # guesses that could all stand without passing what the request may still generate (the sample behind them is one more)
+            room = min(r.max_new - len(r.tokens) - 1, self.max_nodes - 1)
+            tokens, parents = self.drafter(r.prompt + r.tokens, room) if room > 0 else ([], [])
+            if len(tokens) > room or len(tokens) != len(parents) or any(not 0 <= p <= i for i, p in enumerate(parents)):
+                raise ValueError(f"the drafter returned {len(tokens)} tokens and {len(parents)} parents for room {room}, or a parent that is no earlier guess")
+            trees.append(([r.cur] + [int(t) for t in tokens], [-1] + [int(p) for p in parents]))
+        self.steps_run += 1
+        ended = False
+        for r, (tokens, _), new in zip(reqs, trees, self.rt.draft_verify(trees, [r.pos for r in reqs], slots)):
+            self.rows_run += len(tokens)
+            self.drafted += len(tokens) - 1
+            self.stood += len(new) - 1
+            r.pos += len(new)
+            for t in new:
+                r.tokens.append(int(t))
+                if r.tokens[-1] in r.eos:
+                    break                                # what was decoded after its end is dropped
+            self._check_done(r)
+            ended = ended or r.done
+        return not ended
+
+    max_nodes = 64                  # nodes of a tree
+
     def stats(self) -> Dict[str, float]:
         """Counters of the loop so far: how full the batched steps were is what decides the tokens/s of a server."""
         return {"rounds": self.rounds, "steps": self.steps_run, "rows": self.rows_run,
                 "rows_per_step": self.rows_run / self.steps_run if self.steps_run else 0.0,
-                "live": len(self.live), "queued": len(self.queue), "finished": len(self.finished),
+                "drafted": self.drafted, "stood": self.stood, "live": len(self.live), "queued": len(self.queue), "finished": len(self.finished),
                 "pages_promised": self.promised, "pages_in_pool": self.pool_pages}
 
     def run(self) -> Dict[int, List[int]]:
