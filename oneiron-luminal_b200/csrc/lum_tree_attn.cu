@@ -105,18 +105,20 @@ __device__ __forceinline__ int4 piece_find(const TreeAttnArgs& a, const Share& p
     for (int s0 = 32; s0 < a.t.n_seq; s0 += 32) { const SeqWork x = work(s0 + lane); units += x.units; total += x.units * x.tiles; }
     units = __reduce_add_sync(0xffffffffu, units);
     total = __reduce_add_sync(0xffffffffu, total);
-    const float even = (float)total / (float)p.slots;
-    int per = (int)(2.0f * even) + 1;
-    if (units < p.slots) {
-        per = (int)even + 1;
+    // Little work: a CTA on every SM, of two tiles at least, rather than two (which begin at the same time and get in each other's way)
+    const int slots = total < 4 * p.slots ? p.slots / 2 : p.slots;
+    const float even = (float)total / (float)slots;
+    int per = p.shares ? (int)(2.0f * even) + 2 : 1 << 30;
+    if (p.shares && units < slots) {
+        per = max((int)even + 1, 2);
 #pragma unroll 1
         for (int i = 0; i < 2; i++) {
             int n = mine.units * pieces_of(mine.tiles, per);
 #pragma unroll 1
             for (int s0 = 32; s0 < a.t.n_seq; s0 += 32) { const SeqWork x = work(s0 + lane); n += x.units * pieces_of(x.tiles, per); }
             n = __reduce_add_sync(0xffffffffu, n);
-            if (n <= p.slots) break;
-            per = i ? total / (p.slots - units) + 1 : (int)((float)per * (float)n / (float)p.slots) + 1;
+            if (n <= slots) break;
+            per = i ? total / (slots - units) + 1 : (int)((float)per * (float)n / (float)slots) + 1;
         }
     }
     *per_out = per;
@@ -313,8 +315,8 @@ __global__ void __launch_bounds__(256) attn_tree_rows(const TreeAttnArgs a, cons
 //     thousands of keys the cuts add up.  Low terms go first.
 // A key that a row does not see has weight 0, but 0 times infinity is no zero: rows of V behind the last node or before the window are zeroed, and a row whose
 // result is not finite is computed again by tree_row_plain, key by key.
-constexpr int kTcThreads = 224;                     // four softmax warps, K, products, V
 constexpr int kTcGroup = 128 * 16 + 16;              // f32 queries' terms: 16-byte column groups of 128 rows, the next one 16 bytes further on (banks)
+constexpr int kTcThreads = 224;                     // four softmax warps, keys, products, values
 template <int HD, bool F32>
 struct TcShape {
     static constexpr int q_terms = F32 ? 3 : 1, p_terms = F32 ? 3 : 2;
@@ -361,24 +363,25 @@ template <> __device__ __forceinline__ void tc_st<32>(uint32_t at, const uint32_
 }
 __device__ __forceinline__ void tc_st_wait() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
 __device__ __forceinline__ float tc_ex2(float x) { float y; asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x)); return y; }
-// two at a time: the softmax warps are bound by what they issue (beside their exponentials)
-__device__ __forceinline__ float2 fma2(float2 a, float2 b, float2 c) {
-    float2 d;
-    asm("{\n\t.reg .b64 a, b, c, d;\n\tmov.b64 a, {%2, %3};\n\tmov.b64 b, {%4, %5};\n\tmov.b64 c, {%6, %7};\n\tfma.rn.f32x2 d, a, b, c;\n\tmov.b64 {%0, %1}, d;\n\t}"
-        : "=f"(d.x), "=f"(d.y) : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y), "f"(c.x), "f"(c.y));
-    return d;
-}
-__device__ __forceinline__ float2 add2(float2 a, float2 b) {
-    float2 d;
-    asm("{\n\t.reg .b64 a, b, d;\n\tmov.b64 a, {%2, %3};\n\tmov.b64 b, {%4, %5};\n\tadd.rn.f32x2 d, a, b;\n\tmov.b64 {%0, %1}, d;\n\t}"
-        : "=f"(d.x), "=f"(d.y) : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y));
-    return d;
-}
-// (x0, x1) as packed bf16, rounded; what is left of them goes back
-__device__ __forceinline__ uint32_t tc_term(float* x0, float* x1) {
-    const __nv_bfloat162 h = __floats2bfloat162_rn(*x0, *x1);
+// Pairs of floats in 64-bit registers: the softmax warps are bound by what they issue, and these issue once for two.
+using F2 = unsigned long long;
+__device__ __forceinline__ F2 pack2(float a, float b) { F2 r; asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(a), "f"(b)); return r; }
+__device__ __forceinline__ F2 pack2(uint32_t a, uint32_t b) { F2 r; asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "r"(a), "r"(b)); return r; }
+__device__ __forceinline__ float2 unpack2(F2 x) { float2 r; asm("mov.b64 {%0, %1}, %2;" : "=f"(r.x), "=f"(r.y) : "l"(x)); return r; }
+__device__ __forceinline__ F2 fma2(F2 a, F2 b, F2 c) { F2 r; asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c)); return r; }
+__device__ __forceinline__ F2 add2(F2 a, F2 b) { F2 r; asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b)); return r; }
+// x as packed bf16, rounded; what is left of it goes back
+__device__ __forceinline__ uint32_t tc_term(F2* x, F2 minus_one) {
+    const float2 y = unpack2(*x);
+    const __nv_bfloat162 h = __floats2bfloat162_rn(y.x, y.y);
     const uint32_t b = *(const uint32_t*)&h;
-    const float2 r = fma2(make_float2(__uint_as_float(b << 16), __uint_as_float(b & 0xffff0000u)), make_float2(-1.0f, -1.0f), make_float2(*x0, *x1));
+    *x = fma2(pack2(b << 16, b & 0xffff0000u), minus_one, *x);
+    return b;
+}
+__device__ __forceinline__ uint32_t tc_term(float* x0, float* x1) {
+    F2 x = pack2(*x0, *x1);
+    const uint32_t b = tc_term(&x, pack2(-1.0f, -1.0f));
+    const float2 r = unpack2(x);
     *x0 = r.x; *x1 = r.y;
     return b;
 }
@@ -590,7 +593,7 @@ __global__ void __launch_bounds__(kTcThreads, TcShape<HD, F32>::ctas) attn_tree_
             tree_load(tree, a.t, q, a.window, tid, 128, 1, a.status);
             named_sync(1, 128);
         }
-        const int grp = warp / (4 / DUP), warp_row = warp % (4 / DUP) * 32, row = warp_row + lane, f = f0 + row, node = row < live_rows ? node_of(f) : -1;
+        const int grp = warp / (4 / DUP), warp_row = warp % (4 / DUP) * 32, col = grp * KPT, row = warp_row + lane, f = f0 + row, node = row < live_rows ? node_of(f) : -1;
         const bool live = warp_row < live_rows;      // a warp without live rows leaves its rows of P as they are: nobody reads what they make
         float m_run = -INFINITY, l_run = 0.0f;
         float o[F32 ? HD : 1];
@@ -616,7 +619,7 @@ __global__ void __launch_bounds__(kTcThreads, TcShape<HD, F32>::ctas) attn_tree_
                 const uint32_t sc = mine + (uint32_t)b * 64u;
                 float v[KPT];
 #pragma unroll
-                for (int c = 0; c < KPT; c += KPT < 32 ? KPT : 32) tc_ld<(KPT < 32 ? KPT : 32)>(sc + grp * KPT + c, (uint32_t*)v + c);
+                for (int c = 0; c < KPT; c += KPT < 32 ? KPT : 32) tc_ld<(KPT < 32 ? KPT : 32)>(sc + col + c, (uint32_t*)v + c);
                 tmem_ld_wait();
                 if (j0 + kTileKeys > q.prefix || a.window > 0) {     // some key may be out of some row's sight
                     unsigned long long see = 0ull;
@@ -631,7 +634,7 @@ __global__ void __launch_bounds__(kTcThreads, TcShape<HD, F32>::ctas) attn_tree_
                             if (32 * k < q.n && at < 64 && at > -32) see |= at >= 0 ? (unsigned long long)tree.anc[node][k] << at : (unsigned long long)(tree.anc[node][k] >> -at);
                         }
                     }
-                    see >>= grp * KPT;
+                    see >>= col;
 #pragma unroll
                     for (int i = 0; i < KPT; i++)
                         if (!((i < 32 ? (uint32_t)see : (uint32_t)(see >> 32)) >> (i & 31) & 1u)) v[i] = -INFINITY;
@@ -650,14 +653,16 @@ __global__ void __launch_bounds__(kTcThreads, TcShape<HD, F32>::ctas) attn_tree_
                 const float alpha = m_new == m_run ? 1.0f : tc_ex2(m_run - m_new);
                 m_run = m_new;
                 const float off = m_new == -INFINITY ? 0.0f : -m_new;
-                float2 sum[2] = {};
+                F2 w2[KPT / 2], sum[2] = {0ull, 0ull};
+                const F2 scale2 = pack2(scale, scale), off2 = pack2(off, off), minus_one = pack2(-1.0f, -1.0f);
 #pragma unroll
-                for (int i = 0; i < KPT; i += 2) {
-                    const float2 y = fma2(make_float2(v[i], v[i + 1]), make_float2(scale, scale), make_float2(off, off));
-                    v[i] = tc_ex2(y.x); v[i + 1] = tc_ex2(y.y);
-                    sum[i >> 1 & 1] = add2(sum[i >> 1 & 1], make_float2(v[i], v[i + 1]));
+                for (int i = 0; i < KPT / 2; i++) {
+                    const float2 y = unpack2(fma2(pack2(v[2 * i], v[2 * i + 1]), scale2, off2));
+                    w2[i] = pack2(tc_ex2(y.x), tc_ex2(y.y));
+                    sum[i & 1] = add2(sum[i & 1], w2[i]);
                 }
-                l_run = l_run * alpha + ((sum[0].x + sum[0].y) + (sum[1].x + sum[1].y));
+                const float2 sums = unpack2(add2(sum[0], sum[1]));
+                l_run = l_run * alpha + (sums.x + sums.y);
                 // the weights' terms over the scores (the third one beside them), zeros where the keys are another row's
                 constexpr int kCols = KPT / 2 < 16 ? KPT / 2 : 16;
 #pragma unroll
@@ -666,7 +671,7 @@ __global__ void __launch_bounds__(kTcThreads, TcShape<HD, F32>::ctas) attn_tree_
                     for (int c = 0; c < KPT / 2; c += kCols) {
                         uint32_t pk[kCols];
 #pragma unroll
-                        for (int i = 0; i < kCols; i++) pk[i] = tc_term(&v[2 * (c + i)], &v[2 * (c + i) + 1]);
+                        for (int i = 0; i < kCols; i++) pk[i] = tc_term(&w2[c + i], minus_one);
                         const uint32_t to = e == 2 ? mine + S::col_x + (uint32_t)b * 32u : sc + e * 32u;
 #pragma unroll
                         for (int d = 0; d < DUP; d++) {
@@ -720,7 +725,7 @@ __global__ void __launch_bounds__(kTcThreads, TcShape<HD, F32>::ctas) attn_tree_
         if constexpr (DUP > 1) {
             if (live && grp > 0) {
                 s_ml[2 * (grp * (128 / DUP) + row)] = m_run; s_ml[2 * (grp * (128 / DUP) + row) + 1] = l_run;
-#pragma unroll
+#pragma unroll (F32 ? HD / 32 : 1)
                 for (int c = 0; c < HD / 32; c++) {
                     uint32_t y[32];
                     tc_ld<32>(mine + S::col_o + c * 32u, y);
@@ -755,7 +760,7 @@ __global__ void __launch_bounds__(kTcThreads, TcShape<HD, F32>::ctas) attn_tree_
             const float inv = !share && node >= 0 ? tree_inverse(a, h, m_run, l_run) : 1.0f;
             float odd = l_run * 0.0f;            // 0, or NaN where something is not finite
             const size_t at = share_at(part, max(x.share, 0), row);
-#pragma unroll
+#pragma unroll (F32 ? HD / 32 : 1)                   // (code that runs once is fetched as it runs: short code is fast code)
             for (int c = 0; c < HD / 32; c++) {
                 uint32_t y[32];
                 tc_ld<32>(mine + S::col_o + c * 32u, y);
@@ -895,6 +900,7 @@ int copies_of(const TreeAttnArgs& a) {
     return rows <= 32 ? 4 : rows <= 64 ? 2 : 1;
 }
 // What the call knows on the host: the CTAs that run at once, and bounds of the units and pieces the batch can have.
+constexpr int kWhole = 4;                            // tiles of a unit that is not worth cutting
 struct Bounds { long long units, tiles; };
 Bounds bounds_of(const TreeAttnArgs& a, int tile_rows) {
     const int G = a.n_q / a.n_kv;
@@ -910,9 +916,11 @@ Share share_of(const TreeAttnArgs& a, int sm_count) {
     p.rows = std::min(p.tile_rows, a.t.max_rows * G);
     p.slots = sm_count * (a.kv_bf16 && !a.q_bf16 && a.hd == 128 ? 1 : 2);
     const Bounds b = bounds_of(a, p.tile_rows);
+    // Few tiles: nothing is cut, and tree_combine (2 to 3 us, and as much of the caller's time) need not run.
+    if (b.tiles <= kWhole) { p.grid = (int)b.units; return p; }
     // pieces: at most slots of them where there are fewer units, else at most units + tiles / (2 tiles / slots), with two for every cut
     p.grid = (int)std::min(b.units * b.tiles, b.units < p.slots ? (long long)p.slots : b.units + p.slots / 2);
-    p.shares = b.tiles == 1 ? 0 : std::min(p.grid, p.slots);
+    p.shares = std::min(p.grid, p.slots);
     return p;
 }
 size_t plan_bytes(const TreeAttnArgs& a) { return ((size_t)a.t.n_seq + 1 + 3) / 4 * 16; }
