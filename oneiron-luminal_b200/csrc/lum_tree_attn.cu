@@ -353,10 +353,6 @@ template <> __device__ __forceinline__ void tc_st<8>(uint32_t at, const uint32_t
     asm volatile("tcgen05.st.sync.aligned.32x32b.x8.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8};" ::"r"(at), "r"(v[0]), "r"(v[1]), "r"(v[2]), "r"(v[3]), "r"(v[4]), "r"(v[5]), "r"(v[6]), "r"(v[7])
                  : "memory");
 }
-template <> __device__ __forceinline__ void tc_st<16>(uint32_t at, const uint32_t* v) {
-    asm volatile("tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16};" ::"r"(at), "r"(v[0]), "r"(v[1]), "r"(v[2]), "r"(v[3]), "r"(v[4]), "r"(v[5]), "r"(v[6]), "r"(v[7]), "r"(v[8]), "r"(v[9]), "r"(v[10]), "r"(v[11]), "r"(v[12]), "r"(v[13]), "r"(v[14]), "r"(v[15])
-                 : "memory");
-}
 template <> __device__ __forceinline__ void tc_st<32>(uint32_t at, const uint32_t* v) {
     asm volatile("tcgen05.st.sync.aligned.32x32b.x32.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31,%32};" ::"r"(at), "r"(v[0]), "r"(v[1]), "r"(v[2]), "r"(v[3]), "r"(v[4]), "r"(v[5]), "r"(v[6]), "r"(v[7]), "r"(v[8]), "r"(v[9]), "r"(v[10]), "r"(v[11]), "r"(v[12]), "r"(v[13]), "r"(v[14]), "r"(v[15]), "r"(v[16]), "r"(v[17]), "r"(v[18]), "r"(v[19]), "r"(v[20]), "r"(v[21]), "r"(v[22]), "r"(v[23]), "r"(v[24]), "r"(v[25]), "r"(v[26]), "r"(v[27]), "r"(v[28]), "r"(v[29]), "r"(v[30]), "r"(v[31])
                  : "memory");
@@ -653,34 +649,41 @@ __global__ void __launch_bounds__(kTcThreads, TcShape<HD, F32>::ctas) attn_tree_
                 const float alpha = m_new == m_run ? 1.0f : tc_ex2(m_run - m_new);
                 m_run = m_new;
                 const float off = m_new == -INFINITY ? 0.0f : -m_new;
-                F2 w2[KPT / 2], sum[2] = {0ull, 0ull};
+                // 16 keys at a time: their exponentials (one pipe) beside the terms of the 16 before (another), which go over the scores (the third one beside
+                // them), zeros where the keys are another row's
+                constexpr int kStep = 16, kCols = kStep / 2;
+                F2 w2[2][kCols], sum[2] = {0ull, 0ull};
                 const F2 scale2 = pack2(scale, scale), off2 = pack2(off, off), minus_one = pack2(-1.0f, -1.0f);
 #pragma unroll
-                for (int i = 0; i < KPT / 2; i++) {
-                    const float2 y = unpack2(fma2(pack2(v[2 * i], v[2 * i + 1]), scale2, off2));
-                    w2[i] = pack2(tc_ex2(y.x), tc_ex2(y.y));
-                    sum[i & 1] = add2(sum[i & 1], w2[i]);
+                for (int c = 0; c <= KPT / kStep; c++) {
+                    if (c < KPT / kStep) {
+#pragma unroll
+                        for (int i = 0; i < kCols; i++) {
+                            const float2 y = unpack2(fma2(pack2(v[c * kStep + 2 * i], v[c * kStep + 2 * i + 1]), scale2, off2));
+                            w2[c & 1][i] = pack2(tc_ex2(y.x), tc_ex2(y.y));
+                        }
+                    }
+                    if (c > 0) {
+#pragma unroll
+                        for (int i = 0; i < kCols; i++) sum[i & 1] = add2(sum[i & 1], w2[(c - 1) & 1][i]);
+#pragma unroll
+                        for (int e = 0; e < S::p_terms; e++) {
+                            uint32_t pk[kCols];
+#pragma unroll
+                            for (int i = 0; i < kCols; i++) pk[i] = tc_term(&w2[(c - 1) & 1][i], minus_one);
+                            const uint32_t to = (e == 2 ? mine + S::col_x + (uint32_t)b * 32u : sc + e * 32u) + (c - 1) * kCols;
+#pragma unroll
+                            for (int d = 0; d < DUP; d++) {
+                                uint32_t out[kCols];
+#pragma unroll
+                                for (int i = 0; i < kCols; i++) out[i] = d == grp ? pk[i] : 0u;
+                                tc_st<kCols>(to + d * (KPT / 2), out);
+                            }
+                        }
+                    }
                 }
                 const float2 sums = unpack2(add2(sum[0], sum[1]));
                 l_run = l_run * alpha + (sums.x + sums.y);
-                // the weights' terms over the scores (the third one beside them), zeros where the keys are another row's
-                constexpr int kCols = KPT / 2 < 16 ? KPT / 2 : 16;
-#pragma unroll
-                for (int e = 0; e < S::p_terms; e++)
-#pragma unroll
-                    for (int c = 0; c < KPT / 2; c += kCols) {
-                        uint32_t pk[kCols];
-#pragma unroll
-                        for (int i = 0; i < kCols; i++) pk[i] = tc_term(&w2[c + i], minus_one);
-                        const uint32_t to = e == 2 ? mine + S::col_x + (uint32_t)b * 32u : sc + e * 32u;
-#pragma unroll
-                        for (int d = 0; d < DUP; d++) {
-                            uint32_t out[kCols];
-#pragma unroll
-                            for (int i = 0; i < kCols; i++) out[i] = d == grp ? pk[i] : 0u;
-                            tc_st<kCols>(to + d * (KPT / 2) + c, out);
-                        }
-                    }
                 if (t > 0) {
                     if constexpr (F32) {         // O(t - 1) comes out before O(t) is made
                         wait(bar_o, t - 1);
