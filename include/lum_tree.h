@@ -14,7 +14,8 @@
  * Nothing is allocated, so the calls can be captured into graphs; all arrays named `device` are read by the kernels, not by the call.  What a
  * kernel finds wrong in them — a parent that is not an earlier node, a row or page outside the cache, more nodes or cached rows than the call
  * named — is left out (the sequence or span it belongs to keeps its outputs as they were, an unknown page's keys are not seen) and reported by
- * the next lum_op_status as LUM_E_DEVICE.  The pointers must belong to the current device (LUM_E_INVALID otherwise).
+ * the next lum_op_status as LUM_E_DEVICE.  The pointers must belong to the current device (LUM_E_INVALID otherwise).  Calls may run at the
+ * same time on several streams, each with a workspace of its own.
  */
 #ifndef LUM_TREE_H
 #define LUM_TREE_H
@@ -56,7 +57,8 @@ typedef struct lum_kv_map {
 /* Attention of the nodes: out = sum_j w_j v_j, w = softmax over the visible keys of scale * q . k_j.  A node sees the cached rows, its ancestors and
  * itself; with `window` > 0 only what is fewer than `window` places before its own.  q and out: [n_rows][n_q_heads][head_dim], rows q_stride /
  * out_stride elements apart; k and v: rows kv_stride elements apart, each [n_kv_heads][head_dim]; query head h reads K/V head
- * h / (n_q_heads / n_kv_heads).  sinks (device [n_q_heads], or NULL): a logit per head that joins the softmax's denominator. */
+ * h / (n_q_heads / n_kv_heads).  sinks (device [n_q_heads], or NULL): a logit per head that joins the softmax's denominator.  out must not
+ * overlap q. */
 typedef struct lum_tree_attn {
     uint32_t q_dtype;          /* LUM_BF16 or LUM_F32, of q and out */
     uint32_t kv_dtype;         /* LUM_BF16, or LUM_F32 with queries in f32 */
@@ -83,14 +85,15 @@ int32_t lum_op_tree_accept(const lum_draft_tree* tree, const int32_t* tokens_dev
                            const int32_t* picks_dev, int32_t* path_dev, int32_t path_len, int32_t* n_accepted_dev, int32_t* next_dev, void* workspace_dev,
                            size_t workspace_bytes, void* stream);
 
-/* One plane of cache rows (K or V of one layer): rows of row_bytes bytes (a multiple of 16), one behind the other, 16-byte aligned. */
+/* One plane of cache rows (K or V of one layer): rows of row_bytes bytes (a multiple of 16), one behind the other, 16-byte aligned.  A plane that
+ * is not is left out and reported by lum_op_status. */
 typedef struct lum_kv_plane {
     void* rows;
     uint64_t row_bytes;
 } lum_kv_plane;
 
 /* Every plane's row prefix + path[s][i] becomes row prefix + i, for i < n_accepted[s] (as lum_op_tree_accept leaves them: path is increasing).  The
- * rows moved must not share pages with another sequence.  planes_dev: device [n_planes]. */
+ * rows moved must not share pages with another sequence, nor two sequences a slot.  planes_dev: device [n_planes]. */
 int32_t lum_op_kv_compact(const lum_kv_plane* planes_dev, int32_t n_planes, const lum_kv_map* map, const lum_draft_tree* tree, const int32_t* path_dev,
                           int32_t path_len, const int32_t* n_accepted_dev, void* stream);
 /* spans_dev: device [n_spans][3] of {first source row, first destination row, rows}; every plane (of `rows` rows) has rows src .. src + n - 1 copied

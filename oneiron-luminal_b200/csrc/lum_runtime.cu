@@ -1104,6 +1104,7 @@ int kv_move(lum_rt* rt, size_t src, size_t dst, int n) {
         }
         return 0;
     }
+    CU(rt, cudaSetDevice(rt->cfg.device));
     if (int r = kv_planes(rt)) return r;
     const int span[3] = {(int)src, (int)dst, n};
     CU(rt, cudaMemcpyAsync(rt->d_span, span, sizeof span, cudaMemcpyHostToDevice, rt->stream));

@@ -166,6 +166,11 @@ __global__ void __launch_bounds__(kWalkThreads) tree_walk(const TreeAcceptArgs a
 }
 
 // ---------------------------------------------------------------------------------------------------- cache rows
+__device__ __forceinline__ bool plane_ok(const KvPlane& p, uint32_t* status) {
+    if (!((p.row_bytes | (uint64_t)(uintptr_t)p.rows) & 15)) return true;
+    if (threadIdx.x == 0) atomicOr(status, LUM_ST_BAD_PAGE);
+    return false;
+}
 // The rows that stand, one CTA per (plane, sequence).  A thread has a 16-byte column of the rows: it reads eight rows and then writes them.  Rows go up only and
 // in order (path[i] >= i, increasing), so nothing that is still to be read has been written, whatever the rows' places in memory.
 __global__ void __launch_bounds__(128) kv_compact(const KvPlane* planes, const TreeMap m, const TreeBatch t, const int* path, int path_len, const int* n_accepted, uint32_t* status) {
@@ -193,6 +198,7 @@ __global__ void __launch_bounds__(128) kv_compact(const KvPlane* planes, const T
         return;
     }
     const KvPlane p = planes[blockIdx.x];
+    if (!plane_ok(p, status)) return;
     const long long cols = (long long)(p.row_bytes >> 4);
     uint4* rows = (uint4*)p.rows;
     for (long long c = tid; c < cols; c += 128) {
@@ -216,6 +222,7 @@ __global__ void __launch_bounds__(kCopyThreads) kv_copy(const KvPlane* planes, l
         return;
     }
     const KvPlane p = planes[item / n_spans];
+    if (!plane_ok(p, status)) return;
     const long long cols = (long long)(p.row_bytes >> 4), total = n * cols, step = (long long)kCopyThreads * kCopyPieces;
     const uint4* from = (const uint4*)p.rows + src * cols;
     uint4* to = (uint4*)p.rows + dst * cols;
@@ -369,9 +376,10 @@ int32_t check_attn(const lum_tree_attn* d, const lum_draft_tree* tree, const lum
     if (a->q_stride < qw || a->out_stride < qw || a->kv_stride < kw) return refuse(op, "a row stride shorter than a row");
     const int qe = qb ? 2 : 4, ke = kb ? 2 : 4;
     if (a->q_stride * qe % 16 || a->out_stride * qe % 16 || a->kv_stride * ke % 16) return refuse(op, "row strides must be multiples of 16 bytes");
-    a->n_q = d->n_q_heads; a->n_kv = d->n_kv_heads; a->hd = d->head_dim; a->q_bf16 = qb; a->kv_bf16 = kb; a->window = d->window;
+    // a window that reaches over everything is none
+    a->n_q = d->n_q_heads; a->n_kv = d->n_kv_heads; a->hd = d->head_dim; a->q_bf16 = qb; a->kv_bf16 = kb; a->window = (long long)d->window < (long long)a->t.max_prefix + a->t.max_rows ? d->window : 0;
     a->scale = d->scale != 0.0f ? d->scale : 1.0f / __builtin_sqrtf((float)d->head_dim);
-    if (a->t.n_seq && a->t.n_rows && !tree_attn_supported(*a)) return refuse(op, "more than 128 query heads per K/V head, or a batch of 2^31 tiles of 64 keys (sequences x heads x cached rows)", LUM_E_UNSUPPORTED);
+    if (a->t.n_seq && a->t.n_rows && !tree_attn_supported(*a)) return refuse(op, "more than 128 query heads per K/V head, or a batch of 2^31 tiles of 64 keys (sequences x heads x cached rows) or 2^34 rows of heads", LUM_E_UNSUPPORTED);
     return 0;
 }
 
@@ -398,7 +406,7 @@ int32_t lum_op_attn_tree(const lum_tree_attn* desc, const lum_draft_tree* tree, 
     Device d;
     NEED(check_attn(desc, tree, map, &a));
     if (!a.t.n_seq || !a.t.n_rows) return 0;
-    if (!q || !k || !v || !out) return refuse(op, "null q, k, v or out");
+    if (!q || !k || !v || !out || out == q) return refuse(op, "null q, k, v or out, or out in the place of q");
     if (((uintptr_t)q | (uintptr_t)k | (uintptr_t)v | (uintptr_t)out | (uintptr_t)workspace) & 15) return refuse(op, "q, k, v, out and the workspace must be 16-byte aligned");
     NEED(device_of(op, &d));
     const size_t need = tree_attn_workspace(a, d.sms);
@@ -421,7 +429,7 @@ int32_t lum_op_attn_tree(const lum_tree_attn* desc, const lum_draft_tree* tree, 
 size_t lum_op_tree_accept_workspace(const lum_draft_tree* tree, int32_t vocab) {
     TreeBatch t{};
     Device d;
-    if (check_tree("tree_accept", tree, &t) || vocab < 1 || device_of("tree_accept", &d)) return (size_t)-1;
+    if (check_tree("tree_accept", tree, &t) || vocab < 1 || vocab > (1 << 30) || device_of("tree_accept", &d)) return (size_t)-1;
     return t.n_seq && t.n_rows ? tree_accept_workspace(t, vocab, d.sms) : 0;
 }
 
@@ -435,7 +443,8 @@ int32_t lum_op_tree_accept(const lum_draft_tree* tree, const int32_t* tokens, co
     if (!path || !n_accepted || !next) return refuse(op, "null output");
     if (path_len < a.t.max_rows) return refuse(op, "paths of " + std::to_string(path_len) + " nodes cannot hold a tree of " + std::to_string(a.t.max_rows));
     if (a.t.n_rows && (!tokens || (logits != nullptr) == (picks != nullptr))) return refuse(op, "tokens, and either logits or picks");
-    if (logits && (vocab < 1 || (logits_stride && logits_stride < vocab))) return refuse(op, "an empty vocabulary, or rows of logits that overlap");
+    if (logits && (vocab < 1 || vocab > (1 << 30) || (logits_stride && logits_stride < vocab) || ((uintptr_t)logits & 3)))
+        return refuse(op, "a vocabulary of 1 .. 2^30, rows of logits that do not overlap, 4-byte aligned");
     NEED(device_of(op, &d));
     if (!a.t.n_rows) {                               // every sequence is empty
         NEED(on_device(op, "path", path, d.id));

@@ -1008,7 +1008,8 @@ cudaError_t tc_launch(const TreeAttnArgs& a, const Share& p, cudaStream_t st) {
 bool tree_attn_supported(const TreeAttnArgs& a) {
     if (a.kv_bf16 && a.n_q / a.n_kv > 128) return false;
     const Bounds b = bounds_of(a, a.kv_bf16 ? 128 / copies_of(a) / (a.n_q / a.n_kv) * (a.n_q / a.n_kv) : kRowsTile);
-    return b.units < 0x40000000ll && b.units * b.tiles < 0x7fffffffll;       // tiles are counted in 32 bits
+    // tiles are counted in 32 bits, and tree_combine has a CTA for eight (row, head)
+    return b.units < 0x40000000ll && b.units * b.tiles < 0x7fffffffll && (long long)a.t.n_rows * a.n_q < 8 * 0x7fffffffll;
 }
 size_t tree_attn_workspace(const TreeAttnArgs& a, int sm_count) { return share_bytes(a, share_of(a, sm_count)); }
 

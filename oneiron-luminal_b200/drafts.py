@@ -136,7 +136,8 @@ def attn_tree(q, k, v, tree: DraftTree, cache: KvMap, *, n_kv_heads: int, head_d
     ``q`` [rows, heads * head_dim] (or [rows, heads, head_dim]) in bf16 or f32; ``k`` and ``v`` [cache rows, n_kv_heads * head_dim] in bf16, or in f32 with f32
     queries; rows may be strided.  ``scale`` 0: 1 / sqrt(head_dim).  ``window``: a node sees only what is fewer than so many places before its own.  ``sinks``
     [heads] f32: a logit per head that joins the softmax's denominator.  Returns ``out`` (like q; rows of no sequence are left as they were; without ``out``
-    given they are not set).  ``workspace``: scratch to use, a uint8 tensor of at least :func:`attn_tree_workspace` bytes (None: taken from torch)."""
+    given they are not set).  ``workspace``: scratch to use
+    (None: taken from torch); calls that may overlap need one each."""
     device, q_type, k_type = q.device, _types().get(q.dtype), _types().get(k.dtype)
     if device != tree.device or q_type is None or k_type is None or v.dtype != k.dtype:
         _bad(f"attn_tree: q {q.dtype} on {device}, tree on {tree.device}, k {k.dtype}, v {v.dtype}: bf16 or f32 on one device are wanted")
@@ -167,6 +168,8 @@ def attn_tree(q, k, v, tree: DraftTree, cache: KvMap, *, n_kv_heads: int, head_d
             _check(_INVALID)
         if need and workspace is None:
             workspace = torch.empty(need, dtype=torch.uint8, device=device)
+        if workspace is not None and not workspace.is_contiguous():
+            _bad("attn_tree: the workspace must be contiguous")
         w_at, w_bytes = (workspace.data_ptr(), workspace.numel() * workspace.element_size()) if workspace is not None else (None, 0)
         _check(lib.lum_op_attn_tree(desc, tree.desc, cache.desc, q_at, k_at, v_at, s_at, o_at, w_at, w_bytes, _stream(device.index)))
     return out

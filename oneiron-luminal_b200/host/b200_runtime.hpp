@@ -131,6 +131,27 @@ public:
         ck(lum_batch_get_decoded(h_, v.data(), n_steps));
         return v;
     }
+    // Speculative decoding: a tree of drafted tokens per sequence (node 0: the token that comes next at its position, parent -1) verified in one pass;
+    // returns the tokens that follow node 0 of every sequence, at least one
+    struct DraftTree { std::vector<int32_t> tokens, parents; };
+    std::vector<std::vector<int32_t>> draft_verify(const std::vector<DraftTree>& trees, const std::vector<int32_t>& positions, const std::vector<int32_t>& slots) {
+        if (positions.size() != trees.size() || slots.size() != trees.size()) throw Error(LUM_E_INVALID, "draft_verify: one entry per tree in each list");
+        std::vector<int32_t> start{0}, tokens, parents;
+        size_t most = 1;
+        for (const DraftTree& t : trees) {
+            if (t.tokens.size() != t.parents.size()) throw Error(LUM_E_INVALID, "draft_verify: a parent per token");
+            tokens.insert(tokens.end(), t.tokens.begin(), t.tokens.end());
+            parents.insert(parents.end(), t.parents.begin(), t.parents.end());
+            start.push_back((int32_t)tokens.size());
+            if (t.tokens.size() > most) most = t.tokens.size();
+        }
+        ck(lum_draft_verify(h_, (int32_t)trees.size(), slots.data(), positions.data(), start.data(), tokens.data(), parents.data()));
+        std::vector<int32_t> counts(trees.size()), got(trees.size() * most);
+        ck(lum_draft_get(h_, counts.data(), got.data(), most));
+        std::vector<std::vector<int32_t>> out;
+        for (size_t s = 0; s < trees.size(); s++) out.emplace_back(got.begin() + (std::ptrdiff_t)(s * most), got.begin() + (std::ptrdiff_t)(s * most) + counts[s]);
+        return out;
+    }
     std::pair<ProfileMetric, std::string> profile(int trials) {
         double us = 0; char buf[128] = {0};
         ck(lum_profile(h_, trials, &us, buf, sizeof buf));

@@ -81,7 +81,7 @@ def attn(pkg, ptr=(4096,) * 4, **kw):
     (dict(page_rows=64), -1), (dict(page_rows=64, page_table=4096), -1),
     (dict(head_dim=96), -3), (dict(n_q_heads=7), -1), (dict(n_kv_heads=0), -1), (dict(n_q_heads=2048), -1), (dict(q_dtype=1), -3), (dict(kv_dtype=7), -3), (dict(kv_dtype=0), -3),
     (dict(window=-1), -1), (dict(scale=-1.0), -1), (dict(scale=float("nan")), -1), (dict(scale=float("inf")), -1), (dict(q_stride=100), -1), (dict(kv_stride=64), -1), (dict(out_stride=513), -1),
-    (dict(q_stride=516), -1), (dict(n_q_heads=512, n_kv_heads=2), -3), (dict(n_seq=65535, max_prefix=2 ** 30), -3),
+    (dict(q_stride=516), -1), (dict(n_q_heads=512, n_kv_heads=2), -3), (dict(n_seq=65535, max_prefix=2 ** 30), -3), (dict(n_rows=2 ** 31 - 1, n_q_heads=64, n_kv_heads=64), -3),
     (dict(ptr=(None, 4096, 4096, 4096)), -1), (dict(ptr=(4096, 4096, 4096, None)), -1), (dict(ptr=(4104, 4096, 4096, 4096)), -1),
 ])
 def test_attention_refuses(pkg, kw, code):
@@ -102,7 +102,7 @@ def test_accept_compact_and_copy_refuse(pkg):
     lib, tree, cache = pkg.load_library(), pkg.runtime.DraftTreeDesc(**TREE), pkg.runtime.KvMapDesc(**MAP)
     p = 4096
     accept = lambda tokens=p, logits=p, vocab=50, ld=0, picks=None, path=p, length=8, n=p, nxt=p: lib.lum_op_tree_accept(tree, tokens, logits, vocab, ld, picks, path, length, n, nxt, None, 0, None)  # noqa: E731
-    for kw in (dict(tokens=None), dict(logits=None), dict(picks=p), dict(vocab=0), dict(ld=49), dict(path=None), dict(length=7), dict(n=None), dict(nxt=None)):
+    for kw in (dict(tokens=None), dict(logits=None), dict(picks=p), dict(vocab=0), dict(vocab=2 ** 30 + 1), dict(logits=p + 2), dict(ld=49), dict(path=None), dict(length=7), dict(n=None), dict(nxt=None)):
         assert accept(**kw) == -1, kw
     assert lib.lum_op_kv_compact(None, 2, cache, tree, p, 8, p, None) == -1
     assert lib.lum_op_kv_compact(p, 0, cache, tree, p, 8, p, None) == -1

@@ -400,6 +400,66 @@ def test_copy_of_spans_outside_the_cache_is_left_out(torch, ops, pkg):
     assert torch.equal(kv, want)
 
 
+def test_planes_whose_rows_are_no_multiple_of_16_bytes_are_left_out(torch, ops, pkg):
+    kv = torch.randn(2, 40, 16, device="cuda")
+    want = kv.clone()
+    want[0, 20:24] = kv[0, 3:7]
+    planes = ops.kv_planes([kv])
+    planes[1, 1] = 60
+    i32 = dict(dtype=torch.int32, device="cuda")
+    ops.kv_copy(planes, 40, torch.tensor([[3, 20, 4]], **i32), max_rows=4)
+    with pytest.raises(pkg.LumError):
+        ops.status()
+    assert torch.equal(kv, want)
+    with pytest.raises(pkg.LumError):
+        ops.kv_planes([kv[:, :, :3]])
+
+
+@pytest.mark.parametrize("q, cache", TYPES)
+def test_attention_with_a_window_that_reaches_over_everything(torch, ops, q, cache):
+    b = Batch(torch, ops, [200, 3], [70, 500], n_kv=1, group=1, q=q, cache=cache, kind="chain")
+    for window in (2 ** 31 - 1, 756, 700, 270):
+        b.check(b.run(window=window), window=window)
+    ops.status()
+
+
+def test_attention_with_a_workspace_of_the_caller(torch, ops, pkg):
+    b = Batch(torch, ops, [9, 30], [3000, 90], dim=128, group=4)
+    want = b.run().clone()
+    ws = torch.empty(64 << 20, dtype=torch.uint8, device="cuda")
+    assert torch.equal(b.run(workspace=ws), want)
+    with pytest.raises(pkg.LumError):
+        b.run(workspace=ws[:16])
+    with pytest.raises(pkg.LumError):
+        b.run(workspace=ws.view(-1, 64)[:, :32])
+    with pytest.raises(pkg.LumError):
+        b.run(out=b.q)
+
+
+def test_first_calls_of_a_process_inside_a_capture():
+    """Nothing is allocated or synchronised: even the first calls can be captured (the kernels are loaded then)."""
+    import os
+    import subprocess
+    import sys
+    root = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
+    code = """
+import sys; sys.path[:0] = [%r, %r]
+import torch, drafts_plain, test_gpu_drafts as t
+from __graft_entry__ import load_package
+ops = load_package().drafts
+b = t.Batch(torch, ops, [9, 30], [700, 90], dim=128, group=4, page=64)
+out = torch.zeros_like(b.q.contiguous())
+g = torch.cuda.CUDAGraph()
+with torch.cuda.graph(g):
+    b.run(out=out)
+g.replay()
+torch.cuda.synchronize()
+b.check(out)
+""" % (root, os.path.join(root, "tests"))
+    r = subprocess.run([sys.executable, "-c", code], capture_output=True, text=True, timeout=300)
+    assert r.returncode == 0, r.stderr[-2000:]
+
+
 def test_a_step_of_speculative_decoding(torch, ops):
     """Attention over drafts, acceptance, compaction: the kept rows are those of the path, and attending again from a chain over them gives what the tree gave."""
     b = Batch(torch, ops, [12, 7], [100, 33], page=16, q="f32", dim=64)
