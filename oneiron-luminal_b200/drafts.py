@@ -22,6 +22,7 @@ from .runtime import DraftTreeDesc, KvMapDesc, LumError, TreeAttnDesc, load_libr
 MAX_NODES = 256
 _F32, _BF16 = 0, 2
 _INVALID = -1
+_REFUSED = C.c_size_t(-1).value
 
 
 torch = None               # the package itself does not need it: imported by the first tensor
@@ -53,7 +54,7 @@ def _ints(name, t, device, dims=1, optional=False):
         return None
     if torch is None:
         _use_torch()
-    if not isinstance(t, torch.Tensor) or t.dtype != torch.int32 or t.dim() != dims or not t.is_contiguous() or t.device != device or not t.is_cuda:
+    if not isinstance(t, torch.Tensor) or t.dtype is not torch.int32 or t.dim() != dims or not t.is_contiguous() or t.device != device or t.get_device() < 0:
         _bad(f"{name}: a contiguous {dims}-d int32 tensor on {device} is wanted")
     return t.data_ptr()
 
@@ -76,7 +77,7 @@ class _Here:
         self.index = index
 
     def __enter__(self):
-        self.before = torch.cuda.current_device()
+        self.before = torch._C._cuda_getDevice()
         if self.before != self.index:
             torch.cuda.set_device(self.index)
 
@@ -93,8 +94,8 @@ class DraftTree:
         device = getattr(parent, "device", None)
         n_seq = prefix.numel()
         self.device, self.n_seq, self.n_rows, self.max_rows, self.tensors = device, n_seq, parent.numel(), max_rows, (row_start, prefix, parent, slot)
-        self.desc = DraftTreeDesc(_ints("row_start", row_start, device), _ints("prefix", prefix, device), _ints("parent", parent, device),
-                                  _ints("slot", slot, device, optional=True), n_seq, self.n_rows, max_rows, max_prefix)
+        self.ref = C.byref(DraftTreeDesc(_ints("row_start", row_start, device), _ints("prefix", prefix, device), _ints("parent", parent, device),
+                                         None if slot is None else _ints("slot", slot, device), n_seq, self.n_rows, max_rows, max_prefix))
         if row_start.numel() != n_seq + 1 or (slot is not None and slot.numel() != n_seq):
             _bad(f"row_start has {row_start.numel()} entries, slot {n_seq if slot is None else slot.numel()}, for {n_seq} sequences")
 
@@ -108,9 +109,9 @@ class KvMap:
         if (page_table is None) != (page_rows == 0):
             _bad("pages come with a page table")
         if page_table is None:
-            self.desc = KvMapDesc(None, rows, slots or max(1, rows // max(1, max_seq)), max_seq, 0, 0)
+            self.ref = C.byref(KvMapDesc(None, rows, slots or max(1, rows // max(1, max_seq)), max_seq, 0, 0))
         else:
-            self.desc = KvMapDesc(_ints("page_table", page_table, page_table.device, dims=2), rows, page_table.shape[0], max_seq, page_rows, page_table.shape[1])
+            self.ref = C.byref(KvMapDesc(_ints("page_table", page_table, page_table.device, dims=2), rows, page_table.shape[0], max_seq, page_rows, page_table.shape[1]))
 
 
 def _rows_of(name, t, device, width, rows):
@@ -160,18 +161,21 @@ def attn_tree(q, k, v, tree: DraftTree, cache: KvMap, *, n_kv_heads: int, head_d
         if sinks.device != device or sinks.dtype != torch.float32 or not sinks.is_contiguous() or sinks.numel() != width // head_dim:
             _bad(f"attn_tree: sinks must be {width // head_dim} contiguous f32 values on {device}")
         s_at = sinks.data_ptr()
-    desc = TreeAttnDesc(q_type, k_type, width // head_dim, n_kv_heads, head_dim, window, scale, 0, q_stride, k_stride, o_stride)
+    desc = C.byref(TreeAttnDesc(q_type, k_type, width // head_dim, n_kv_heads, head_dim, window, scale, 0, q_stride, k_stride, o_stride))
     lib = load_library()
     with _Here(device.index):
-        need = lib.lum_op_attn_tree_workspace(desc, tree.desc, cache.desc)
-        if need == C.c_size_t(-1).value:
+        need = lib.lum_op_attn_tree_workspace(desc, tree.ref, cache.ref)
+        if need == _REFUSED:
             _check(_INVALID)
-        if need and workspace is None:
-            workspace = torch.empty(need, dtype=torch.uint8, device=device)
-        if workspace is not None and not workspace.is_contiguous():
-            _bad("attn_tree: the workspace must be contiguous")
-        w_at, w_bytes = (workspace.data_ptr(), workspace.numel() * workspace.element_size()) if workspace is not None else (None, 0)
-        _check(lib.lum_op_attn_tree(desc, tree.desc, cache.desc, q_at, k_at, v_at, s_at, o_at, w_at, w_bytes, _stream(device.index)))
+        w_at, w_bytes = None, need
+        if workspace is not None:
+            if not workspace.is_contiguous():
+                _bad("attn_tree: the workspace must be contiguous")
+            w_at, w_bytes = workspace.data_ptr(), workspace.numel() * workspace.element_size()
+        elif need:
+            workspace = tree.tensors[0].new_empty(need // 4 + 1)        # (a tensor's own kind: half the time of torch.empty)
+            w_at = workspace.data_ptr()
+        _check(lib.lum_op_attn_tree(desc, tree.ref, cache.ref, q_at, k_at, v_at, s_at, o_at, w_at, w_bytes, _stream(device.index)))
     return out
 
 
@@ -191,19 +195,15 @@ def tree_accept(tree: DraftTree, tokens, *, logits=None, picks=None, path_len: i
         if logits.dtype != torch.float32 or logits.dim() != 2 or logits.device != device or logits.shape[0] != rows or logits.stride(1) != 1:
             _bad(f"tree_accept: logits must be [{rows}, vocab] f32 on {device}, dense in a row")
         l_at, vocab, ld = logits.data_ptr(), logits.shape[1], (logits.stride(0) if rows > 1 else 0)
-    path = torch.empty((n, path_len), dtype=torch.int32, device=device)
-    count, after = torch.empty((2, n), dtype=torch.int32, device=device).unbind(0)
     lib = load_library()
     with _Here(device.index):
-        w_at, need = None, 0
-        if logits is not None:
-            need = lib.lum_op_tree_accept_workspace(tree.desc, vocab)
-            if need == C.c_size_t(-1).value:
-                _check(_INVALID)
-            if need:
-                workspace = torch.empty(need, dtype=torch.uint8, device=device)
-                w_at = workspace.data_ptr()
-        _check(lib.lum_op_tree_accept(tree.desc, t_at, l_at, vocab, ld, p_at, path.data_ptr(), path_len, count.data_ptr(), after.data_ptr(), w_at, need, _stream(device.index)))
+        need = lib.lum_op_tree_accept_workspace(tree.ref, vocab) if logits is not None else 0
+        if need == _REFUSED:
+            _check(_INVALID)
+        path, count, after = tokens.new_empty((n, path_len)), tokens.new_empty(n), tokens.new_empty(n)
+        scratch = tokens.new_empty(need // 4) if need else None
+        _check(lib.lum_op_tree_accept(tree.ref, t_at, l_at, vocab, ld, p_at, path.data_ptr(), path_len, count.data_ptr(), after.data_ptr(), scratch.data_ptr() if need else None, need,
+                                      _stream(device.index)))
     return path, count, after
 
 
@@ -242,7 +242,7 @@ def kv_compact(planes, cache: KvMap, tree: DraftTree, path, n_accepted) -> None:
     if device != tree.device or path.shape[0] != tree.n_seq or n_accepted.numel() != tree.n_seq:
         _bad(f"kv_compact: paths of {path.shape[0]} and counts of {n_accepted.numel()} sequences for {tree.n_seq}")
     with _Here(device.index):
-        _check(load_library().lum_op_kv_compact(p_at, n, cache.desc, tree.desc, path_at, path.shape[1], n_at, _stream(device.index)))
+        _check(load_library().lum_op_kv_compact(p_at, n, cache.ref, tree.ref, path_at, path.shape[1], n_at, _stream(device.index)))
 
 
 def kv_copy(planes, rows: int, spans, *, max_rows: int) -> None:
