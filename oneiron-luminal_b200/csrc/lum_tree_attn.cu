@@ -72,37 +72,35 @@ struct Share {
 };
 __device__ __forceinline__ size_t share_at(const Share& p, int share, int r) { return (size_t)share * p.rows + r; }
 
-struct Piece {
+struct alignas(16) Piece {
     TreeSeq q;
     TreeWork w;
     int s, kvh, f0, tile, tiles, share;              // sequence, K/V head, first query row, tiles [tile, tile + tiles) of the unit's; share -1: the whole unit
 };
-struct SeqWork { int units, tiles; };                // units of a sequence (0: none, or its numbers are wrong), tiles of keys of each
-__device__ __forceinline__ SeqWork seq_work(const TreeAttnArgs& a, const Share& p, int s, TreeSeq* q, TreeWork* w) {
-    const bool ok = tree_seq(a.t, &a.m, s, q, a.status);
-    *w = tree_work(q->prefix, q->n, a.window);
-    return {ok ? a.n_kv * ((q->n * (a.n_q / a.n_kv) + p.tile_rows - 1) / p.tile_rows) : 0, w->n_tiles};
-}
+struct SeqWork { TreeSeq q; int units, tiles; };       // units of a sequence (0: none, or its numbers are wrong), tiles of keys of each
 __device__ __forceinline__ int pieces_of(int tiles, int per) { return (tiles + per - 1) / per; }
 __device__ __forceinline__ int warp_scan(int x, int lane) {                    // inclusive
 #pragma unroll
     for (int i = 1; i < 32; i <<= 1) { const int y = __shfl_up_sync(0xffffffffu, x, i); if (lane >= i) x += y; }
     return x;
 }
-// The CTA's piece, by one warp: {sequence or -1, unit, which of its pieces, first share of the unit or -1}; CTA 0 writes the plan down.
+// The CTA's piece, by one warp (x->s -1: none); CTA 0 writes the plan down.
 // A piece is at most `per` tiles long.  Where there are fewer units than CTAs that run at once, the pieces should be as many as those, nearly: the even share of all
-// tiles, longer by what rounding up makes of it.  (Pieces are at most units + tiles / per, so the third choice always fits.)  Where there are more units, only one longer
+// tiles, longer by what rounding up makes of it.  (Pieces are at most units + tiles / per, so the last choice always fits.)  Where there are more units, only one longer
 // than twice the even share is cut.  Short code: every CTA runs it once, cold.
-__device__ __forceinline__ int4 piece_find(const TreeAttnArgs& a, const Share& p, int lane, int* per_out) {
+__device__ __forceinline__ void piece_find(const TreeAttnArgs& a, const Share& p, int lane, Piece* x) {
     auto work = [&](int s) {
-        TreeSeq q;
-        TreeWork w;
-        return s < a.t.n_seq ? seq_work(a, p, s, &q, &w) : SeqWork{0, 1};
+        SeqWork y{{}, 0, 1};
+        if (s < a.t.n_seq && tree_seq(a.t, &a.m, s, &y.q, a.status)) {
+            y.units = a.n_kv * ((y.q.n * (a.n_q / a.n_kv) + p.tile_rows - 1) / p.tile_rows);
+            y.tiles = tree_work(y.q.prefix, y.q.n, a.window).n_tiles;
+        }
+        return y;
     };
     const SeqWork mine = work(lane);                 // (batches of up to 32 sequences: all there is)
     int units = mine.units, total = mine.units * mine.tiles;                   // (the call bounds them)
 #pragma unroll 1
-    for (int s0 = 32; s0 < a.t.n_seq; s0 += 32) { const SeqWork x = work(s0 + lane); units += x.units; total += x.units * x.tiles; }
+    for (int s0 = 32; s0 < a.t.n_seq; s0 += 32) { const SeqWork y = work(s0 + lane); units += y.units; total += y.units * y.tiles; }
     units = __reduce_add_sync(0xffffffffu, units);
     total = __reduce_add_sync(0xffffffffu, total);
     // Little work: a CTA on every SM, of two tiles at least, rather than two (which begin at the same time and get in each other's way)
@@ -112,44 +110,40 @@ __device__ __forceinline__ int4 piece_find(const TreeAttnArgs& a, const Share& p
     if (p.shares && units < slots) {
         per = max((int)even + 1, 2);
 #pragma unroll 1
-        for (int i = 0; i < 2; i++) {
+        for (int i = 0; i < 4; i++) {
             int n = mine.units * pieces_of(mine.tiles, per);
 #pragma unroll 1
-            for (int s0 = 32; s0 < a.t.n_seq; s0 += 32) { const SeqWork x = work(s0 + lane); n += x.units * pieces_of(x.tiles, per); }
+            for (int s0 = 32; s0 < a.t.n_seq; s0 += 32) { const SeqWork y = work(s0 + lane); n += y.units * pieces_of(y.tiles, per); }
             n = __reduce_add_sync(0xffffffffu, n);
             if (n <= slots) break;
-            per = i ? total / (slots - units) + 1 : (int)((float)per * (float)n / (float)slots) + 1;
+            per = i == 3 ? total / (slots - units) + 1 : (int)((float)per * (float)n / (float)slots) + 1;
         }
     }
-    *per_out = per;
     if (blockIdx.x == 0 && lane == 0) p.plan[0] = per;
+    if (lane == 0) x->s = -1;
+    __syncwarp();
     int before = 0, shares = 0;
-    int4 found = make_int4(-1, 0, 0, -1);
 #pragma unroll 1
     for (int s0 = 0; s0 < a.t.n_seq; s0 += 32) {
-        const SeqWork x = s0 ? work(s0 + lane) : mine;
-        const int k = pieces_of(x.tiles, per), sum = warp_scan(x.units * k, lane), cut = k > 1 ? x.units * k : 0, cuts = warp_scan(cut, lane);
+        const SeqWork y = s0 ? work(s0 + lane) : mine;
+        const int k = pieces_of(y.tiles, per), n = y.units * k, sum = warp_scan(n, lane), cut = k > 1 ? n : 0, cuts = warp_scan(cut, lane);
         if (blockIdx.x == 0 && s0 + lane < a.t.n_seq) p.plan[1 + s0 + lane] = shares + cuts - cut;
-        const unsigned int in = __ballot_sync(0xffffffffu, (int)blockIdx.x < before + sum);
-        if (in && found.x < 0) {
-            const int l = __ffs(in) - 1, kl = __shfl_sync(0xffffffffu, k, l), at = (int)blockIdx.x - before - __shfl_sync(0xffffffffu, sum - x.units * k, l), unit = at / kl;
-            found = make_int4(s0 + l, unit, at - unit * kl, kl > 1 ? shares + __shfl_sync(0xffffffffu, cuts - cut, l) + unit * kl : -1);
-            if (blockIdx.x) break;
+        const int at = (int)blockIdx.x - before - (sum - n);
+        if (at >= 0 && at < n) {                     // (of all lanes and rounds, one)
+            const int unit = at / k, i = at - unit * k, per_head = y.units / a.n_kv, least = y.tiles / k, more = y.tiles - least * k;
+            x->q = y.q;
+            x->w = tree_work(y.q.prefix, y.q.n, a.window);
+            x->s = s0 + lane;
+            x->kvh = unit / per_head;                // a K/V head's row tiles follow each other: their keys are in L2
+            x->f0 = (unit - x->kvh * per_head) * p.tile_rows;
+            x->tile = i * least + min(i, more);
+            x->tiles = least + (i < more ? 1 : 0);
+            x->share = k > 1 ? shares + cuts - cut + at : -1;
         }
         before += __shfl_sync(0xffffffffu, sum, 31);
         shares += __shfl_sync(0xffffffffu, cuts, 31);
+        if (blockIdx.x && (int)blockIdx.x < before) break;
     }
-    return found;
-}
-__device__ __forceinline__ void piece_load(const TreeAttnArgs& a, const Share& p, int4 found, int per, Piece& x) {
-    x.s = found.x;
-    const SeqWork y = seq_work(a, p, x.s, &x.q, &x.w);
-    const int per_head = y.units / a.n_kv, k = pieces_of(y.tiles, per), least = y.tiles / k, more = y.tiles - least * k;
-    x.kvh = found.y / per_head;                      // a K/V head's row tiles follow each other: their keys are in L2
-    x.f0 = (found.y - x.kvh * per_head) * p.tile_rows;
-    x.tile = found.z * least + min(found.z, more);
-    x.tiles = least + (found.z < more ? 1 : 0);
-    x.share = found.w < 0 ? -1 : found.w + found.z;
 }
 
 template <typename T> __device__ __forceinline__ T out_of(float x);
@@ -169,7 +163,7 @@ __device__ __forceinline__ float tree_inverse(const TreeAttnArgs& a, int h, floa
 // then four (two) dimensions of the values with their weights.
 constexpr int kRowsTile = 32, kRowsKeys = 32;
 template <int HD>
-constexpr int rows_smem() { return (kRowsTile * HD + kRowsKeys * (HD + 4) + kRowsKeys * HD + kRowsTile * kRowsKeys) * 4 + 32 + (int)sizeof(TreeNodes); }
+constexpr int rows_smem() { return (kRowsTile * HD + kRowsKeys * (HD + 4) + kRowsKeys * HD + kRowsTile * kRowsKeys) * 4 + (int)sizeof(Piece) + (int)sizeof(TreeNodes); }
 
 template <int HD>
 __global__ void __launch_bounds__(256) attn_tree_rows(const TreeAttnArgs a, const Share part) {
@@ -178,19 +172,14 @@ __global__ void __launch_bounds__(256) attn_tree_rows(const TreeAttnArgs a, cons
     float* s_k = s_q + kRowsTile * HD;               // [32][HD + 4]
     float* s_v = s_k + kRowsKeys * (HD + 4);         // [32][HD]
     float* s_p = s_v + kRowsKeys * HD;               // [32 rows][32 keys]
-    int* s_piece = (int*)(s_p + kRowsTile * kRowsKeys);
-    TreeNodes& tree = *(TreeNodes*)(s_piece + 8);
+    Piece* s_piece = (Piece*)(s_p + kRowsTile * kRowsKeys);
+    TreeNodes& tree = *(TreeNodes*)(s_piece + 1);
     constexpr int DPL = HD / 32;
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, G = a.n_q / a.n_kv;
-    if (warp == 0) {
-        int per;
-        const int4 found = piece_find(a, part, lane, &per);
-        if (lane == 0) { *(int4*)s_piece = found; s_piece[4] = per; }
-    }
+    if (warp == 0) piece_find(a, part, lane, s_piece);
     __syncthreads();
-    if (s_piece[0] < 0) return;
-    Piece x;
-    piece_load(a, part, *(int4*)s_piece, s_piece[4], x);
+    if (s_piece->s < 0) return;
+    const Piece x = *s_piece;
     const float scale = a.scale * kLog2e;
     {
         const TreeSeq& q = x.q;
@@ -322,7 +311,7 @@ struct TcShape {
     static constexpr int q_terms = F32 ? 3 : 1, p_terms = F32 ? 3 : 2;
     static constexpr int tile = kTileKeys * HD * 2;  // bytes of K (or V)
     static constexpr int q_bytes = F32 ? HD / 8 * kTcGroup : 128 * HD * 2;
-    static constexpr int off_k = 0, off_v = 2 * tile, off_q = 4 * tile, off_misc = off_q + q_terms * q_bytes, off_tree = off_misc + 144;
+    static constexpr int off_k = 0, off_v = 2 * tile, off_q = 4 * tile, off_misc = off_q + q_terms * q_bytes, off_tree = off_misc + 112 + (int)sizeof(Piece);
     static constexpr int smem = off_tree + (int)sizeof(TreeNodes);
     static constexpr int ctas = F32 && HD == 128 ? 1 : 2;                 // per SM
     static constexpr int cols = F32 && HD == 128 ? 512 : 256;             // tensor memory: scores 2 x 64, O, third terms 2 x 32
@@ -429,7 +418,7 @@ __global__ void __launch_bounds__(kTcThreads, TcShape<HD, F32>::ctas) attn_tree_
     const uint32_t base = smem_u32(tc_smem), misc = base + S::off_misc;
     const uint32_t bar_k = misc, bar_v = misc + 16, bar_s = misc + 32, bar_p = misc + 48, bar_o = misc + 64, bar_q = misc + 80;      // two of each (queries: one): tile t uses number t % 2
     volatile int* gave_up = (volatile int*)(tc_smem + S::off_misc + 104);
-    int* s_piece = (int*)(tc_smem + S::off_misc + 112);
+    Piece* s_piece = (Piece*)(tc_smem + S::off_misc + 112);
     TreeNodes& tree = *(TreeNodes*)(tc_smem + S::off_tree);
     pdl_launch_dependents();                         // (tree_combine waits for this kernel's end)
     if (tid == 32) {
@@ -444,22 +433,17 @@ __global__ void __launch_bounds__(kTcThreads, TcShape<HD, F32>::ctas) attn_tree_
         mbar_fence_init();
         *gave_up = 0;
     }
-    if (warp == 0) {
-        int per;
-        const int4 found = piece_find(a, part, lane, &per);
-        if (lane == 0) { *(int4*)s_piece = found; s_piece[4] = per; }
-    }
+    if (warp == 0) piece_find(a, part, lane, s_piece);
     if (warp == 5) tmem_alloc(misc + 96, S::cols);
     tc_fence_before_sync();
     __syncthreads();
     tc_fence_after_sync();
     const uint32_t tmem = *(volatile uint32_t*)(tc_smem + S::off_misc + 96);
-    if (s_piece[0] < 0) {
+    if (s_piece->s < 0) {
         if (warp == 5) tmem_dealloc(tmem, S::cols);
         return;
     }
-    Piece x;
-    piece_load(a, part, *(int4*)s_piece, s_piece[4], x);
+    const Piece x = *s_piece;
     const TreeSeq q = x.q;
     const TreeWork w = x.w;
     const int t_first = w.t_lo + x.tile, n_tiles = x.tiles, kvh = x.kvh, f0 = x.f0;
@@ -830,40 +814,48 @@ __global__ void __launch_bounds__(kTcThreads, TcShape<HD, F32>::ctas) attn_tree_
     if (tid == 0 && *gave_up) atomicOr(a.status, LUM_ST_WAIT_TMEM);
 }
 
-// ---- joins the shares of units that were cut: a warp per (row, head); o = sum_c 2^(m_c - M) o_c / (sum_c 2^(m_c - M) l_c + 2^(sink - M))
+// ---- joins the shares of units that were cut: a warp per (row, head); o = sum_c 2^(m_c - M) o_c / (sum_c 2^(m_c - M) l_c + 2^(sink - M)).  Most warps of a batch find
+// that their unit was not cut, so what counts is how soon they know.
 template <int HD, typename TQ>
-__global__ void __launch_bounds__(256) tree_combine(const TreeAttnArgs a, const Share part) {
+__global__ void __launch_bounds__(256, 6) tree_combine(const TreeAttnArgs a, const Share part) {
     constexpr int DPL = HD / 32;
-    const int lane = threadIdx.x & 31, G = a.n_q / a.n_kv;
-    const long long item = (long long)blockIdx.x * 8 + (threadIdx.x >> 5);
-    if (item >= (long long)a.t.n_rows * a.n_q) { pdl_grid_wait(); return; }
-    const int row = (int)(item / a.n_q), h = (int)(item % a.n_q);
-    // the row's sequence: the last one that starts at or before it
-    Piece x;
-    int hi = a.t.n_seq - 1;
-    x.s = 0;
-    while (x.s < hi) {
-        const int mid = (x.s + hi + 1) >> 1;
-        if (__ldg(a.t.row_start + mid) <= row) x.s = mid; else hi = mid - 1;
+    const int lane = threadIdx.x & 31, G = a.n_q / a.n_kv, blocks = (a.n_q + 7) >> 3, row = (int)(blockIdx.x / (unsigned)blocks), h = ((int)blockIdx.x - row * blocks) * 8 + (threadIdx.x >> 5);
+    // the row's sequence: the last one that starts at or before it, 32 at a time
+    int s = 0;
+    for (int len = a.t.n_seq; len > 1;) {
+        const int step = (len + 31) >> 5, at = lane * step;
+        const unsigned int m = __ballot_sync(0xffffffffu, at < len && __ldg(a.t.row_start + s + min(at, len - 1)) <= row);
+        const int k = m ? 31 - __clz(m) : 0;
+        s += k * step;
+        len = min(step, len - k * step);
     }
-    const bool mine = tree_seq(a.t, &a.m, x.s, &x.q, nullptr) && row >= x.q.r0 && row < x.q.r0 + x.q.n;
+    TreeSeq q;
+    const bool mine = h < a.n_q && tree_seq(a.t, &a.m, s, &q, nullptr) && row >= q.r0 && row < q.r0 + q.n;
     pdl_grid_wait();                                 // (what comes before does not depend on the kernel before; every warp waits, so that this kernel ends behind that one)
     if (!mine) return;
-    x.w = tree_work(x.q.prefix, x.q.n, a.window);
-    const int f = (row - x.q.r0) * G + h % G, R = part.tile_rows, unit = h / G * ((x.q.n * G + R - 1) / R) + f / R, r = f % R;
-    const int shares = pieces_of(x.w.n_tiles, __ldcg(part.plan)), first = __ldcg(part.plan + 1 + x.s) + unit * shares;
+    const int per = __ldcg(part.plan), first_of_seq = __ldcg(part.plan + 1 + s), shares = pieces_of(tree_work(q.prefix, q.n, a.window).n_tiles, per);
     if (shares == 1) return;                         // finished by its CTA
+    const int f = (row - q.r0) * G + h % G, R = part.tile_rows, first = first_of_seq + (h / G * ((q.n * G + R - 1) / R) + f / R) * shares, r = f % R;
     const float sink = a.sinks ? a.sinks[h] * kLog2e : -INFINITY;
     float top = sink, sum = a.sinks ? 1.0f : 0.0f, o[DPL];
 #pragma unroll
     for (int i = 0; i < DPL; i++) o[i] = 0.0f;
-    // 32 shares at a time: a lane has the factor of one, all have their dimensions of each, eight on their way
+    // 32 shares at a time: a lane has the factor of one, all have their dimensions of each, four on their way
     for (int c0 = 0; c0 < shares; c0 += 32) {
         float m = -INFINITY, l = 0.0f;
         if (c0 + lane < shares) {
             const float2 v = __ldcg((const float2*)part.ml + share_at(part, first + c0 + lane, r));
             m = v.x; l = v.y;
         }
+        const int n = min(32, shares - c0);
+        using V = typename std::conditional<DPL == 4, float4, float2>::type;
+        V y[4];
+        auto fetch = [&](int c) {
+#pragma unroll
+            for (int u = 0; u < 4; u++)
+                if (c + u < n) y[u] = __ldcg((const V*)(part.o + share_at(part, first + c0 + c + u, r) * HD) + lane);
+        };
+        fetch(0);
         float t = fmaxf(top, m);
 #pragma unroll
         for (int i = 16; i > 0; i >>= 1) t = fmaxf(t, __shfl_xor_sync(0xffffffffu, t, i));
@@ -874,21 +866,17 @@ __global__ void __launch_bounds__(256) tree_combine(const TreeAttnArgs a, const 
         top = t;
 #pragma unroll
         for (int i = 0; i < DPL; i++) o[i] *= before;
-        const int n = min(32, shares - c0);
-        for (int c = 0; c < n; c += 8) {
-            float y[8][DPL], g[8];
+        for (int c = 0; c < n; c += 4) {
+            if (c) fetch(c);
 #pragma unroll
-            for (int u = 0; u < 8; u++) {
-                g[u] = __shfl_sync(0xffffffffu, factor, min(c + u, 31));
-                const bool in = c + u < n && g[u] >= 0.0f;
-                const float* src = part.o + share_at(part, first + min(c0 + c + u, shares - 1), r) * HD + lane * DPL;
+            for (int u = 0; u < 4; u++) {
+                const float g = __shfl_sync(0xffffffffu, factor, min(c + u, 31));
+                if (c + u < n && g >= 0.0f) {
+                    const float* z = (const float*)&y[u];
 #pragma unroll
-                for (int i = 0; i < DPL; i++) y[u][i] = in ? __ldcg(src + i) : 0.0f;
+                    for (int i = 0; i < DPL; i++) o[i] = fmaf(z[i], g, o[i]);
+                }
             }
-#pragma unroll
-            for (int u = 0; u < 8; u++)
-#pragma unroll
-                for (int i = 0; i < DPL; i++) o[i] = fmaf(y[u][i], fmaxf(g[u], 0.0f), o[i]);
         }
     }
     const float inv = sum > 0.0f ? 1.0f / sum : sum;
@@ -932,9 +920,8 @@ size_t share_bytes(const TreeAttnArgs& a, const Share& p) { return plan_bytes(a)
 template <int HD, typename TQ>
 cudaError_t combine(const TreeAttnArgs& a, const Share& p, cudaStream_t st) {
     if (!p.shares) return cudaSuccess;               // nothing is cut
-    const long long items = (long long)a.t.n_rows * a.n_q;
     cudaLaunchConfig_t cfg = {};
-    cfg.gridDim = dim3((unsigned)((items + 7) / 8));
+    cfg.gridDim = dim3((unsigned)(a.t.n_rows * ((a.n_q + 7) / 8)));
     cfg.blockDim = dim3(256);
     cfg.stream = st;
     cudaLaunchAttribute at[1];
@@ -1009,7 +996,7 @@ bool tree_attn_supported(const TreeAttnArgs& a) {
     if (a.kv_bf16 && a.n_q / a.n_kv > 128) return false;
     const Bounds b = bounds_of(a, a.kv_bf16 ? 128 / copies_of(a) / (a.n_q / a.n_kv) * (a.n_q / a.n_kv) : kRowsTile);
     // tiles are counted in 32 bits, and tree_combine has a CTA for eight (row, head)
-    return b.units < 0x40000000ll && b.units * b.tiles < 0x7fffffffll && (long long)a.t.n_rows * a.n_q < 8 * 0x7fffffffll;
+    return b.units < 0x40000000ll && b.units * b.tiles < 0x7fffffffll && (long long)a.t.n_rows * ((a.n_q + 7) / 8) < 0x7fffffffll;
 }
 size_t tree_attn_workspace(const TreeAttnArgs& a, int sm_count) { return share_bytes(a, share_of(a, sm_count)); }
 
