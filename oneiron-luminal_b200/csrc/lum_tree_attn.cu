@@ -347,6 +347,8 @@ template <> __device__ __forceinline__ void tc_st<32>(uint32_t at, const uint32_
                  : "memory");
 }
 __device__ __forceinline__ void tc_st_wait() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
+// (passes over NaN as fmaxf does)
+__device__ __forceinline__ float max3(float a, float b, float c) { float r; asm("max.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c)); return r; }
 __device__ __forceinline__ float tc_ex2(float x) { float y; asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x)); return y; }
 // Pairs of floats in 64-bit registers: the softmax warps are bound by what they issue, and these issue once for two.
 using F2 = unsigned long long;
@@ -573,7 +575,7 @@ __global__ void __launch_bounds__(kTcThreads, TcShape<HD, F32>::ctas) attn_tree_
             tree_load(tree, a.t, q, a.window, tid, 128, 1, a.status);
             named_sync(1, 128);
         }
-        const int grp = warp / (4 / DUP), warp_row = warp % (4 / DUP) * 32, col = grp * KPT, row = warp_row + lane, f = f0 + row, node = row < live_rows ? node_of(f) : -1;
+        const int grp = DUP == 1 ? 0 : warp / (4 / DUP), warp_row = warp % (4 / DUP) * 32, col = grp * KPT, row = warp_row + lane, f = f0 + row, node = row < live_rows ? node_of(f) : -1;
         const bool live = warp_row < live_rows;      // a warp without live rows leaves its rows of P as they are: nobody reads what they make
         float m_run = -INFINITY, l_run = 0.0f;
         float o[F32 ? HD : 1];
@@ -621,12 +623,8 @@ __global__ void __launch_bounds__(kTcThreads, TcShape<HD, F32>::ctas) attn_tree_
                 }
                 float top[4] = {v[0], v[1], v[2], v[3]};
 #pragma unroll
-                for (int i = 4; i < KPT - 4; i += 8)
-#pragma unroll
-                    for (int e = 0; e < 4; e++) top[e] = fmaxf(top[e], fmaxf(v[i + e], v[i + 4 + e]));
-#pragma unroll
-                for (int e = 0; e < 4; e++) top[e] = fmaxf(top[e], v[KPT - 4 + e]);
-                const float tm = node >= 0 ? fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3])) * scale : -INFINITY;
+                for (int i = 4; i < KPT; i += 2) top[i >> 1 & 3] = max3(top[i >> 1 & 3], v[i], v[i + 1]);
+                const float tm = node >= 0 ? fmaxf(max3(top[0], top[1], top[2]), top[3]) * scale : -INFINITY;
                 // the reference of the exponents: kept while nothing is more than 2^8 times it
                 const bool grows = tm > m_run + (F32 ? 0.0f : 8.0f) || m_run == -INFINITY;
                 const float m_new = grows ? fmaxf(tm, m_run) : m_run;
@@ -660,7 +658,7 @@ __global__ void __launch_bounds__(kTcThreads, TcShape<HD, F32>::ctas) attn_tree_
                             for (int d = 0; d < DUP; d++) {
                                 uint32_t out[kCols];
 #pragma unroll
-                                for (int i = 0; i < kCols; i++) out[i] = d == grp ? pk[i] : 0u;
+                                for (int i = 0; i < kCols; i++) out[i] = DUP == 1 || d == grp ? pk[i] : 0u;
                                 tc_st<kCols>(to + d * (KPT / 2), out);
                             }
                         }
