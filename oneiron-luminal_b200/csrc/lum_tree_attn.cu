@@ -907,8 +907,9 @@ Share share_of(const TreeAttnArgs& a, int sm_count) {
     const Bounds b = bounds_of(a, p.tile_rows);
     // Few tiles: nothing is cut, and tree_combine (2 to 3 us, and as much of the caller's time) need not run.
     if (b.tiles <= kWhole) { p.grid = (int)b.units; return p; }
-    // pieces: at most slots of them where there are fewer units, else at most units + tiles / (2 tiles / slots), with two for every cut
-    p.grid = (int)std::min(b.units * b.tiles, b.units < p.slots ? (long long)p.slots : b.units + p.slots / 2);
+    // Pieces, as piece_find cuts them: at most `slots` where there are fewer units than the slots it takes (all, or half of them), else at most units + tiles / (2 tiles
+    // / slots).  Shares: the pieces of units that are cut; at most `slots` in both cases.
+    p.grid = (int)std::min(b.units * b.tiles, std::max((long long)p.slots, b.units + p.slots / 2));
     p.shares = std::min(p.grid, p.slots);
     return p;
 }

@@ -162,6 +162,17 @@ def test_attention_of_long_and_uneven_batches(torch, ops, q, cache):
 
 
 @pytest.mark.parametrize("q, cache", TYPES)
+@pytest.mark.parametrize("page", [16, 64])
+@pytest.mark.parametrize("short, n_kv", [(34, 8), (17, 8), (140, 2), (20, 8)])
+def test_attention_of_one_long_sequence_among_many_short_ones(torch, ops, q, cache, page, short, n_kv):
+    """About as many short units as CTAs that run at once, and a long unit that is cut as well: every piece has to be computed by some CTA."""
+    b = Batch(torch, ops, [1] * (short // 2) + [2] + [1] * (short - short // 2), [5] * (short // 2) + [6000] + [7] * (short - short // 2), n_kv=n_kv, group=1, dim=64, q=q,
+              cache=cache, page=page)
+    b.check(b.run())
+    ops.status()
+
+
+@pytest.mark.parametrize("q, cache", TYPES)
 @pytest.mark.parametrize("value", [float("inf"), float("-inf"), float("nan"), 3.0e38])
 def test_attention_leaves_out_what_is_masked_whatever_it_holds(torch, ops, q, cache, value):
     """A node that the others do not see, a row of the cache outside the window, and keys of the next sequence hold infinities: only who sees them is touched."""
