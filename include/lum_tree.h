@@ -13,8 +13,8 @@
  *
  * Nothing is allocated, so the calls can be captured into graphs; all arrays named `device` are read by the kernels, not by the call.  What a
  * kernel finds wrong in them — a parent that is not an earlier node, a row or page outside the cache, more nodes or cached rows than the call
- * named — is left out (the sequence or span it belongs to keeps its outputs as they were, an unknown page's keys are not seen) and reported by
- * the next lum_op_status as LUM_E_DEVICE.  The pointers must belong to the current device (LUM_E_INVALID otherwise).  Calls may run at the
+ * named — is left out and reported by the next lum_op_status as LUM_E_DEVICE: the sequence or span it belongs to keeps its outputs as they were
+ * (every sequence of a batch whose row_start decreases may), a parent counts as none, the rows of an unknown page as zeros.  The pointers must belong to the current device (LUM_E_INVALID otherwise).  Calls may run at the
  * same time on several streams, each with a workspace of its own.
  */
 #ifndef LUM_TREE_H

@@ -394,16 +394,18 @@ __device__ __noinline__ void tree_row_plain(const TreeAttnArgs& a, const TreeNod
     for (int j = j0; j < j1; j++) {
         if (!tree_sees(tree, q, a.window, node, j)) continue;
         const long long at = tree_row(a.m, q.slot, j, nullptr);
-        if (at < 0) continue;
-        const size_t off = (size_t)at * a.kv_stride + (size_t)kvh * HD + lane * DPL;
-        float d = 0.0f;
+        const size_t off = (size_t)max(at, 0ll) * a.kv_stride + (size_t)kvh * HD + lane * DPL;
+        float d = 0.0f, v[DPL];
 #pragma unroll
-        for (int i = 0; i < DPL; i++) d = fmaf(x[i], __bfloat162float(((const __nv_bfloat16*)a.k)[off + i]), d);
+        for (int i = 0; i < DPL; i++) {                              // (the rows of an unknown page are zeros)
+            d = fmaf(x[i], at >= 0 ? __bfloat162float(((const __nv_bfloat16*)a.k)[off + i]) : 0.0f, d);
+            v[i] = at >= 0 ? __bfloat162float(((const __nv_bfloat16*)a.v)[off + i]) : 0.0f;
+        }
         d = warp_sum(d) * scale;
         const float mn = fmaxf(mx, d), c = mx == mn ? 1.0f : exp2f(mx - mn), p = exp2f(d - (mn == -INFINITY ? 0.0f : mn));
         sum = sum * c + p;
 #pragma unroll
-        for (int i = 0; i < DPL; i++) o[i] = fmaf(p, __bfloat162float(((const __nv_bfloat16*)a.v)[off + i]), o[i] * c);
+        for (int i = 0; i < DPL; i++) o[i] = fmaf(p, v[i], o[i] * c);
         mx = mn;
     }
     *m = mx; *l = sum;

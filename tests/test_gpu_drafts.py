@@ -268,6 +268,24 @@ def test_attention_bad_numbers_on_the_device_are_left_out_and_reported(torch, op
     refused()
 
 
+@pytest.mark.parametrize("q, cache", TYPES)
+@pytest.mark.parametrize("masked", [0.0, float("inf")])
+def test_attention_takes_the_rows_of_an_unknown_page_as_zeros(torch, ops, pkg, q, cache, masked):
+    """Also where a row is computed key by key, because a value that it does not see is infinite."""
+    b = Batch(torch, ops, [6], [100], page=16, q=q, cache=cache, kind="star")
+    node = int(b.where[0][100 + 5])                          # the others do not see it
+    b.v[node] = masked
+    b.map.tensors[0][0, 2] = 10 ** 6
+    got = b.run()[:5].clone()
+    with pytest.raises(pkg.LumError):
+        ops.status()
+    gone = b.where[0][32:48]
+    b.k[gone], b.v[gone], b.v[node] = 0.0, 0.0, 0.0
+    want, off = b.want()
+    bound = off[:5] + (2.0 ** -8 * (np.abs(want[:5]) + off[:5]) + 2.0 ** -14 if q == "bf16" else 0.0)
+    assert (np.abs(got.double().cpu().numpy() - want[:5]) <= bound).all()
+
+
 # ---------------------------------------------------------------------------------------------------- accepted nodes
 
 
