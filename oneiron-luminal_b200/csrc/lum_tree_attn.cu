@@ -65,7 +65,7 @@ __device__ __forceinline__ bool tree_sees(const TreeNodes& s, const TreeSeq& q, 
 // long a piece may be is chosen on the device, where the lengths are.  A whole unit is finished by its CTA; a unit in pieces leaves a share (maximum, sum,
 // outputs) of each in the workspace, and tree_combine joins them.
 struct Share {
-    int* plan;                                       // [0] tiles of a piece at most, [1 + s] the first share of sequence s; written by CTA 0
+    int* plan;                                       // [0] tiles of a piece at most, [1 + s] the first share of sequence s; written by CTA 0 for tree_combine
     float *ml, *o;                                   // [share][rows][2], [share][rows][hd]
     int grid, shares, slots;                         // CTAs launched, shares there is room for, CTAs that run at once
     int copies, rows, tile_rows;                     // copies of a query row in a tile, query rows of a share, of a unit
@@ -119,7 +119,8 @@ __device__ __forceinline__ void piece_find(const TreeAttnArgs& a, const Share& p
             per = i == 3 ? total / (slots - units) + 1 : (int)((float)per * (float)n / (float)slots) + 1;
         }
     }
-    if (blockIdx.x == 0 && lane == 0) p.plan[0] = per;
+    const bool plans = blockIdx.x == 0 && p.shares;  // (without shares nobody reads it)
+    if (plans && lane == 0) p.plan[0] = per;
     if (lane == 0) x->s = -1;
     __syncwarp();
     int before = 0, shares = 0;
@@ -127,7 +128,7 @@ __device__ __forceinline__ void piece_find(const TreeAttnArgs& a, const Share& p
     for (int s0 = 0; s0 < a.t.n_seq; s0 += 32) {
         const SeqWork y = s0 ? work(s0 + lane) : mine;
         const int k = pieces_of(y.tiles, per), n = y.units * k, sum = warp_scan(n, lane), cut = k > 1 ? n : 0, cuts = warp_scan(cut, lane);
-        if (blockIdx.x == 0 && s0 + lane < a.t.n_seq) p.plan[1 + s0 + lane] = shares + cuts - cut;
+        if (plans && s0 + lane < a.t.n_seq) p.plan[1 + s0 + lane] = shares + cuts - cut;
         const int at = (int)blockIdx.x - before - (sum - n);
         if (at >= 0 && at < n) {                     // (of all lanes and rounds, one)
             const int unit = at / k, i = at - unit * k, per_head = y.units / a.n_kv, least = y.tiles / k, more = y.tiles - least * k;
@@ -891,7 +892,6 @@ int copies_of(const TreeAttnArgs& a) {
     return rows <= 32 ? 4 : rows <= 64 ? 2 : 1;
 }
 // What the call knows on the host: the CTAs that run at once, and bounds of the units and pieces the batch can have.
-constexpr int kWhole = 4;                            // tiles of a unit that is not worth cutting
 struct Bounds { long long units, tiles; };
 Bounds bounds_of(const TreeAttnArgs& a, int tile_rows) {
     const int G = a.n_q / a.n_kv;
@@ -907,8 +907,10 @@ Share share_of(const TreeAttnArgs& a, int sm_count) {
     p.rows = std::min(p.tile_rows, a.t.max_rows * G);
     p.slots = sm_count * (a.kv_bf16 && !a.q_bf16 && a.hd == 128 ? 1 : 2);
     const Bounds b = bounds_of(a, p.tile_rows);
-    // Few tiles: nothing is cut, and tree_combine (2 to 3 us, and as much of the caller's time) need not run.
-    if (b.tiles <= kWhole) { p.grid = (int)b.units; return p; }
+    // Few tiles: nothing is cut, and tree_combine (2 to 3 us, and as much of the caller's time) need not run.  Measured, us in a graph / per call from a program:
+    // one tree of 8 nodes over 508 rows in bf16 (8 tiles, 8 units) whole 12.7 / 18.2, cut 11.6 / 20.4; 5 trees of 13 over windows of 128 in f32 (3 tiles) whole 16.5, cut
+    // 18.0.  A tile takes CUDA cores four times as long: an f32 cache is cut sooner.
+    if (b.tiles <= (a.kv_bf16 ? 8 : 4)) { p.grid = (int)b.units; return p; }
     // Pieces, as piece_find cuts them: at most `slots` where there are fewer units than the slots it takes (all, or half of them), else at most units + tiles / (2 tiles
     // / slots).  Shares: the pieces of units that are cut; at most `slots` in both cases.
     p.grid = (int)std::min(b.units * b.tiles, std::max((long long)p.slots, b.units + p.slots / 2));
@@ -916,7 +918,7 @@ Share share_of(const TreeAttnArgs& a, int sm_count) {
     return p;
 }
 size_t plan_bytes(const TreeAttnArgs& a) { return ((size_t)a.t.n_seq + 1 + 3) / 4 * 16; }
-size_t share_bytes(const TreeAttnArgs& a, const Share& p) { return plan_bytes(a) + (size_t)p.shares * p.rows * (a.hd + 2) * 4; }
+size_t share_bytes(const TreeAttnArgs& a, const Share& p) { return !p.shares ? 0 : plan_bytes(a) + (size_t)p.shares * p.rows * (a.hd + 2) * 4; }
 
 template <int HD, typename TQ>
 cudaError_t combine(const TreeAttnArgs& a, const Share& p, cudaStream_t st) {

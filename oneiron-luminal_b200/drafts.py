@@ -187,7 +187,7 @@ def tree_accept(tree: DraftTree, tokens, *, logits=None, picks=None, path_len: i
     ``next_token`` is the pick at the last of them."""
     device, n, rows = tree.device, tree.n_seq, tree.n_rows
     path_len = path_len or tree.max_rows
-    t_at, p_at = _ints("tokens", tokens, device), _ints("picks", picks, device, optional=True)
+    t_at, k_at = _ints("tokens", tokens, device), _ints("picks", picks, device, optional=True)
     if tokens.numel() != rows or (picks is not None and picks.numel() != rows):
         _bad(f"tree_accept: {tokens.numel()} tokens for {rows} rows")
     l_at, vocab, ld = None, 0, 0
@@ -200,9 +200,12 @@ def tree_accept(tree: DraftTree, tokens, *, logits=None, picks=None, path_len: i
         need = lib.lum_op_tree_accept_workspace(tree.ref, vocab) if logits is not None else 0
         if need == _REFUSED:
             _check(_INVALID)
-        path, count, after = tokens.new_empty((n, path_len)), tokens.new_empty(n), tokens.new_empty(n)
-        scratch = tokens.new_empty(need // 4) if need else None
-        _check(lib.lum_op_tree_accept(tree.ref, t_at, l_at, vocab, ld, p_at, path.data_ptr(), path_len, count.data_ptr(), after.data_ptr(), scratch.data_ptr() if need else None, need,
+        # one allocation (a tensor of torch's costs a third of a launch): the scratch first, for its alignment, then the results
+        room, at = tokens.new_empty(need // 4 + n * (path_len + 2)), need // 4
+        path, count, after = room.as_strided((n, path_len), (path_len, 1), at), room.as_strided((n,), (1,), at + n * path_len), room.as_strided((n,), (1,), at + n * (path_len + 1))
+        base = room.data_ptr()
+        p_at = base + need
+        _check(lib.lum_op_tree_accept(tree.ref, t_at, l_at, vocab, ld, k_at, p_at, path_len, p_at + 4 * n * path_len, p_at + 4 * n * (path_len + 1), base if need else None, need,
                                       _stream(device.index)))
     return path, count, after
 
