@@ -14,6 +14,7 @@ namespace lum {
 namespace {
 
 constexpr float kLog2e = 1.4426950408889634f;
+constexpr int kClusterMax = 8;                       // CTAs of a (portable) cluster
 constexpr int kTileKeys = 64;                        // tiles of so many cache rows, from the first visible one's tile on
 
 struct TreeWork {                                    // the keys of a sequence that any node sees: rows low .. n_keys - 1, tiles t_lo .. t_lo + n_tiles - 1
@@ -69,13 +70,14 @@ struct Share {
     float *ml, *o;                                   // [share][rows][2], [share][rows][hd]
     int grid, shares, slots;                         // CTAs launched, shares there is room for, CTAs that run at once
     int copies, rows, tile_rows;                     // copies of a query row in a tile, query rows of a share, of a unit
+    int cluster, row_tiles;                          // > 1: a cluster of so many CTAs per unit; units of a K/V head there may be
 };
 __device__ __forceinline__ size_t share_at(const Share& p, int share, int r) { return (size_t)share * p.rows + r; }
 
 struct alignas(16) Piece {
     TreeSeq q;
     TreeWork w;
-    int s, kvh, f0, tile, tiles, share;              // sequence, K/V head, first query row, tiles [tile, tile + tiles) of the unit's; share -1: the whole unit
+    int s, kvh, f0, tile, tiles, share;              // sequence, K/V head, first query row, tiles [tile, tile + tiles) of the unit's; share -1: none
 };
 struct SeqWork { TreeSeq q; int units, tiles; };       // units of a sequence (0: none, or its numbers are wrong), tiles of keys of each
 __device__ __forceinline__ int pieces_of(int tiles, int per) { return (tiles + per - 1) / per; }
@@ -145,6 +147,20 @@ __device__ __forceinline__ void piece_find(const TreeAttnArgs& a, const Share& p
         shares += __shfl_sync(0xffffffffu, cuts, 31);
         if (blockIdx.x && (int)blockIdx.x < before) break;
     }
+}
+
+// The piece of a CTA of a cluster: its part of the unit's tiles (perhaps none).  By one thread.
+__device__ __forceinline__ void piece_of_cluster(const TreeAttnArgs& a, const Share& p, Piece* x) {
+    const int unit = (int)blockIdx.x / p.cluster, i = (int)blockIdx.x - unit * p.cluster, u = unit / p.row_tiles, s = u / a.n_kv, f0 = (unit - u * p.row_tiles) * p.tile_rows;
+    const bool live = tree_seq(a.t, &a.m, s, &x->q, a.status) && f0 < x->q.n * (a.n_q / a.n_kv);
+    x->w = tree_work(x->q.prefix, live ? x->q.n : 0, a.window);
+    x->s = live ? s : -1;
+    x->kvh = u - s * a.n_kv;
+    x->f0 = f0;
+    const int least = x->w.n_tiles / p.cluster, more = x->w.n_tiles - least * p.cluster;
+    x->tile = i * least + min(i, more);
+    x->tiles = least + (i < more ? 1 : 0);
+    x->share = -1;
 }
 
 template <typename T> __device__ __forceinline__ T out_of(float x);
@@ -373,6 +389,12 @@ __device__ __forceinline__ uint32_t tc_term(float* x0, float* x1) {
     *x0 = r.x; *x1 = r.y;
     return b;
 }
+__device__ __forceinline__ float2 cluster_ld2(uint32_t at) { float2 v; asm volatile("ld.shared::cluster.v2.f32 {%0, %1}, [%2];" : "=f"(v.x), "=f"(v.y) : "r"(at) : "memory"); return v; }
+__device__ __forceinline__ float4 cluster_ld4(uint32_t at) {
+    float4 v;
+    asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];" : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w) : "r"(at) : "memory");
+    return v;
+}
 __device__ __forceinline__ void tma_box(uint32_t dst, const CUtensorMap* map, int row, int col, uint32_t bar) {
     asm volatile("cp.async.bulk.tensor.3d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4}], [%5];" ::"r"(dst), "l"(map), "r"(0), "r"(row), "r"(col), "r"(bar) : "memory");
 }
@@ -438,7 +460,8 @@ __global__ void __launch_bounds__(kTcThreads, TcShape<HD, F32>::ctas) attn_tree_
         mbar_fence_init();
         *gave_up = 0;
     }
-    if (warp == 0) piece_find(a, part, lane, s_piece);
+    if (part.cluster > 1) { if (tid == 0) piece_of_cluster(a, part, s_piece); }
+    else if (warp == 0) piece_find(a, part, lane, s_piece);
     if (warp == 5) tmem_alloc(misc + 96, S::cols);
     tc_fence_before_sync();
     __syncthreads();
@@ -451,7 +474,13 @@ __global__ void __launch_bounds__(kTcThreads, TcShape<HD, F32>::ctas) attn_tree_
     const Piece x = *s_piece;
     const TreeSeq q = x.q;
     const TreeWork w = x.w;
-    const int t_first = w.t_lo + x.tile, n_tiles = x.tiles, kvh = x.kvh, f0 = x.f0;
+    const int t_first = w.t_lo + x.tile, n_tiles = x.tiles, kvh = x.kvh, f0 = x.f0, live_rows = min(part.tile_rows, q.n * G - f0);
+    const bool clustered = part.cluster > 1;
+    // Room of the tiles and queries behind the last product: copies' outputs and (maximum, sum), then a cluster's
+    constexpr int kLd = HD + 4, kCopyRows = 128 / DUP;
+    constexpr int off_copy_ml = (DUP - 1) * kCopyRows * kLd * 4, off_share = DUP > 1 ? off_copy_ml + 1024 : 0, off_share_ml = off_share + kCopyRows * kLd * 4;
+    static_assert(off_share_ml + kCopyRows * 8 <= S::off_misc, "fits");
+    float *c_o = (float*)(tc_smem + off_share), *c_ml = (float*)(tc_smem + off_share_ml);      // [row][kLd], [row][2]
 
     // A wait that runs out of its budget is remembered; what follows hardly waits and multiplies no more, but meets every barrier.
     auto wait = [&](uint32_t bar, int t) {
@@ -544,7 +573,6 @@ __global__ void __launch_bounds__(kTcThreads, TcShape<HD, F32>::ctas) attn_tree_
         const uint32_t mine = tmem + ((uint32_t)(warp * 32) << 16);
         const uint32_t magic = 0xffffffffu / (uint32_t)G + 1u;           // f / G = f magic / 2^32 for f < 2^18, 2 <= G <= 2^10
         auto node_of = [&](int f) { return G == 1 ? f : (int)__umulhi((uint32_t)f, magic); };
-        const int live_rows = min(part.tile_rows, q.n * G - f0);
         if constexpr (F32) {                         // three terms of the queries (rows beyond the last one are left as they are: nobody reads what they make)
             constexpr int kPieces = HD / 8, kStep = 128 / kPieces, kAhead = 4;
             const int c = tid % kPieces;
@@ -702,13 +730,19 @@ __global__ void __launch_bounds__(kTcThreads, TcShape<HD, F32>::ctas) attn_tree_
             if (lane == 0) mbar_arrive(bar_p + 8u * b);
         }
         if (n_tiles > 1) wait(bar_o, n_tiles - 2);
-        wait(bar_o, n_tiles - 1);
+        if (n_tiles > 0) wait(bar_o, n_tiles - 1);
+        else wait(bar_q, 0);                         // (a cluster's CTA without a tile: the queries are there, nothing else comes)
         tc_fence_after_sync();
+        auto outputs = [&](int c, uint32_t* y) {     // columns 32 c .. 32 c + 31 of this thread's row
+            if (n_tiles > 0) {
+                tc_ld<32>(mine + S::col_o + c * 32u, y);
+                tmem_ld_wait();
+            } else
+#pragma unroll
+                for (int i = 0; i < 32; i++) y[i] = 0u;
+        };
         // ---- the row's other copies: (maximum, sum, outputs) of their keys, through the room of the tiles (all of them have been used)
-        constexpr int kLd = HD + 4;
-        float* s_o = (float*)tc_smem;                // [copy - 1][row][kLd]
-        float* s_ml = (float*)(tc_smem + 2 * S::tile + 2 * S::tile) - 2 * 128;
-        static_assert(DUP == 1 || (DUP - 1) * (128 / DUP) * kLd * 4 + 1024 <= 4 * S::tile, "fits");
+        float *s_o = (float*)tc_smem, *s_ml = (float*)(tc_smem + off_copy_ml);         // [copy - 1][row][kLd], [copy][row][2]
         float f_own = 1.0f, f_other[DUP > 1 ? DUP - 1 : 1];
         if constexpr (DUP > 1) {
             if (live && grp > 0) {
@@ -716,8 +750,7 @@ __global__ void __launch_bounds__(kTcThreads, TcShape<HD, F32>::ctas) attn_tree_
 #pragma unroll (F32 ? HD / 32 : 1)
                 for (int c = 0; c < HD / 32; c++) {
                     uint32_t y[32];
-                    tc_ld<32>(mine + S::col_o + c * 32u, y);
-                    tmem_ld_wait();
+                    outputs(c, y);
 #pragma unroll
                     for (int i = 0; i < 32; i += 4) {
                         float4 z = make_float4(__uint_as_float(y[i]), __uint_as_float(y[i + 1]), __uint_as_float(y[i + 2]), __uint_as_float(y[i + 3]));
@@ -745,14 +778,13 @@ __global__ void __launch_bounds__(kTcThreads, TcShape<HD, F32>::ctas) attn_tree_
         const bool share = x.share >= 0;
         if (live && grp == 0) {
             const int h = kvh * G + (node >= 0 ? f - node * G : 0), out_row = q.r0 + max(node, 0);
-            const float inv = !share && node >= 0 ? tree_inverse(a, h, m_run, l_run) : 1.0f;
+            const float inv = !share && !clustered && node >= 0 ? tree_inverse(a, h, m_run, l_run) : 1.0f;
             float odd = l_run * 0.0f;            // 0, or NaN where something is not finite
             const size_t at = share_at(part, max(x.share, 0), row);
 #pragma unroll (F32 ? HD / 32 : 1)                   // (code that runs once is fetched as it runs: short code is fast code)
             for (int c = 0; c < HD / 32; c++) {
                 uint32_t y[32];
-                tc_ld<32>(mine + S::col_o + c * 32u, y);
-                tmem_ld_wait();
+                outputs(c, y);
 #pragma unroll
                 for (int i = 0; i < 32; i++) {
                     float z = __uint_as_float(y[i]);
@@ -766,9 +798,10 @@ __global__ void __launch_bounds__(kTcThreads, TcShape<HD, F32>::ctas) attn_tree_
                     y[i] = __float_as_uint(z * inv);
                 }
                 if (node >= 0) {
-                    if (share) {
+                    if (share || clustered) {
+                        float* to = clustered ? c_o + row * kLd : part.o + at * HD;
 #pragma unroll
-                        for (int i = 0; i < 32; i += 4) *(uint4*)(part.o + at * HD + c * 32 + i) = make_uint4(y[i], y[i + 1], y[i + 2], y[i + 3]);
+                        for (int i = 0; i < 32; i += 4) *(uint4*)(to + c * 32 + i) = make_uint4(y[i], y[i + 1], y[i + 2], y[i + 3]);
                     } else {
                         TQ* dst = (TQ*)a.out + (size_t)out_row * a.out_stride + (size_t)h * HD + c * 32;
                         if constexpr (F32) {
@@ -789,7 +822,8 @@ __global__ void __launch_bounds__(kTcThreads, TcShape<HD, F32>::ctas) attn_tree_
                     }
                 }
             }
-            if (share && node >= 0) { part.ml[2 * at] = m_run; part.ml[2 * at + 1] = l_run; }
+            if ((share || clustered) && node >= 0) *(float2*)(clustered ? c_ml + 2 * row : part.ml + 2 * at) = make_float2(m_run, l_run);
+            __syncwarp();                            // (before another lane writes a row's share once more)
             // rows that are not finite, once more and key by key
             unsigned int bad = __ballot_sync(0xffffffffu, node >= 0 && odd != 0.0f && !*gave_up);
             const int j_first = max(t_first * kTileKeys, w.low), j_end = min(w.n_keys, (t_first + n_tiles) * kTileKeys);
@@ -797,10 +831,11 @@ __global__ void __launch_bounds__(kTcThreads, TcShape<HD, F32>::ctas) attn_tree_
                 const int r = warp_row + __ffs(bad) - 1, fr = f0 + r, nr = node_of(fr), hr = kvh * G + fr - nr * G;
                 float m, l, z[HD / 32];
                 tree_row_plain<HD, TQ>(a, tree, q, kvh, fr, j_first, j_end, lane, &m, &l, z);
-                if (share) {
-                    const size_t to = share_at(part, x.share, r);
-                    for (int i = 0; i < HD / 32; i++) part.o[to * HD + lane * (HD / 32) + i] = z[i];
-                    if (lane == 0) { part.ml[2 * to] = m; part.ml[2 * to + 1] = l; }
+                if (share || clustered) {
+                    const size_t to = share_at(part, max(x.share, 0), r);
+                    float* z_to = clustered ? c_o + r * kLd : part.o + to * HD;
+                    for (int i = 0; i < HD / 32; i++) z_to[lane * (HD / 32) + i] = z[i];
+                    if (lane == 0) *(float2*)(clustered ? c_ml + 2 * r : part.ml + 2 * to) = make_float2(m, l);
                 } else {
                     const float c = tree_inverse(a, hr, m, l);
                     TQ* dst = (TQ*)a.out + (size_t)(q.r0 + nr) * a.out_stride + (size_t)hr * HD + lane * (HD / 32);
@@ -809,6 +844,51 @@ __global__ void __launch_bounds__(kTcThreads, TcShape<HD, F32>::ctas) attn_tree_
             }
         }
         tc_fence_before_sync();
+    }
+    if (clustered) {                                 // ---- the unit's rows are shared out among the cluster's warps, which join the CTAs' shares of them
+        __syncwarp();
+        cluster_arrive_release();
+        cluster_wait_acquire();
+        const int C = part.cluster, rank = (int)blockIdx.x % C;
+        const uint32_t o_at = smem_u32(c_o), ml_at = smem_u32(c_ml);
+        using V = typename std::conditional<HD == 128, float4, float2>::type;
+        for (int r = rank + C * warp; r < live_rows; r += C * (kTcThreads / 32)) {
+            const int node = (f0 + r) / G, h = kvh * G + (f0 + r) - node * G;
+            float2 ml[kClusterMax];
+            V y[kClusterMax];
+#pragma unroll
+            for (int c = 0; c < kClusterMax; c++) {                  // all on their way at once
+                ml[c] = make_float2(-INFINITY, 0.0f);
+                if (c < C) {
+                    ml[c] = cluster_ld2(cluster_map(ml_at + (uint32_t)r * 8u, (uint32_t)c));
+                    const uint32_t from = cluster_map(o_at + (uint32_t)(r * kLd + lane * (HD / 32)) * 4u, (uint32_t)c);
+                    if constexpr (HD == 128) y[c] = cluster_ld4(from); else y[c] = cluster_ld2(from);
+                }
+            }
+            const float sink = a.sinks ? a.sinks[h] * kLog2e : -INFINITY;
+            float top = sink, z[HD / 32];
+#pragma unroll
+            for (int c = 0; c < kClusterMax; c++) top = fmaxf(top, ml[c].x);
+            float sum = !a.sinks ? 0.0f : sink == top ? 1.0f : exp2f(sink - top);
+#pragma unroll
+            for (int i = 0; i < HD / 32; i++) z[i] = 0.0f;
+#pragma unroll
+            for (int c = 0; c < kClusterMax; c++) {
+                if (ml[c].x == -INFINITY && ml[c].y == 0.0f) continue;         // no key that this row sees
+                const float f = ml[c].x == top || ml[c].y != ml[c].y ? 1.0f : exp2f(ml[c].x - top);      // (undefined sums stay undefined)
+                const float* part_of = (const float*)&y[c];
+                sum = fmaf(ml[c].y, f, sum);
+#pragma unroll
+                for (int i = 0; i < HD / 32; i++) z[i] = fmaf(part_of[i], f, z[i]);
+            }
+            const float inv = sum > 0.0f ? 1.0f / sum : sum;
+            TQ* dst = (TQ*)a.out + (size_t)(q.r0 + node) * a.out_stride + (size_t)h * HD + lane * (HD / 32);
+#pragma unroll
+            for (int i = 0; i < HD / 32; i++) dst[i] = out_of<TQ>(z[i] * inv);
+        }
+        __syncwarp();
+        cluster_arrive_release();                    // nobody leaves while another may read its shares
+        cluster_wait_acquire();
     }
     __syncthreads();
     if (warp == 5) tmem_dealloc(tmem, S::cols);
@@ -899,6 +979,15 @@ Bounds bounds_of(const TreeAttnArgs& a, int tile_rows) {
     if (a.window > 0) tiles = std::min(tiles, ((long long)a.window + a.t.max_rows) / kTileKeys + 2);
     return {(long long)a.t.n_seq * a.n_kv * ((a.t.max_rows * G + tile_rows - 1) / tile_rows), tiles};
 }
+// Few units of not too many tiles: a cluster for each, whose CTAs share its tiles evenly and join their shares through distributed shared memory.  One launch, no scratch, and
+// no search for pieces.  Measured against pieces and tree_combine (or, below 9 tiles, whole units), us in a graph, 8 K/V heads of 4 query heads of 128 in bf16, trees of 8:
+// 1 x 4 tiles 10.1 / 10.6 (of 32 nodes 13.7 / 12.6: more rows to join), 1 x 8 9.9 / 13.0, 1 x 63 13.7 / 17.5, 4 x 63 19.9 / 24.6, 1 x 251 27.6 / 34.7, 2 x 251 41.9 / 40.7, 1 x 501
+// 55.0 / 45.1 (8 CTAs a unit are too few).  Clusters of 16 gain 1 us at most and lose up to 10 where an SM holds one CTA.
+int cluster_of(const Bounds& b, int sm_count) {
+    int C = 1;
+    while (C < kClusterMax && 2 * C * b.units <= sm_count && 2 * C <= b.tiles) C *= 2;
+    return b.tiles > 4 && b.tiles <= (long long)C * 32 ? C : 1;
+}
 Share share_of(const TreeAttnArgs& a, int sm_count) {
     Share p{};
     const int G = a.n_q / a.n_kv;
@@ -907,9 +996,11 @@ Share share_of(const TreeAttnArgs& a, int sm_count) {
     p.rows = std::min(p.tile_rows, a.t.max_rows * G);
     p.slots = sm_count * (a.kv_bf16 && !a.q_bf16 && a.hd == 128 ? 1 : 2);
     const Bounds b = bounds_of(a, p.tile_rows);
-    // Few tiles: nothing is cut, and tree_combine (2 to 3 us, and as much of the caller's time) need not run.  Measured, us in a graph / per call from a program:
-    // one tree of 8 nodes over 508 rows in bf16 (8 tiles, 8 units) whole 12.7 / 18.2, cut 11.6 / 20.4; 5 trees of 13 over windows of 128 in f32 (3 tiles) whole 16.5, cut
-    // 18.0.  A tile takes CUDA cores four times as long: an f32 cache is cut sooner.
+    p.cluster = a.kv_bf16 ? cluster_of(b, sm_count) : 1;
+    p.row_tiles = (a.t.max_rows * G + p.tile_rows - 1) / p.tile_rows;
+    if (p.cluster > 1) { p.grid = (int)b.units * p.cluster; return p; }
+    // Few tiles: nothing is cut, and tree_combine (2 to 3 us, and as much of the caller's time) need not run.  Measured, us, whole / cut: 16 trees of 8 nodes over 508 rows in
+    // bf16 (8 tiles, 128 units) 14.4 / 16.8, 64 of them 39.6 / 44.6; an f32 cache takes four times as long a tile on CUDA cores, and is cut sooner.
     if (b.tiles <= (a.kv_bf16 ? 8 : 4)) { p.grid = (int)b.units; return p; }
     // Pieces, as piece_find cuts them: at most `slots` where there are fewer units than the slots it takes (all, or half of them), else at most units + tiles / (2 tiles
     // / slots).  Shares: the pieces of units that are cut; at most `slots` in both cases.
@@ -984,8 +1075,17 @@ cudaError_t tc_launch_copies(const TreeAttnArgs& a, const Share& p, cudaStream_t
     if constexpr (!F32) if (const cudaError_t e = map_queries(&map_q, a, p.tile_rows)) return e;
     if (const cudaError_t e = map_cache(&map_k, a, a.k, box_rows)) return e;
     if (const cudaError_t e = map_cache(&map_v, a, a.v, box_rows)) return e;
-    attn_tree_tc<HD, F32, DUP><<<p.grid, kTcThreads, S::smem, st>>>(a, p, map_q, map_k, map_v, box_rows);
-    const cudaError_t e = cudaGetLastError();
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3((unsigned)p.grid);
+    cfg.blockDim = dim3(kTcThreads);
+    cfg.dynamicSmemBytes = S::smem;
+    cfg.stream = st;
+    cudaLaunchAttribute at[1];
+    at[0].id = cudaLaunchAttributeClusterDimension;
+    at[0].val.clusterDim.x = (unsigned)p.cluster; at[0].val.clusterDim.y = 1; at[0].val.clusterDim.z = 1;
+    cfg.attrs = at;
+    cfg.numAttrs = p.cluster > 1 ? 1 : 0;
+    const cudaError_t e = cudaLaunchKernelEx(&cfg, attn_tree_tc<HD, F32, DUP>, a, p, map_q, map_k, map_v, box_rows);
     return e != cudaSuccess ? e : combine<HD, typename std::conditional<F32, float, __nv_bfloat16>::type>(a, p, st);
 }
 template <int HD, bool F32>

@@ -269,6 +269,38 @@ def test_attention_bad_numbers_on_the_device_are_left_out_and_reported(torch, op
 
 
 @pytest.mark.parametrize("q, cache", TYPES)
+@pytest.mark.parametrize("hint", [1000, 30000])
+@pytest.mark.parametrize("dim", [64, 128])
+@pytest.mark.parametrize("nodes, prefix, group", [([1, 0, 3], [0, 9, 300], 1), ([12, 2], [70, 1], 4), ([40, 33], [700, 2], 4), ([3], [63], 3), ([200], [500], 2)])
+def test_attention_of_few_keys_in_the_room_of_many(torch, ops, q, cache, hint, dim, nodes, prefix, group):
+    """The call's bounds ask for many CTAs per unit, the lengths leave some of them without a key."""
+    for window, sinks in ((0, False), (90, True)):
+        b = Batch(torch, ops, nodes, prefix, group=group, dim=dim, q=q, cache=cache, hint=hint, page=16, sinks=sinks)
+        b.check(b.run(window=window), window=window)
+    ops.status()
+
+
+@pytest.mark.parametrize("q, cache", TYPES)
+@pytest.mark.parametrize("hint", [0, 30000])
+@pytest.mark.parametrize("group", [1, 4, 8])
+def test_attention_leaves_out_infinities_where_a_unit_is_shared(torch, ops, q, cache, hint, group):
+    """As above, where several CTAs share a unit: their rows that are not finite are computed once more."""
+    b = Batch(torch, ops, [16], [1000], group=group, dim=128, q=q, cache=cache, kind="star", hint=hint)
+    at = [int(b.where[0][1000 + 5]), int(b.where[0][3])]     # a node, and a row that no node sees with this window
+    for r in at:
+        b.v[r] = float("inf")
+    got = b.run(window=990).clone()
+    ops.status()
+    for r in at:
+        b.v[r] = 0.0
+    want, off = b.want(window=990)
+    keep = [i for i in range(16) if i != 5]
+    bound = off[keep] + (2.0 ** -8 * (np.abs(want[keep]) + off[keep]) + 2.0 ** -14 if q == "bf16" else 0.0)
+    assert (np.abs(got.double().cpu().numpy()[keep] - want[keep]) <= bound).all()
+    assert not np.isfinite(got[5].float().cpu().numpy()).all()
+
+
+@pytest.mark.parametrize("q, cache", TYPES)
 @pytest.mark.parametrize("masked", [0.0, float("inf")])
 def test_attention_takes_the_rows_of_an_unknown_page_as_zeros(torch, ops, pkg, q, cache, masked):
     """Also where a row is computed key by key, because a value that it does not see is infinite."""
@@ -453,7 +485,7 @@ def test_attention_with_a_window_that_reaches_over_everything(torch, ops, q, cac
 
 
 def test_attention_with_a_workspace_of_the_caller(torch, ops, pkg):
-    b = Batch(torch, ops, [9, 30], [3000, 90], dim=128, group=4)
+    b = Batch(torch, ops, [9, 30], [3000, 90], dim=128, group=4, hint=30000)     # (a shorter bound needs none)
     want = b.run().clone()
     ws = torch.empty(64 << 20, dtype=torch.uint8, device="cuda")
     assert torch.equal(b.run(workspace=ws), want)
