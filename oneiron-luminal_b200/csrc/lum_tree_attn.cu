@@ -100,17 +100,17 @@ __device__ __forceinline__ void piece_find(const TreeAttnArgs& a, const Share& p
         return y;
     };
     const SeqWork mine = work(lane);                 // (batches of up to 32 sequences: all there is)
-    int units = mine.units, total = mine.units * mine.tiles;                   // (the call bounds them)
+    int units = mine.units, total = mine.units * mine.tiles, longest = mine.units ? mine.tiles : 0;             // (the call bounds them)
 #pragma unroll 1
-    for (int s0 = 32; s0 < a.t.n_seq; s0 += 32) { const SeqWork y = work(s0 + lane); units += y.units; total += y.units * y.tiles; }
+    for (int s0 = 32; s0 < a.t.n_seq; s0 += 32) { const SeqWork y = work(s0 + lane); units += y.units; total += y.units * y.tiles; longest = max(longest, y.units ? y.tiles : 0); }
     units = __reduce_add_sync(0xffffffffu, units);
     total = __reduce_add_sync(0xffffffffu, total);
-    // Little work: a CTA on every SM, of two tiles at least, rather than two (which begin at the same time and get in each other's way)
-    const int slots = total < 4 * p.slots ? p.slots / 2 : p.slots;
+    longest = __reduce_max_sync(0xffffffffu, longest);
+    const int slots = p.slots;
     const float even = (float)total / (float)slots;
     int per = p.shares ? (int)(2.0f * even) + 2 : 1 << 30;
     if (p.shares && units < slots) {
-        per = max((int)even + 1, 2);
+        per = max((int)even + 1, (int)sqrtf((float)longest * (a.kv_bf16 ? 1.0f / 3.0f : 1.0f / 48.0f)) + 1);
 #pragma unroll 1
         for (int i = 0; i < 4; i++) {
             int n = mine.units * pieces_of(mine.tiles, per);
@@ -175,23 +175,32 @@ __device__ __forceinline__ float tree_inverse(const TreeAttnArgs& a, int h, floa
     return sum > 0.0f ? c / sum : sum;
 }
 
+// Pairs of floats in 64-bit registers, whose operations issue once for two.
+using F2 = unsigned long long;
+__device__ __forceinline__ F2 pack2(float a, float b) { F2 r; asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(a), "f"(b)); return r; }
+__device__ __forceinline__ F2 pack2(uint32_t a, uint32_t b) { F2 r; asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "r"(a), "r"(b)); return r; }
+__device__ __forceinline__ float2 unpack2(F2 x) { float2 r; asm("mov.b64 {%0, %1}, %2;" : "=f"(r.x), "=f"(r.y) : "l"(x)); return r; }
+__device__ __forceinline__ F2 fma2(F2 a, F2 b, F2 c) { F2 r; asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c)); return r; }
+__device__ __forceinline__ F2 mul2(F2 a, F2 b) { F2 r; asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b)); return r; }
+__device__ __forceinline__ F2 add2(F2 a, F2 b) { F2 r; asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b)); return r; }
+
 // ---- products on CUDA cores, in 32 bits: an f32 cache
-// A unit has 32 query rows; 8 warps of 4 query rows.  32 keys at a time lie in shared memory as f32: a lane multiplies its key with the warp's four rows, and
-// then four (two) dimensions of the values with their weights.
-constexpr int kRowsTile = 32, kRowsKeys = 32;
+// A unit has 32 query rows; 8 warps of 4 query rows.  A tile of 64 keys lies in shared memory as f32: a lane multiplies two keys with the warp's four rows, and then four
+// (two) dimensions of the values with their weights.  Bound by what is read from shared memory.
+constexpr int kRowsTile = 32, kRowsKeys = kTileKeys;
 template <int HD>
-constexpr int rows_smem() { return (kRowsTile * HD + kRowsKeys * (HD + 4) + kRowsKeys * HD + kRowsTile * kRowsKeys) * 4 + (int)sizeof(Piece) + (int)sizeof(TreeNodes); }
+constexpr int rows_smem() { return (kRowsTile * HD + kRowsKeys * (HD + 4) + kRowsKeys * HD + 2 * kRowsTile * kRowsKeys) * 4 + (int)sizeof(Piece) + (int)sizeof(TreeNodes); }
 
 template <int HD>
-__global__ void __launch_bounds__(256) attn_tree_rows(const TreeAttnArgs a, const Share part) {
+__global__ void __launch_bounds__(256, 2) attn_tree_rows(const TreeAttnArgs a, const Share part) {
     extern __shared__ __align__(16) unsigned char smem[];
     float* s_q = (float*)smem;                       // [32][HD]
-    float* s_k = s_q + kRowsTile * HD;               // [32][HD + 4]
-    float* s_v = s_k + kRowsKeys * (HD + 4);         // [32][HD]
-    float* s_p = s_v + kRowsKeys * HD;               // [32 rows][32 keys]
-    Piece* s_piece = (Piece*)(s_p + kRowsTile * kRowsKeys);
+    float* s_k = s_q + kRowsTile * HD;               // [64][HD + 4]
+    float* s_v = s_k + kRowsKeys * (HD + 4);         // [64][HD]
+    float* s_p = s_v + kRowsKeys * HD;               // [8 warps][64 keys][4 rows], each weight twice
+    Piece* s_piece = (Piece*)(s_p + 2 * kRowsTile * kRowsKeys);
     TreeNodes& tree = *(TreeNodes*)(s_piece + 1);
-    constexpr int DPL = HD / 32;
+    constexpr int DPL = HD / 32, PPL = DPL / 2;
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, G = a.n_q / a.n_kv;
     if (warp == 0) piece_find(a, part, lane, s_piece);
     __syncthreads();
@@ -208,7 +217,8 @@ __global__ void __launch_bounds__(256) attn_tree_rows(const TreeAttnArgs a, cons
             if (f < q.n * G) v = *(const float4*)((const float*)a.q + (size_t)(q.r0 + f / G) * a.q_stride + ((size_t)x.kvh * G + f % G) * HD + c);
             *(float4*)(s_q + r * HD + c) = v;
         }
-        float o[4][DPL], mx[4], l[4];
+        F2 o[4][PPL];
+        float mx[4], l[4];
         int node[4];
 #pragma unroll
         for (int r = 0; r < 4; r++) {
@@ -216,75 +226,117 @@ __global__ void __launch_bounds__(256) attn_tree_rows(const TreeAttnArgs a, cons
             const int f = x.f0 + warp * 4 + r;
             node[r] = f < q.n * G ? f / G : -1;
 #pragma unroll
-            for (int i = 0; i < DPL; i++) o[r][i] = 0.0f;
+            for (int i = 0; i < PPL; i++) o[r][i] = 0ull;
         }
         const int j_first = (w.t_lo + x.tile) * kTileKeys, j_end = min(w.n_keys, j_first + x.tiles * kTileKeys);
 #pragma unroll 1
         for (int j0 = j_first; j0 < j_end; j0 += kRowsKeys) {
             __syncthreads();                         // (the tree and the queries are there; the tile before has been read)
-            for (int e = tid; e < kRowsKeys * HD / 4; e += 256) {
-                const int r = e / (HD / 4), c = e % (HD / 4) * 4, j = j0 + r;
-                float4 kf = make_float4(0.0f, 0.0f, 0.0f, 0.0f), vf = kf;
-                const long long at = j >= w.low && j < j_end ? tree_row(a.m, q.slot, j, a.status) : -1;
-                if (at >= 0) {
-                    const size_t off = (size_t)at * a.kv_stride + (size_t)x.kvh * HD + c;
-                    kf = *(const float4*)((const float*)a.k + off);
-                    vf = *(const float4*)((const float*)a.v + off);
+            constexpr int kStep = 256 / (HD / 4), kBatch = 4;        // a thread has one column of every kStep-th row
+            const int col = tid % (HD / 4) * 4;
+#pragma unroll 1
+            for (int r0 = tid / (HD / 4); r0 < kRowsKeys; r0 += kStep * kBatch) {
+                float4 kf[kBatch], vf[kBatch];
+#pragma unroll
+                for (int u = 0; u < kBatch; u++) {
+                    const int j = j0 + r0 + u * kStep;
+                    const long long at = j >= w.low && j < j_end ? tree_row(a.m, q.slot, j, a.status) : -1;
+                    kf[u] = vf[u] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+                    if (at >= 0) {
+                        const size_t off = (size_t)at * a.kv_stride + (size_t)x.kvh * HD + col;
+                        kf[u] = *(const float4*)((const float*)a.k + off);
+                        vf[u] = *(const float4*)((const float*)a.v + off);
+                    }
                 }
-                *(float4*)(s_k + r * (HD + 4) + c) = kf;
-                *(float4*)(s_v + r * HD + c) = vf;
+#pragma unroll
+                for (int u = 0; u < kBatch; u++) {
+                    *(float4*)(s_k + (r0 + u * kStep) * (HD + 4) + col) = kf[u];
+                    *(float4*)(s_v + (r0 + u * kStep) * HD + col) = vf[u];
+                }
             }
             __syncthreads();
-            float y[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+            F2 y[2][4];
+#pragma unroll
+            for (int r = 0; r < 4; r++) y[0][r] = y[1][r] = 0ull;
             const float* qr = s_q + warp * 4 * HD;
-#pragma unroll 8
+#pragma unroll 4
             for (int c = 0; c < HD; c += 4) {
-                const float4 k4 = *(const float4*)(s_k + lane * (HD + 4) + c);
+                const ulonglong2 ka = *(const ulonglong2*)(s_k + lane * (HD + 4) + c), kb = *(const ulonglong2*)(s_k + (lane + 32) * (HD + 4) + c);
 #pragma unroll
                 for (int r = 0; r < 4; r++) {
-                    const float4 q4 = *(const float4*)(qr + r * HD + c);
-                    y[r] = fmaf(q4.x, k4.x, fmaf(q4.y, k4.y, fmaf(q4.z, k4.z, fmaf(q4.w, k4.w, y[r]))));
+                    const ulonglong2 q4 = *(const ulonglong2*)(qr + r * HD + c);
+                    y[0][r] = fma2(q4.y, ka.y, fma2(q4.x, ka.x, y[0][r]));
+                    y[1][r] = fma2(q4.y, kb.y, fma2(q4.x, kb.x, y[1][r]));
                 }
             }
-            const int j = j0 + lane;
-            const bool live = j >= w.low && j < j_end;
-            unsigned int vis[4], all = 0xffffffffu;
+            unsigned int vis[2][4], all = 0xffffffffu;
+            float pr[2][4];
 #pragma unroll
             for (int r = 0; r < 4; r++) {
-                const bool see = live && node[r] >= 0 && tree_sees(tree, q, a.window, node[r], j);
-                vis[r] = __ballot_sync(0xffffffffu, see);
-                all &= vis[r];
-                const float z = see ? y[r] * scale : -INFINITY;
-                float top = z;
+                float z[2];
+#pragma unroll
+                for (int h = 0; h < 2; h++) {
+                    const int j = j0 + lane + 32 * h;
+                    const bool see = j >= w.low && j < j_end && node[r] >= 0 && tree_sees(tree, q, a.window, node[r], j);
+                    vis[h][r] = __ballot_sync(0xffffffffu, see);
+                    all &= vis[h][r];
+                    const float2 t = unpack2(y[h][r]);
+                    z[h] = see ? (t.x + t.y) * scale : -INFINITY;
+                }
+                float top = fmaxf(z[0], z[1]);
 #pragma unroll
                 for (int i = 16; i > 0; i >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, i));
-                const float mn = fmaxf(mx[r], top);
-                const float p = see ? exp2f(z - (mn == -INFINITY ? 0.0f : mn)) : 0.0f;
+                const float mn = fmaxf(mx[r], top), off = mn == -INFINITY ? 0.0f : mn;
+#pragma unroll
+                for (int h = 0; h < 2; h++) pr[h][r] = vis[h][r] >> lane & 1u ? exp2f(z[h] - off) : 0.0f;
                 const float corr = mx[r] == mn ? 1.0f : exp2f(mx[r] - mn);
-                l[r] = l[r] * corr + p;
+                l[r] = l[r] * corr + (pr[0][r] + pr[1][r]);
                 mx[r] = mn;
+                const F2 corr2 = pack2(corr, corr);
 #pragma unroll
-                for (int i = 0; i < DPL; i++) o[r][i] *= corr;
-                s_p[(warp * 4 + r) * kRowsKeys + lane] = p;
+                for (int i = 0; i < PPL; i++) o[r][i] = mul2(o[r][i], corr2);
             }
+#pragma unroll
+            for (int h = 0; h < 2; h++)
+#pragma unroll
+                for (int r = 0; r < 4; r += 2)
+                    *(float4*)(s_p + ((warp * kRowsKeys + lane + 32 * h) * 4 + r) * 2) = make_float4(pr[h][r], pr[h][r], pr[h][r + 1], pr[h][r + 1]);
             __syncwarp();
-            // a key that a row does not see adds nothing to it, whatever its value holds (0 times infinity is no zero)
-#pragma unroll 4
-            for (int key = 0; key < kRowsKeys; key++) {
-                float v[DPL];
+            using V = typename std::conditional<HD == 128, ulonglong2, F2>::type;
+            const float *pw = s_p + warp * kRowsKeys * 8, *vl = s_v + lane * DPL;
+            if (all == 0xffffffffu) {
+#pragma unroll 8
+                for (int key = 0; key < kRowsKeys; key++) {
+                    const V v = *(const V*)(vl + key * HD);
+                    const ulonglong2 p01 = *(const ulonglong2*)(pw + key * 8), p23 = *(const ulonglong2*)(pw + key * 8 + 4);
+                    const F2 p2[4] = {p01.x, p01.y, p23.x, p23.y};
 #pragma unroll
-                for (int i = 0; i < DPL; i++) v[i] = s_v[key * HD + lane * DPL + i];
+                    for (int r = 0; r < 4; r++)
 #pragma unroll
-                for (int r = 0; r < 4; r++) {
-                    if (all == 0xffffffffu || (vis[r] >> key & 1u)) {
-                        const float p = s_p[(warp * 4 + r) * kRowsKeys + key];
+                        for (int i = 0; i < PPL; i++) o[r][i] = fma2(p2[r], ((const F2*)&v)[i], o[r][i]);
+                }
+            } else {
+                // a key that a row does not see adds nothing to it, whatever its value holds (0 times infinity is no zero)
+#pragma unroll 1
+                for (int key = 0; key < kRowsKeys; key++) {
+                    const V v = *(const V*)(vl + key * HD);
 #pragma unroll
-                        for (int i = 0; i < DPL; i++) o[r][i] = fmaf(p, v[i], o[r][i]);
+                    for (int r = 0; r < 4; r++) {
+                        if ((key < 32 ? vis[0][r] : vis[1][r]) >> (key & 31) & 1u) {
+                            const F2 p2 = *(const F2*)(pw + key * 8 + 2 * r);
+#pragma unroll
+                            for (int i = 0; i < PPL; i++) o[r][i] = fma2(p2, ((const F2*)&v)[i], o[r][i]);
+                        }
                     }
                 }
             }
             __syncwarp();
         }
+        float out[4][DPL];
+#pragma unroll
+        for (int r = 0; r < 4; r++)
+#pragma unroll
+            for (int i = 0; i < PPL; i++) { const float2 t = unpack2(o[r][i]); out[r][2 * i] = t.x; out[r][2 * i + 1] = t.y; }
 #pragma unroll
         for (int r = 0; r < 4; r++) {
             if (node[r] < 0) continue;
@@ -293,13 +345,13 @@ __global__ void __launch_bounds__(256) attn_tree_rows(const TreeAttnArgs a, cons
             if (x.share >= 0) {
                 const size_t at = share_at(part, x.share, warp * 4 + r);
 #pragma unroll
-                for (int i = 0; i < DPL; i++) part.o[at * HD + lane * DPL + i] = o[r][i];
+                for (int i = 0; i < DPL; i++) part.o[at * HD + lane * DPL + i] = out[r][i];
                 if (lane == 0) { part.ml[2 * at] = mx[r]; part.ml[2 * at + 1] = sum; }
             } else {
                 const float inv = tree_inverse(a, h, mx[r], sum);
                 float* dst = (float*)a.out + (size_t)row * a.out_stride + (size_t)h * HD + lane * DPL;
 #pragma unroll
-                for (int i = 0; i < DPL; i++) dst[i] = o[r][i] * inv;
+                for (int i = 0; i < DPL; i++) dst[i] = out[r][i] * inv;
             }
         }
     }
@@ -367,13 +419,6 @@ __device__ __forceinline__ void tc_st_wait() { asm volatile("tcgen05.wait::st.sy
 // (passes over NaN as fmaxf does)
 __device__ __forceinline__ float max3(float a, float b, float c) { float r; asm("max.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c)); return r; }
 __device__ __forceinline__ float tc_ex2(float x) { float y; asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x)); return y; }
-// Pairs of floats in 64-bit registers: the softmax warps are bound by what they issue, and these issue once for two.
-using F2 = unsigned long long;
-__device__ __forceinline__ F2 pack2(float a, float b) { F2 r; asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(a), "f"(b)); return r; }
-__device__ __forceinline__ F2 pack2(uint32_t a, uint32_t b) { F2 r; asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "r"(a), "r"(b)); return r; }
-__device__ __forceinline__ float2 unpack2(F2 x) { float2 r; asm("mov.b64 {%0, %1}, %2;" : "=f"(r.x), "=f"(r.y) : "l"(x)); return r; }
-__device__ __forceinline__ F2 fma2(F2 a, F2 b, F2 c) { F2 r; asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c)); return r; }
-__device__ __forceinline__ F2 add2(F2 a, F2 b) { F2 r; asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b)); return r; }
 // x as packed bf16, rounded; what is left of it goes back
 __device__ __forceinline__ uint32_t tc_term(F2* x, F2 minus_one) {
     const float2 y = unpack2(*x);
@@ -1002,9 +1047,9 @@ Share share_of(const TreeAttnArgs& a, int sm_count) {
     // Few tiles: nothing is cut, and tree_combine (2 to 3 us, and as much of the caller's time) need not run.  Measured, us, whole / cut: 16 trees of 8 nodes over 508 rows in
     // bf16 (8 tiles, 128 units) 14.4 / 16.8, 64 of them 39.6 / 44.6; an f32 cache takes four times as long a tile on CUDA cores, and is cut sooner.
     if (b.tiles <= (a.kv_bf16 ? 8 : 4)) { p.grid = (int)b.units; return p; }
-    // Pieces, as piece_find cuts them: at most `slots` where there are fewer units than the slots it takes (all, or half of them), else at most units + tiles / (2 tiles
-    // / slots).  Shares: the pieces of units that are cut; at most `slots` in both cases.
-    p.grid = (int)std::min(b.units * b.tiles, std::max((long long)p.slots, b.units + p.slots / 2));
+    // Pieces, as piece_find cuts them: at most `slots` where there are fewer units, else at most units + tiles / (2 tiles / slots).  Shares: the pieces of units that are cut, at
+    // most `slots` in both cases.
+    p.grid = (int)std::min(b.units * b.tiles, b.units < p.slots ? (long long)p.slots : b.units + p.slots / 2);
     p.shares = std::min(p.grid, p.slots);
     return p;
 }
