@@ -88,8 +88,11 @@ __device__ __forceinline__ int warp_scan(int x, int lane) {                    /
 }
 // The CTA's piece, by one warp (x->s -1: none); CTA 0 writes the plan down.
 // A piece is at most `per` tiles long.  Where there are fewer units than CTAs that run at once, the pieces should be as many as those, nearly: the even share of all
-// tiles, longer by what rounding up makes of it.  (Pieces are at most units + tiles / per, so the last choice always fits.)  Where there are more units, only one longer
-// than twice the even share is cut.  Short code: every CTA runs it once, cold.
+// tiles, longer by what rounding up makes of it.  (Pieces are at most units + tiles / per, so the last choice always fits.)  But a piece costs tree_combine about a third
+// of a tile's time (a 48th, of a tile on CUDA cores): n tiles in pieces of p take p + n / (3 p) tiles' time, least at p = sqrt(n / 3).  Measured with this bound /
+// without, us: 1 K/V head of 4 query heads, a tree of 8 over 32000 rows 25 / 60, 2 of them over 40000 28 / 47.  Where there are more units, only one longer than twice the even
+// share is cut.  Pieces twice to six times as many (for SMs that are faster than others) gained nothing: 284 to 345 us for 16 trees of 32 over up to 32768 rows, 268 so; nor
+// did an order that puts long and short pieces together on an SM (271 / 272).  Short code: every CTA runs it once, cold.
 __device__ __forceinline__ void piece_find(const TreeAttnArgs& a, const Share& p, int lane, Piece* x) {
     auto work = [&](int s) {
         SeqWork y{{}, 0, 1};
@@ -167,7 +170,7 @@ template <typename T> __device__ __forceinline__ T out_of(float x);
 template <> __device__ __forceinline__ float out_of<float>(float x) { return x; }
 template <> __device__ __forceinline__ __nv_bfloat16 out_of<__nv_bfloat16>(float x) { return __float2bfloat16_rn(x); }      // the one rounding of the result
 
-// What a finished segment's row becomes: its share, or the result, which is out = o / l with the sink's part in l.
+// The factor of a finished row: out = o / l, with the sink's part in l.
 __device__ __forceinline__ float tree_inverse(const TreeAttnArgs& a, int h, float m, float l) {
     if (!a.sinks) return l > 0.0f ? 1.0f / l : l;    // (undefined stays undefined)
     const float sink = a.sinks[h] * kLog2e, top = fmaxf(m, sink), c = m == -INFINITY ? 0.0f : exp2f(m - top);
@@ -186,7 +189,8 @@ __device__ __forceinline__ F2 add2(F2 a, F2 b) { F2 r; asm("add.rn.f32x2 %0, %1,
 
 // ---- products on CUDA cores, in 32 bits: an f32 cache
 // A unit has 32 query rows; 8 warps of 4 query rows.  A tile of 64 keys lies in shared memory as f32: a lane multiplies two keys with the warp's four rows, and then four
-// (two) dimensions of the values with their weights.  Bound by what is read from shared memory.
+// (two) dimensions of the values with their weights.  Bound by what is read from shared memory: every warp reads all keys and values.  8 trees of 8 nodes over 4000 rows, 8 K/V
+// heads of 4 query heads of 128 (8.4 GFLOP): 208 us, 40 TFLOP/s; with one key a lane and no pairs 291.
 constexpr int kRowsTile = 32, kRowsKeys = kTileKeys;
 template <int HD>
 constexpr int rows_smem() { return (kRowsTile * HD + kRowsKeys * (HD + 4) + kRowsKeys * HD + 2 * kRowsTile * kRowsKeys) * 4 + (int)sizeof(Piece) + (int)sizeof(TreeNodes); }
@@ -358,11 +362,13 @@ __global__ void __launch_bounds__(256, 2) attn_tree_rows(const TreeAttnArgs a, c
 }
 
 // ---- products on the tensor core (tcgen05): a bf16 cache
-// CTA = chunk x (K/V head, 128 query rows) x sequence: four softmax warps, a thread per query row; one warp that asks for keys, one for
-// values, one that issues the products.  Per tile of 64 cache rows:
+// Four softmax warps, a thread per query row; one warp that asks for keys, one for values, one that issues the products (and asks for bf16 queries: a copy per 64
+// dimensions brings a unit's rows as the operand wants them).  Per tile of 64 cache rows:
 //     S = Q K^T             M 128, N 64; Q in shared memory, one bf16 term (bf16 queries) or three (f32 queries, 24 bits)
 //     p = 2^(S - m)         a thread reads its row's 64 scores, masks, exponentiates, and stores the weights' terms over them
 //     O (+)= P V            M 128, N head_dim; P from tensor memory, V as stored (MN-major)
+// Up to 64 (32) query rows lie in the operand two (four) times: copy c takes the softmax of every tile's c-th half (quarter) of the keys, with zeros as the weights of the
+// others, and the copies are joined at the end, so that all four warps have work whatever the rows.
 // Tiles arrive by one tensor-map copy each for K and V (a box per page where pages are smaller than a tile), two tiles ahead; rows that the call must not
 // read (before the window, behind the last node, pages outside the pool) are asked for outside the tensor and read as zeros.  S(t + 1) is computed while tile t
 // is exponentiated.
@@ -373,6 +379,12 @@ __global__ void __launch_bounds__(256, 2) attn_tree_rows(const TreeAttnArgs a, c
 //     thousands of keys the cuts add up.  Low terms go first.
 // A key that a row does not see has weight 0, but 0 times infinity is no zero: rows of V behind the last node or before the window are zeroed, and a row whose
 // result is not finite is computed again by tree_row_plain, key by key.
+// What bounds it, and what it measured (in a graph, SM clock 1.9 GHz): 16 trees of 32 nodes over up to 32768 rows in pages of 16, 8 K/V heads of 4 query heads of 128 (1.28 GB):
+// 268 us, 4.8 TB/s; with more products per byte than HBM alone would let them wait for, it slows down with the SMs' clock (328 us at the 1.4 GHz that a second of such calls is
+// held to).  8 trees of 64 over 4096 rows, 8 query heads of 64 per K/V head (34.6 GFLOP): 90 us, 385 TFLOP/s; bound by the softmax warps (ALU and exponentials busy half of the
+// time each, issue 46 %).  32 trees of up to 16 over up to 2048 rows (0.18 GB): 49 us, 3.7 TB/s, of which launch, first tiles and joining are 15.  Tried without gain: two
+// threads per query row (104 us to 107 where this came to 104), weights by the maximum of the tile before with a second try where it grew (112), room for four tiles
+// (n_seq 1 .. 8 with 4000 .. 16000 rows: 13.9 / 14.1, 27.8 / 29.7, 36.4 / 32.2, 25.1 / 37.0: with that much shared memory clusters no longer fit beside one another).
 constexpr int kTcGroup = 128 * 16 + 16;              // f32 queries' terms: 16-byte column groups of 128 rows, the next one 16 bytes further on (banks)
 constexpr int kTcThreads = 224;                     // four softmax warps, keys, products, values
 template <int HD, bool F32>
@@ -1011,7 +1023,8 @@ __global__ void __launch_bounds__(256, 6) tree_combine(const TreeAttnArgs a, con
     for (int i = 0; i < DPL; i++) dst[i] = out_of<TQ>(o[i] * inv);
 }
 
-// Copies of the query rows in a tile of 128 (see attn_tree_tc): as many as there is room for.
+// Copies of the query rows in a tile of 128 (see attn_tree_tc): as many as there is room for.  Measured with / without, us: 32 trees of 16 nodes of 4 query heads (2 copies) 53 / 65
+// when they came in, 10 trees of 8 over 850 rows (4) 20.3 / 22.2, 16 of 16 over 16000 (2) 212 / 241, 16 of 8 over 16000 (4; bound by HBM) 185 / 177, one of 8 over 500 10.0 / 9.5.
 int copies_of(const TreeAttnArgs& a) {
     const int rows = a.t.max_rows * (a.n_q / a.n_kv);
     return rows <= 32 ? 4 : rows <= 64 ? 2 : 1;
