@@ -14,6 +14,7 @@ namespace lum {
 namespace {
 
 constexpr float kLog2e = 1.4426950408889634f;
+constexpr int kJoinCtas = 5;                         // CTAs of tree_combine per SM
 constexpr int kClusterMax = 8;                       // CTAs of a (portable) cluster
 constexpr int kTileKeys = 64;                        // tiles of so many cache rows, from the first visible one's tile on
 
@@ -65,12 +66,13 @@ __device__ __forceinline__ bool tree_sees(const TreeNodes& s, const TreeSeq& q, 
 // How the work is shared out.  A unit is a (sequence, K/V head, tile of query rows); it may be cut into equal pieces of its tiles of keys, one CTA per piece.  How
 // long a piece may be is chosen on the device, where the lengths are.  A whole unit is finished by its CTA; a unit in pieces leaves a share (maximum, sum,
 // outputs) of each in the workspace, and tree_combine joins them.
+constexpr int kNoCut = 1 << 30;                       // as the longest piece: longer than any unit
 struct Share {
     int* plan;                                       // [0] tiles of a piece at most, [1 + s] the first share of sequence s; written by CTA 0 for tree_combine
     float *ml, *o;                                   // [share][rows][2], [share][rows][hd]
     int grid, shares, slots;                         // CTAs launched, shares there is room for, CTAs that run at once
     int copies, rows, tile_rows;                     // copies of a query row in a tile, query rows of a share, of a unit
-    int cluster, row_tiles;                          // > 1: a cluster of so many CTAs per unit; units of a K/V head there may be
+    int cluster, row_tiles, sms;                     // > 1: a cluster of so many CTAs per unit; units of a K/V head there may be; the card's SMs
 };
 __device__ __forceinline__ size_t share_at(const Share& p, int share, int r) { return (size_t)share * p.rows + r; }
 
@@ -111,7 +113,7 @@ __device__ __forceinline__ void piece_find(const TreeAttnArgs& a, const Share& p
     longest = __reduce_max_sync(0xffffffffu, longest);
     const int slots = p.slots;
     const float even = (float)total / (float)slots;
-    int per = p.shares ? (int)(2.0f * even) + 2 : 1 << 30;
+    int per = p.shares ? (int)(2.0f * even) + 2 : kNoCut;
     if (p.shares && units < slots) {
         per = max((int)even + 1, (int)sqrtf((float)longest * (a.kv_bf16 ? 1.0f / 3.0f : 1.0f / 48.0f)) + 1);
 #pragma unroll 1
@@ -125,7 +127,6 @@ __device__ __forceinline__ void piece_find(const TreeAttnArgs& a, const Share& p
         }
     }
     const bool plans = blockIdx.x == 0 && p.shares;  // (without shares nobody reads it)
-    if (plans && lane == 0) p.plan[0] = per;
     if (lane == 0) x->s = -1;
     __syncwarp();
     int before = 0, shares = 0;
@@ -150,6 +151,7 @@ __device__ __forceinline__ void piece_find(const TreeAttnArgs& a, const Share& p
         shares += __shfl_sync(0xffffffffu, cuts, 31);
         if (blockIdx.x && (int)blockIdx.x < before) break;
     }
+    if (plans && lane == 0) p.plan[0] = shares ? per : kNoCut;
 }
 
 // The piece of a CTA of a cluster: its part of the unit's tiles (perhaps none).  By one thread.
@@ -381,7 +383,7 @@ __global__ void __launch_bounds__(256, 2) attn_tree_rows(const TreeAttnArgs a, c
 // result is not finite is computed again by tree_row_plain, key by key.
 // What bounds it, and what it measured (in a graph, SM clock 1.9 GHz): 16 trees of 32 nodes over up to 32768 rows in pages of 16, 8 K/V heads of 4 query heads of 128 (1.28 GB):
 // 268 us, 4.8 TB/s; with more products per byte than HBM alone would let them wait for, it slows down with the SMs' clock (328 us at the 1.4 GHz that a second of such calls is
-// held to).  8 trees of 64 over 4096 rows, 8 query heads of 64 per K/V head (34.6 GFLOP): 90 us, 385 TFLOP/s; bound by the softmax warps (ALU and exponentials busy half of the
+// held to).  8 trees of 64 over 4096 rows, 8 query heads of 64 per K/V head (34.6 GFLOP): 84 us, 410 TFLOP/s; bound by the softmax warps (ALU and exponentials busy half of the
 // time each, issue 46 %).  32 trees of up to 16 over up to 2048 rows (0.18 GB): 49 us, 3.7 TB/s, of which launch, first tiles and joining are 15.  Tried without gain: two
 // threads per query row (104 us to 107 where this came to 104), weights by the maximum of the tile before with a second try where it grew (112), room for four tiles
 // (n_seq 1 .. 8 with 4000 .. 16000 rows: 13.9 / 14.1, 27.8 / 29.7, 36.4 / 32.2, 25.1 / 37.0: with that much shared memory clusters no longer fit beside one another).
@@ -953,74 +955,84 @@ __global__ void __launch_bounds__(kTcThreads, TcShape<HD, F32>::ctas) attn_tree_
 }
 
 // ---- joins the shares of units that were cut: a warp per (row, head); o = sum_c 2^(m_c - M) o_c / (sum_c 2^(m_c - M) l_c + 2^(sink - M)).  Most warps of a batch find
-// that their unit was not cut, so what counts is how soon they know.
+// that their unit was not cut, so what counts is how soon they know: no more than two rounds of CTAs, which end at once where nothing was cut
+// (8 trees of 64 nodes over 4096 rows, none cut, 84 us, with a CTA for every eight results 89; 64 of 32 over 1000, 71 and 83).
 template <int HD, typename TQ>
-__global__ void __launch_bounds__(256, 6) tree_combine(const TreeAttnArgs a, const Share part) {
+__global__ void __launch_bounds__(256, kJoinCtas) tree_combine(const TreeAttnArgs a, const Share part) {
     constexpr int DPL = HD / 32;
-    const int lane = threadIdx.x & 31, G = a.n_q / a.n_kv, blocks = (a.n_q + 7) >> 3, row = (int)(blockIdx.x / (unsigned)blocks), h = ((int)blockIdx.x - row * blocks) * 8 + (threadIdx.x >> 5);
-    // the row's sequence: the last one that starts at or before it, 32 at a time
-    int s = 0;
-    for (int len = a.t.n_seq; len > 1;) {
-        const int step = (len + 31) >> 5, at = lane * step;
-        const unsigned int m = __ballot_sync(0xffffffffu, at < len && __ldg(a.t.row_start + s + min(at, len - 1)) <= row);
-        const int k = m ? 31 - __clz(m) : 0;
-        s += k * step;
-        len = min(step, len - k * step);
-    }
-    TreeSeq q;
-    const bool mine = h < a.n_q && tree_seq(a.t, &a.m, s, &q, nullptr) && row >= q.r0 && row < q.r0 + q.n;
-    pdl_grid_wait();                                 // (what comes before does not depend on the kernel before; every warp waits, so that this kernel ends behind that one)
-    if (!mine) return;
-    const int per = __ldcg(part.plan), first_of_seq = __ldcg(part.plan + 1 + s), shares = pieces_of(tree_work(q.prefix, q.n, a.window).n_tiles, per);
-    if (shares == 1) return;                         // finished by its CTA
-    const int f = (row - q.r0) * G + h % G, R = part.tile_rows, first = first_of_seq + (h / G * ((q.n * G + R - 1) / R) + f / R) * shares, r = f % R;
-    const float sink = a.sinks ? a.sinks[h] * kLog2e : -INFINITY;
-    float top = sink, sum = a.sinks ? 1.0f : 0.0f, o[DPL];
-#pragma unroll
-    for (int i = 0; i < DPL; i++) o[i] = 0.0f;
-    // 32 shares at a time: a lane has the factor of one, all have their dimensions of each, four on their way
-    for (int c0 = 0; c0 < shares; c0 += 32) {
-        float m = -INFINITY, l = 0.0f;
-        if (c0 + lane < shares) {
-            const float2 v = __ldcg((const float2*)part.ml + share_at(part, first + c0 + lane, r));
-            m = v.x; l = v.y;
+    const int lane = threadIdx.x & 31, G = a.n_q / a.n_kv, blocks = (a.n_q + 7) >> 3;
+    const unsigned int items = (unsigned)a.t.n_rows * (unsigned)blocks;      // (below 2^31)
+    int per = 0;
+#pragma unroll 1
+    for (unsigned int item = blockIdx.x; item < items; item += gridDim.x) {
+        const int row = (int)(item / (unsigned)blocks), h = ((int)item - row * blocks) * 8 + (threadIdx.x >> 5);
+        // the row's sequence: the last one that starts at or before it, 32 at a time
+        int s = 0;
+        for (int len = a.t.n_seq; len > 1;) {
+            const int step = (len + 31) >> 5, at = lane * step;
+            const unsigned int m = __ballot_sync(0xffffffffu, at < len && __ldg(a.t.row_start + s + min(at, len - 1)) <= row);
+            const int k = m ? 31 - __clz(m) : 0;
+            s += k * step;
+            len = min(step, len - k * step);
         }
-        const int n = min(32, shares - c0);
-        using V = typename std::conditional<DPL == 4, float4, float2>::type;
-        V y[4];
-        auto fetch = [&](int c) {
+        TreeSeq q;
+        const bool mine = h < a.n_q && tree_seq(a.t, &a.m, s, &q, nullptr) && row >= q.r0 && row < q.r0 + q.n;
+        if (!per) pdl_grid_wait();                   // (what comes before does not depend on the kernel before; every warp waits, so that this kernel ends behind that one)
+        per = __ldcg(part.plan);
+        const int first_of_seq = __ldcg(part.plan + 1 + s);
+        if (per == kNoCut) return;
+        if (!mine) continue;
+        const int shares = pieces_of(tree_work(q.prefix, q.n, a.window).n_tiles, per);
+        if (shares == 1) continue;                       // finished by its CTA
+        const int f = (row - q.r0) * G + h % G, R = part.tile_rows, first = first_of_seq + (h / G * ((q.n * G + R - 1) / R) + f / R) * shares, r = f % R;
+        const float sink = a.sinks ? a.sinks[h] * kLog2e : -INFINITY;
+        float top = sink, sum = a.sinks ? 1.0f : 0.0f, o[DPL];
 #pragma unroll
-            for (int u = 0; u < 4; u++)
-                if (c + u < n) y[u] = __ldcg((const V*)(part.o + share_at(part, first + c0 + c + u, r) * HD) + lane);
-        };
-        fetch(0);
-        float t = fmaxf(top, m);
+        for (int i = 0; i < DPL; i++) o[i] = 0.0f;
+        // 32 shares at a time: a lane has the factor of one, all have their dimensions of each, four on their way
+        for (int c0 = 0; c0 < shares; c0 += 32) {
+            float m = -INFINITY, l = 0.0f;
+            if (c0 + lane < shares) {
+                const float2 v = __ldcg((const float2*)part.ml + share_at(part, first + c0 + lane, r));
+                m = v.x; l = v.y;
+            }
+            const int n = min(32, shares - c0);
+            using V = typename std::conditional<DPL == 4, float4, float2>::type;
+            V y[4];
+            auto fetch = [&](int c) {
 #pragma unroll
-        for (int i = 16; i > 0; i >>= 1) t = fmaxf(t, __shfl_xor_sync(0xffffffffu, t, i));
-        const float before = top == t ? 1.0f : exp2f(top - t);
-        // negative: a share without a key that this row sees; undefined sums stay undefined
-        const float factor = m == -INFINITY && l == 0.0f ? -1.0f : m == t || l != l ? 1.0f : exp2f(m - t);
-        sum = sum * before + warp_sum(factor >= 0.0f ? l * factor : 0.0f);
-        top = t;
+                for (int u = 0; u < 4; u++)
+                    if (c + u < n) y[u] = __ldcg((const V*)(part.o + share_at(part, first + c0 + c + u, r) * HD) + lane);
+            };
+            fetch(0);
+            float t = fmaxf(top, m);
 #pragma unroll
-        for (int i = 0; i < DPL; i++) o[i] *= before;
-        for (int c = 0; c < n; c += 4) {
-            if (c) fetch(c);
+            for (int i = 16; i > 0; i >>= 1) t = fmaxf(t, __shfl_xor_sync(0xffffffffu, t, i));
+            const float before = top == t ? 1.0f : exp2f(top - t);
+            // negative: a share without a key that this row sees; undefined sums stay undefined
+            const float factor = m == -INFINITY && l == 0.0f ? -1.0f : m == t || l != l ? 1.0f : exp2f(m - t);
+            sum = sum * before + warp_sum(factor >= 0.0f ? l * factor : 0.0f);
+            top = t;
 #pragma unroll
-            for (int u = 0; u < 4; u++) {
-                const float g = __shfl_sync(0xffffffffu, factor, min(c + u, 31));
-                if (c + u < n && g >= 0.0f) {
-                    const float* z = (const float*)&y[u];
+            for (int i = 0; i < DPL; i++) o[i] *= before;
+            for (int c = 0; c < n; c += 4) {
+                if (c) fetch(c);
 #pragma unroll
-                    for (int i = 0; i < DPL; i++) o[i] = fmaf(z[i], g, o[i]);
+                for (int u = 0; u < 4; u++) {
+                    const float g = __shfl_sync(0xffffffffu, factor, min(c + u, 31));
+                    if (c + u < n && g >= 0.0f) {
+                        const float* z = (const float*)&y[u];
+#pragma unroll
+                        for (int i = 0; i < DPL; i++) o[i] = fmaf(z[i], g, o[i]);
+                    }
                 }
             }
         }
-    }
-    const float inv = sum > 0.0f ? 1.0f / sum : sum;
-    TQ* dst = (TQ*)a.out + (size_t)row * a.out_stride + (size_t)h * HD + lane * DPL;
+        const float inv = sum > 0.0f ? 1.0f / sum : sum;
+        TQ* dst = (TQ*)a.out + (size_t)row * a.out_stride + (size_t)h * HD + lane * DPL;
 #pragma unroll
-    for (int i = 0; i < DPL; i++) dst[i] = out_of<TQ>(o[i] * inv);
+        for (int i = 0; i < DPL; i++) dst[i] = out_of<TQ>(o[i] * inv);
+    }
 }
 
 // Copies of the query rows in a tile of 128 (see attn_tree_tc): as many as there is room for.  Measured with / without, us: 32 trees of 16 nodes of 4 query heads (2 copies) 53 / 65
@@ -1054,6 +1066,7 @@ Share share_of(const TreeAttnArgs& a, int sm_count) {
     p.rows = std::min(p.tile_rows, a.t.max_rows * G);
     p.slots = sm_count * (a.kv_bf16 && !a.q_bf16 && a.hd == 128 ? 1 : 2);
     const Bounds b = bounds_of(a, p.tile_rows);
+    p.sms = sm_count;
     p.cluster = a.kv_bf16 ? cluster_of(b, sm_count) : 1;
     p.row_tiles = (a.t.max_rows * G + p.tile_rows - 1) / p.tile_rows;
     if (p.cluster > 1) { p.grid = (int)b.units * p.cluster; return p; }
@@ -1073,7 +1086,7 @@ template <int HD, typename TQ>
 cudaError_t combine(const TreeAttnArgs& a, const Share& p, cudaStream_t st) {
     if (!p.shares) return cudaSuccess;               // nothing is cut
     cudaLaunchConfig_t cfg = {};
-    cfg.gridDim = dim3((unsigned)(a.t.n_rows * ((a.n_q + 7) / 8)));
+    cfg.gridDim = dim3((unsigned)std::min<long long>((long long)a.t.n_rows * ((a.n_q + 7) / 8), 2ll * p.sms * kJoinCtas));
     cfg.blockDim = dim3(256);
     cfg.stream = st;
     cudaLaunchAttribute at[1];
