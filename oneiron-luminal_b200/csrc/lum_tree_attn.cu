@@ -6,6 +6,7 @@
 #include <cuda.h>
 #include <algorithm>
 #include <type_traits>
+#include <utility>
 
 #include "lum_tree.cuh"
 
@@ -180,6 +181,59 @@ __device__ __forceinline__ float tree_inverse(const TreeAttnArgs& a, int h, floa
     return sum > 0.0f ? c / sum : sum;
 }
 
+__device__ __forceinline__ float2 cluster_ld2(uint32_t at) { float2 v; asm volatile("ld.shared::cluster.v2.f32 {%0, %1}, [%2];" : "=f"(v.x), "=f"(v.y) : "r"(at) : "memory"); return v; }
+__device__ __forceinline__ float4 cluster_ld4(uint32_t at) {
+    float4 v;
+    asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];" : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w) : "r"(at) : "memory");
+    return v;
+}
+// The unit's rows are shared out among the warps of the cluster, which join the CTAs' shares of them: o_at(r) and ml_at(r) are where a CTA has its outputs and (maximum, sum).
+template <int HD, typename TQ, typename At, typename MlAt>
+__device__ __forceinline__ void join_cluster(const TreeAttnArgs& a, const Share& p, const Piece& x, int live_rows, int warp, int warps, int lane, At o_at, MlAt ml_at) {
+    using V = typename std::conditional<HD == 128, float4, float2>::type;
+    const int C = p.cluster, rank = (int)blockIdx.x % C, G = a.n_q / a.n_kv;
+    __syncwarp();
+    cluster_arrive_release();
+    cluster_wait_acquire();
+    for (int r = rank + C * warp; r < live_rows; r += C * warps) {
+        const int node = (x.f0 + r) / G, h = x.kvh * G + (x.f0 + r) - node * G;
+        float2 ml[kClusterMax];
+        V y[kClusterMax];
+#pragma unroll
+        for (int c = 0; c < kClusterMax; c++) {                      // all on their way at once
+            ml[c] = make_float2(-INFINITY, 0.0f);
+            if (c < C) {
+                ml[c] = cluster_ld2(cluster_map(ml_at(r), (uint32_t)c));
+                const uint32_t from = cluster_map(o_at(r) + (uint32_t)(lane * (HD / 32)) * 4u, (uint32_t)c);
+                if constexpr (HD == 128) y[c] = cluster_ld4(from); else y[c] = cluster_ld2(from);
+            }
+        }
+        const float sink = a.sinks ? a.sinks[h] * kLog2e : -INFINITY;
+        float top = sink, z[HD / 32];
+#pragma unroll
+        for (int c = 0; c < kClusterMax; c++) top = fmaxf(top, ml[c].x);
+        float sum = !a.sinks ? 0.0f : sink == top ? 1.0f : exp2f(sink - top);
+#pragma unroll
+        for (int i = 0; i < HD / 32; i++) z[i] = 0.0f;
+#pragma unroll
+        for (int c = 0; c < kClusterMax; c++) {
+            if (ml[c].x == -INFINITY && ml[c].y == 0.0f) continue;   // no key that this row sees
+            const float f = ml[c].x == top || ml[c].y != ml[c].y ? 1.0f : exp2f(ml[c].x - top);      // (undefined sums stay undefined)
+            const float* part_of = (const float*)&y[c];
+            sum = fmaf(ml[c].y, f, sum);
+#pragma unroll
+            for (int i = 0; i < HD / 32; i++) z[i] = fmaf(part_of[i], f, z[i]);
+        }
+        const float inv = sum > 0.0f ? 1.0f / sum : sum;
+        TQ* dst = (TQ*)a.out + (size_t)(x.q.r0 + node) * a.out_stride + (size_t)h * HD + lane * (HD / 32);
+#pragma unroll
+        for (int i = 0; i < HD / 32; i++) dst[i] = out_of<TQ>(z[i] * inv);
+    }
+    __syncwarp();
+    cluster_arrive_release();                        // nobody leaves while another may read its shares
+    cluster_wait_acquire();
+}
+
 // Pairs of floats in 64-bit registers, whose operations issue once for two.
 using F2 = unsigned long long;
 __device__ __forceinline__ F2 pack2(float a, float b) { F2 r; asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(a), "f"(b)); return r; }
@@ -208,10 +262,12 @@ __global__ void __launch_bounds__(256, 2) attn_tree_rows(const TreeAttnArgs a, c
     TreeNodes& tree = *(TreeNodes*)(s_piece + 1);
     constexpr int DPL = HD / 32, PPL = DPL / 2;
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, G = a.n_q / a.n_kv;
-    if (warp == 0) piece_find(a, part, lane, s_piece);
+    if (part.cluster > 1) { if (tid == 0) piece_of_cluster(a, part, s_piece); }
+    else if (warp == 0) piece_find(a, part, lane, s_piece);
     __syncthreads();
     if (s_piece->s < 0) return;
     const Piece x = *s_piece;
+    const bool clustered = part.cluster > 1;
     const float scale = a.scale * kLog2e;
     {
         const TreeSeq& q = x.q;
@@ -343,16 +399,18 @@ __global__ void __launch_bounds__(256, 2) attn_tree_rows(const TreeAttnArgs a, c
         for (int r = 0; r < 4; r++)
 #pragma unroll
             for (int i = 0; i < PPL; i++) { const float2 t = unpack2(o[r][i]); out[r][2 * i] = t.x; out[r][2 * i + 1] = t.y; }
+        if (clustered) __syncthreads();              // (a CTA without a tile: the queries are there, which a share takes the place of)
 #pragma unroll
         for (int r = 0; r < 4; r++) {
             if (node[r] < 0) continue;
             const int row = q.r0 + node[r], h = x.kvh * G + (x.f0 + warp * 4 + r) % G;
             const float sum = warp_sum(l[r]);
-            if (x.share >= 0) {
-                const size_t at = share_at(part, x.share, warp * 4 + r);
+            if (clustered || x.share >= 0) {
+                const size_t at = share_at(part, max(x.share, 0), warp * 4 + r);
+                float *o_to = clustered ? s_q + (warp * 4 + r) * HD : part.o + at * HD, *ml_to = clustered ? s_p + (warp * kRowsKeys * 4 + r) * 2 : part.ml + 2 * at;      // (this warp's own)
 #pragma unroll
-                for (int i = 0; i < DPL; i++) part.o[at * HD + lane * DPL + i] = out[r][i];
-                if (lane == 0) { part.ml[2 * at] = mx[r]; part.ml[2 * at + 1] = sum; }
+                for (int i = 0; i < DPL; i++) o_to[lane * DPL + i] = out[r][i];
+                if (lane == 0) { ml_to[0] = mx[r]; ml_to[1] = sum; }
             } else {
                 const float inv = tree_inverse(a, h, mx[r], sum);
                 float* dst = (float*)a.out + (size_t)row * a.out_stride + (size_t)h * HD + lane * DPL;
@@ -360,6 +418,9 @@ __global__ void __launch_bounds__(256, 2) attn_tree_rows(const TreeAttnArgs a, c
                 for (int i = 0; i < DPL; i++) dst[i] = out[r][i] * inv;
             }
         }
+        if (clustered)
+            join_cluster<HD, float>(a, part, x, min(kRowsTile, q.n * G - x.f0), warp, 8, lane, [&](int r) { return smem_u32(s_q + r * HD); },
+                                    [&](int r) { return smem_u32(s_p + ((r >> 2) * kRowsKeys * 4 + (r & 3)) * 2); });
     }
 }
 
@@ -447,12 +508,6 @@ __device__ __forceinline__ uint32_t tc_term(float* x0, float* x1) {
     const float2 r = unpack2(x);
     *x0 = r.x; *x1 = r.y;
     return b;
-}
-__device__ __forceinline__ float2 cluster_ld2(uint32_t at) { float2 v; asm volatile("ld.shared::cluster.v2.f32 {%0, %1}, [%2];" : "=f"(v.x), "=f"(v.y) : "r"(at) : "memory"); return v; }
-__device__ __forceinline__ float4 cluster_ld4(uint32_t at) {
-    float4 v;
-    asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];" : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w) : "r"(at) : "memory");
-    return v;
 }
 __device__ __forceinline__ void tma_box(uint32_t dst, const CUtensorMap* map, int row, int col, uint32_t bar) {
     asm volatile("cp.async.bulk.tensor.3d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4}], [%5];" ::"r"(dst), "l"(map), "r"(0), "r"(row), "r"(col), "r"(bar) : "memory");
@@ -904,51 +959,8 @@ __global__ void __launch_bounds__(kTcThreads, TcShape<HD, F32>::ctas) attn_tree_
         }
         tc_fence_before_sync();
     }
-    if (clustered) {                                 // ---- the unit's rows are shared out among the cluster's warps, which join the CTAs' shares of them
-        __syncwarp();
-        cluster_arrive_release();
-        cluster_wait_acquire();
-        const int C = part.cluster, rank = (int)blockIdx.x % C;
-        const uint32_t o_at = smem_u32(c_o), ml_at = smem_u32(c_ml);
-        using V = typename std::conditional<HD == 128, float4, float2>::type;
-        for (int r = rank + C * warp; r < live_rows; r += C * (kTcThreads / 32)) {
-            const int node = (f0 + r) / G, h = kvh * G + (f0 + r) - node * G;
-            float2 ml[kClusterMax];
-            V y[kClusterMax];
-#pragma unroll
-            for (int c = 0; c < kClusterMax; c++) {                  // all on their way at once
-                ml[c] = make_float2(-INFINITY, 0.0f);
-                if (c < C) {
-                    ml[c] = cluster_ld2(cluster_map(ml_at + (uint32_t)r * 8u, (uint32_t)c));
-                    const uint32_t from = cluster_map(o_at + (uint32_t)(r * kLd + lane * (HD / 32)) * 4u, (uint32_t)c);
-                    if constexpr (HD == 128) y[c] = cluster_ld4(from); else y[c] = cluster_ld2(from);
-                }
-            }
-            const float sink = a.sinks ? a.sinks[h] * kLog2e : -INFINITY;
-            float top = sink, z[HD / 32];
-#pragma unroll
-            for (int c = 0; c < kClusterMax; c++) top = fmaxf(top, ml[c].x);
-            float sum = !a.sinks ? 0.0f : sink == top ? 1.0f : exp2f(sink - top);
-#pragma unroll
-            for (int i = 0; i < HD / 32; i++) z[i] = 0.0f;
-#pragma unroll
-            for (int c = 0; c < kClusterMax; c++) {
-                if (ml[c].x == -INFINITY && ml[c].y == 0.0f) continue;         // no key that this row sees
-                const float f = ml[c].x == top || ml[c].y != ml[c].y ? 1.0f : exp2f(ml[c].x - top);      // (undefined sums stay undefined)
-                const float* part_of = (const float*)&y[c];
-                sum = fmaf(ml[c].y, f, sum);
-#pragma unroll
-                for (int i = 0; i < HD / 32; i++) z[i] = fmaf(part_of[i], f, z[i]);
-            }
-            const float inv = sum > 0.0f ? 1.0f / sum : sum;
-            TQ* dst = (TQ*)a.out + (size_t)(q.r0 + node) * a.out_stride + (size_t)h * HD + lane * (HD / 32);
-#pragma unroll
-            for (int i = 0; i < HD / 32; i++) dst[i] = out_of<TQ>(z[i] * inv);
-        }
-        __syncwarp();
-        cluster_arrive_release();                    // nobody leaves while another may read its shares
-        cluster_wait_acquire();
-    }
+    if (clustered)
+        join_cluster<HD, TQ>(a, part, x, live_rows, warp, kTcThreads / 32, lane, [&](int r) { return smem_u32(c_o + r * kLd); }, [&](int r) { return smem_u32(c_ml + 2 * r); });
     __syncthreads();
     if (warp == 5) tmem_dealloc(tmem, S::cols);
     if (tid == 0 && *gave_up) atomicOr(a.status, LUM_ST_WAIT_TMEM);
@@ -1052,11 +1064,12 @@ Bounds bounds_of(const TreeAttnArgs& a, int tile_rows) {
 // Few units of not too many tiles: a cluster for each, whose CTAs share its tiles evenly and join their shares through distributed shared memory.  One launch, no scratch, and
 // no search for pieces.  Measured against pieces and tree_combine (or, below 9 tiles, whole units), us in a graph, 8 K/V heads of 4 query heads of 128 in bf16, trees of 8:
 // 1 x 4 tiles 10.1 / 10.6 (of 32 nodes 13.7 / 12.6: more rows to join), 1 x 8 9.9 / 13.0, 1 x 63 13.7 / 17.5, 4 x 63 19.9 / 24.6, 1 x 251 27.6 / 34.7, 2 x 251 41.9 / 40.7, 1 x 501
-// 55.0 / 45.1 (8 CTAs a unit are too few).  Clusters of 16 gain 1 us at most and lose up to 10 where an SM holds one CTA.
-int cluster_of(const Bounds& b, int sm_count) {
+// 55.0 / 45.1 (8 CTAs a unit are too few).  From an f32 cache, whose tiles take CUDA cores 7 us, only one tile a CTA: 1 x 4 17.8 / 18.9, 1 x 8 19.1 / 20.5,
+// but 1 x 16 in 8 CTAs 26.0 / 22.0.  Clusters of 16 gain 1 us at most and lose up to 10 where an SM holds one CTA.
+int cluster_of(const Bounds& b, int sm_count, bool tc) {
     int C = 1;
     while (C < kClusterMax && 2 * C * b.units <= sm_count && 2 * C <= b.tiles) C *= 2;
-    return b.tiles > 4 && b.tiles <= (long long)C * 32 ? C : 1;
+    return b.tiles > (tc ? 4 : 1) && b.tiles <= (long long)C * (tc ? 32 : 1) ? C : 1;
 }
 Share share_of(const TreeAttnArgs& a, int sm_count) {
     Share p{};
@@ -1067,12 +1080,12 @@ Share share_of(const TreeAttnArgs& a, int sm_count) {
     p.slots = sm_count * (a.kv_bf16 && !a.q_bf16 && a.hd == 128 ? 1 : 2);
     const Bounds b = bounds_of(a, p.tile_rows);
     p.sms = sm_count;
-    p.cluster = a.kv_bf16 ? cluster_of(b, sm_count) : 1;
+    p.cluster = cluster_of(b, sm_count, a.kv_bf16);
     p.row_tiles = (a.t.max_rows * G + p.tile_rows - 1) / p.tile_rows;
     if (p.cluster > 1) { p.grid = (int)b.units * p.cluster; return p; }
     // Few tiles: nothing is cut, and tree_combine (2 to 3 us, and as much of the caller's time) need not run.  Measured, us, whole / cut: 16 trees of 8 nodes over 508 rows in
-    // bf16 (8 tiles, 128 units) 14.4 / 16.8, 64 of them 39.6 / 44.6; an f32 cache takes four times as long a tile on CUDA cores, and is cut sooner.
-    if (b.tiles <= (a.kv_bf16 ? 8 : 4)) { p.grid = (int)b.units; return p; }
+    // bf16 (8 tiles, 128 units) 14.4 / 16.8, 64 of them 39.6 / 44.6; over f32 caches of 208 rows (4 tiles) 8 trees (64 units) 37.9 / 25.2, 16 37.7 / 39.3, 32 57.0 / 60.5.
+    if (b.tiles <= (a.kv_bf16 ? 8 : 2 * b.units >= sm_count ? 4 : 1)) { p.grid = (int)b.units; return p; }
     // Pieces, as piece_find cuts them: at most `slots` where there are fewer units, else at most units + tiles / (2 tiles / slots).  Shares: the pieces of units that are cut, at
     // most `slots` in both cases.
     p.grid = (int)std::min(b.units * b.tiles, b.units < p.slots ? (long long)p.slots : b.units + p.slots / 2);
@@ -1128,12 +1141,25 @@ cudaError_t map_queries(CUtensorMap* map, const TreeAttnArgs& a, int tile_rows) 
     const cuuint32_t box[4] = {64, (cuuint32_t)G, (cuuint32_t)(tile_rows / G), 1};
     return encode_bf16(map, a.q, 4, dims, strides, box);
 }
+template <typename... Params, typename... Args>
+cudaError_t launch_pieces(const Share& p, int threads, int smem, cudaStream_t st, void (*kernel)(Params...), Args&&... args) {
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3((unsigned)p.grid);
+    cfg.blockDim = dim3((unsigned)threads);
+    cfg.dynamicSmemBytes = (size_t)smem;
+    cfg.stream = st;
+    cudaLaunchAttribute at[1];
+    at[0].id = cudaLaunchAttributeClusterDimension;
+    at[0].val.clusterDim.x = (unsigned)p.cluster; at[0].val.clusterDim.y = 1; at[0].val.clusterDim.z = 1;
+    cfg.attrs = at;
+    cfg.numAttrs = p.cluster > 1 ? 1 : 0;
+    return cudaLaunchKernelEx(&cfg, kernel, std::forward<Args>(args)...);
+}
 template <int HD>
 cudaError_t rows_launch(const TreeAttnArgs& a, const Share& p, cudaStream_t st) {
     static std::atomic<uint64_t> raised{0};
     if (const cudaError_t e = allow_smem(raised, (const void*)attn_tree_rows<HD>, rows_smem<HD>())) return e;
-    attn_tree_rows<HD><<<p.grid, 256, rows_smem<HD>(), st>>>(a, p);
-    const cudaError_t e = cudaGetLastError();
+    const cudaError_t e = launch_pieces(p, 256, rows_smem<HD>(), st, attn_tree_rows<HD>, a, p);
     return e != cudaSuccess ? e : combine<HD, float>(a, p, st);
 }
 template <int HD, bool F32, int DUP>
@@ -1146,17 +1172,7 @@ cudaError_t tc_launch_copies(const TreeAttnArgs& a, const Share& p, cudaStream_t
     if constexpr (!F32) if (const cudaError_t e = map_queries(&map_q, a, p.tile_rows)) return e;
     if (const cudaError_t e = map_cache(&map_k, a, a.k, box_rows)) return e;
     if (const cudaError_t e = map_cache(&map_v, a, a.v, box_rows)) return e;
-    cudaLaunchConfig_t cfg = {};
-    cfg.gridDim = dim3((unsigned)p.grid);
-    cfg.blockDim = dim3(kTcThreads);
-    cfg.dynamicSmemBytes = S::smem;
-    cfg.stream = st;
-    cudaLaunchAttribute at[1];
-    at[0].id = cudaLaunchAttributeClusterDimension;
-    at[0].val.clusterDim.x = (unsigned)p.cluster; at[0].val.clusterDim.y = 1; at[0].val.clusterDim.z = 1;
-    cfg.attrs = at;
-    cfg.numAttrs = p.cluster > 1 ? 1 : 0;
-    const cudaError_t e = cudaLaunchKernelEx(&cfg, attn_tree_tc<HD, F32, DUP>, a, p, map_q, map_k, map_v, box_rows);
+    const cudaError_t e = launch_pieces(p, kTcThreads, S::smem, st, attn_tree_tc<HD, F32, DUP>, a, p, map_q, map_k, map_v, box_rows);
     return e != cudaSuccess ? e : combine<HD, typename std::conditional<F32, float, __nv_bfloat16>::type>(a, p, st);
 }
 template <int HD, bool F32>
