@@ -237,7 +237,6 @@ __device__ __forceinline__ void join_cluster(const TreeAttnArgs& a, const Share&
 // Pairs of floats in 64-bit registers, whose operations issue once for two.
 using F2 = unsigned long long;
 __device__ __forceinline__ F2 pack2(float a, float b) { F2 r; asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(a), "f"(b)); return r; }
-__device__ __forceinline__ F2 pack2(uint32_t a, uint32_t b) { F2 r; asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "r"(a), "r"(b)); return r; }
 __device__ __forceinline__ float2 unpack2(F2 x) { float2 r; asm("mov.b64 {%0, %1}, %2;" : "=f"(r.x), "=f"(r.y) : "l"(x)); return r; }
 __device__ __forceinline__ F2 fma2(F2 a, F2 b, F2 c) { F2 r; asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c)); return r; }
 __device__ __forceinline__ F2 mul2(F2 a, F2 b) { F2 r; asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b)); return r; }
@@ -444,7 +443,7 @@ __global__ void __launch_bounds__(256, 2) attn_tree_rows(const TreeAttnArgs a, c
 // result is not finite is computed again by tree_row_plain, key by key.
 // What bounds it, and what it measured (in a graph, SM clock 1.9 GHz): 16 trees of 32 nodes over up to 32768 rows in pages of 16, 8 K/V heads of 4 query heads of 128 (1.28 GB):
 // 268 us, 4.8 TB/s; with more products per byte than HBM alone would let them wait for, it slows down with the SMs' clock (328 us at the 1.4 GHz that a second of such calls is
-// held to).  8 trees of 64 over 4096 rows, 8 query heads of 64 per K/V head (34.6 GFLOP): 84 us, 410 TFLOP/s; bound by the softmax warps (ALU and exponentials busy half of the
+// held to).  8 trees of 64 over 4096 rows, 8 query heads of 64 per K/V head (34.6 GFLOP): 82 us, 420 TFLOP/s; bound by the softmax warps (ALU and exponentials busy half of the
 // time each, issue 46 %).  32 trees of up to 16 over up to 2048 rows (0.18 GB): 49 us, 3.7 TB/s, of which launch, first tiles and joining are 15.  Tried without gain: two
 // threads per query row (104 us to 107 where this came to 104), weights by the maximum of the tile before with a second try where it grew (112), room for four tiles
 // (n_seq 1 .. 8 with 4000 .. 16000 rows: 13.9 / 14.1, 27.8 / 29.7, 36.4 / 32.2, 25.1 / 37.0: with that much shared memory clusters no longer fit beside one another).
@@ -494,19 +493,18 @@ __device__ __forceinline__ void tc_st_wait() { asm volatile("tcgen05.wait::st.sy
 // (passes over NaN as fmaxf does)
 __device__ __forceinline__ float max3(float a, float b, float c) { float r; asm("max.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c)); return r; }
 __device__ __forceinline__ float tc_ex2(float x) { float y; asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x)); return y; }
-// x as packed bf16, rounded; what is left of it goes back
-__device__ __forceinline__ uint32_t tc_term(F2* x, F2 minus_one) {
-    const float2 y = unpack2(*x);
-    const __nv_bfloat162 h = __floats2bfloat162_rn(y.x, y.y);
+// x as packed bf16, rounded; what is left of it goes back, by additions that take a bf16 operand as it is (8 trees of 64 nodes over 4096 rows 81.8 us; with the terms made f32
+// again 84.3)
+__device__ __forceinline__ uint32_t tc_term(float* x0, float* x1) {
+    const __nv_bfloat162 h = __floats2bfloat162_rn(*x0, *x1);
     const uint32_t b = *(const uint32_t*)&h;
-    *x = fma2(pack2(b << 16, b & 0xffff0000u), minus_one, *x);
+    asm("{\n\t.reg .b16 lo, hi, m;\n\tmov.b32 {lo, hi}, %2;\n\tmov.b16 m, 0xBF80;\n\tfma.rn.f32.bf16 %0, lo, m, %0;\n\tfma.rn.f32.bf16 %1, hi, m, %1;\n\t}" : "+f"(*x0), "+f"(*x1) : "r"(b));      // m: -1
     return b;
 }
-__device__ __forceinline__ uint32_t tc_term(float* x0, float* x1) {
-    F2 x = pack2(*x0, *x1);
-    const uint32_t b = tc_term(&x, pack2(-1.0f, -1.0f));
-    const float2 r = unpack2(x);
-    *x0 = r.x; *x1 = r.y;
+__device__ __forceinline__ uint32_t tc_term(F2* x) {
+    float2 y = unpack2(*x);
+    const uint32_t b = tc_term(&y.x, &y.y);
+    *x = pack2(y.x, y.y);
     return b;
 }
 __device__ __forceinline__ void tma_box(uint32_t dst, const CUtensorMap* map, int row, int col, uint32_t bar) {
@@ -780,7 +778,7 @@ __global__ void __launch_bounds__(kTcThreads, TcShape<HD, F32>::ctas) attn_tree_
                 // them), zeros where the keys are another row's
                 constexpr int kStep = 16, kCols = kStep / 2;
                 F2 w2[2][kCols], sum[2] = {0ull, 0ull};
-                const F2 scale2 = pack2(scale, scale), off2 = pack2(off, off), minus_one = pack2(-1.0f, -1.0f);
+                const F2 scale2 = pack2(scale, scale), off2 = pack2(off, off);
 #pragma unroll
                 for (int c = 0; c <= KPT / kStep; c++) {
                     if (c < KPT / kStep) {
@@ -797,7 +795,7 @@ __global__ void __launch_bounds__(kTcThreads, TcShape<HD, F32>::ctas) attn_tree_
                         for (int e = 0; e < S::p_terms; e++) {
                             uint32_t pk[kCols];
 #pragma unroll
-                            for (int i = 0; i < kCols; i++) pk[i] = tc_term(&w2[(c - 1) & 1][i], minus_one);
+                            for (int i = 0; i < kCols; i++) pk[i] = tc_term(&w2[(c - 1) & 1][i]);
                             const uint32_t to = (e == 2 ? mine + S::col_x + (uint32_t)b * 32u : sc + e * 32u) + (c - 1) * kCols;
 #pragma unroll
                             for (int d = 0; d < DUP; d++) {
