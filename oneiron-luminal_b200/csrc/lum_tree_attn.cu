@@ -1064,10 +1064,14 @@ Bounds bounds_of(const TreeAttnArgs& a, int tile_rows) {
 // 1 x 4 tiles 10.1 / 10.6 (of 32 nodes 13.7 / 12.6: more rows to join), 1 x 8 9.9 / 13.0, 1 x 63 13.7 / 17.5, 4 x 63 19.9 / 24.6, 1 x 251 27.6 / 34.7, 2 x 251 41.9 / 40.7, 1 x 501
 // 55.0 / 45.1 (8 CTAs a unit are too few).  From an f32 cache, whose tiles take CUDA cores 7 us, only one tile a CTA: 1 x 4 17.8 / 18.9, 1 x 8 19.1 / 20.5,
 // but 1 x 16 in 8 CTAs 26.0 / 22.0.  Clusters of 16 gain 1 us at most and lose up to 10 where an SM holds one CTA.
-int cluster_of(const Bounds& b, int sm_count, bool tc) {
+// A second CTA on an SM pays from six tiles each on: 16 x 16 tiles (8 a CTA) 19.4 in 256 CTAs / 23.5, but 4 x 8 (1 a CTA) 12.3 / 11.1.  Where lengths differ, pieces find the long
+// sequence more CTAs (one of 63 tiles and 7 of 2: 16.8, in 4 CTAs a unit 19.7, in 2 28.4; with 15 of 2 18.4, in 2 29.1), so batches get fewer
+// tiles a CTA: one of 63 and 3 of 2 (8 CTAs a unit) 14.8 / 16.6.
+int cluster_of(const TreeAttnArgs& a, const Bounds& b, int sm_count, int slots) {
     int C = 1;
-    while (C < kClusterMax && 2 * C * b.units <= sm_count && 2 * C <= b.tiles) C *= 2;
-    return b.tiles > (tc ? 4 : 1) && b.tiles <= (long long)C * (tc ? 32 : 1) ? C : 1;
+    while (C < kClusterMax && 2 * C <= b.tiles && (2 * C * b.units <= sm_count || (2 * C * b.units <= slots && 12 * C <= b.tiles))) C *= 2;
+    const int most = !a.kv_bf16 ? 1 : a.t.n_seq == 1 ? 32 : 8 + C;             // tiles of a CTA
+    return b.tiles > (a.kv_bf16 ? 4 : 1) && b.tiles <= (long long)C * most ? C : 1;
 }
 Share share_of(const TreeAttnArgs& a, int sm_count) {
     Share p{};
@@ -1078,7 +1082,7 @@ Share share_of(const TreeAttnArgs& a, int sm_count) {
     p.slots = sm_count * (a.kv_bf16 && !a.q_bf16 && a.hd == 128 ? 1 : 2);
     const Bounds b = bounds_of(a, p.tile_rows);
     p.sms = sm_count;
-    p.cluster = cluster_of(b, sm_count, a.kv_bf16);
+    p.cluster = cluster_of(a, b, sm_count, p.slots);
     p.row_tiles = (a.t.max_rows * G + p.tile_rows - 1) / p.tile_rows;
     if (p.cluster > 1) { p.grid = (int)b.units * p.cluster; return p; }
     // Few tiles: nothing is cut, and tree_combine (2 to 3 us, and as much of the caller's time) need not run.  Measured, us, whole / cut: 16 trees of 8 nodes over 508 rows in
