@@ -295,6 +295,7 @@ __global__ void __launch_bounds__(256, 2) attn_tree_rows(const TreeAttnArgs a, c
             __syncthreads();                         // (the tree and the queries are there; the tile before has been read)
             constexpr int kStep = 256 / (HD / 4), kBatch = 4;        // a thread has one column of every kStep-th row
             const int col = tid % (HD / 4) * 4;
+            float odd = 0.0f;                        // 0, or NaN where a value is not finite
 #pragma unroll 1
             for (int r0 = tid / (HD / 4); r0 < kRowsKeys; r0 += kStep * kBatch) {
                 float4 kf[kBatch], vf[kBatch];
@@ -313,9 +314,10 @@ __global__ void __launch_bounds__(256, 2) attn_tree_rows(const TreeAttnArgs a, c
                 for (int u = 0; u < kBatch; u++) {
                     *(float4*)(s_k + (r0 + u * kStep) * (HD + 4) + col) = kf[u];
                     *(float4*)(s_v + (r0 + u * kStep) * HD + col) = vf[u];
+                    odd = fmaf(vf[u].x, 0.0f, fmaf(vf[u].y, 0.0f, fmaf(vf[u].z, 0.0f, fmaf(vf[u].w, 0.0f, odd))));
                 }
             }
-            __syncthreads();
+            const bool finite = !__syncthreads_or(odd != 0.0f);
             F2 y[2][4];
 #pragma unroll
             for (int r = 0; r < 4; r++) y[0][r] = y[1][r] = 0ull;
@@ -365,7 +367,7 @@ __global__ void __launch_bounds__(256, 2) attn_tree_rows(const TreeAttnArgs a, c
             __syncwarp();
             using V = typename std::conditional<HD == 128, ulonglong2, F2>::type;
             const float *pw = s_p + warp * kRowsKeys * 8, *vl = s_v + lane * DPL;
-            if (all == 0xffffffffu) {
+            if (finite || all == 0xffffffffu) {      // (keys that a row does not see have weight 0)
 #pragma unroll 8
                 for (int key = 0; key < kRowsKeys; key++) {
                     const V v = *(const V*)(vl + key * HD);
@@ -377,7 +379,7 @@ __global__ void __launch_bounds__(256, 2) attn_tree_rows(const TreeAttnArgs a, c
                         for (int i = 0; i < PPL; i++) o[r][i] = fma2(p2[r], ((const F2*)&v)[i], o[r][i]);
                 }
             } else {
-                // a key that a row does not see adds nothing to it, whatever its value holds (0 times infinity is no zero)
+                // but 0 times infinity is no zero
 #pragma unroll 1
                 for (int key = 0; key < kRowsKeys; key++) {
                     const V v = *(const V*)(vl + key * HD);
