@@ -66,7 +66,8 @@ __device__ __forceinline__ bool tree_sees(const TreeNodes& s, const TreeSeq& q, 
 
 // How the work is shared out.  A unit is a (sequence, K/V head, tile of query rows); it may be cut into equal pieces of its tiles of keys, one CTA per piece.  How
 // long a piece may be is chosen on the device, where the lengths are.  A whole unit is finished by its CTA; a unit in pieces leaves a share (maximum, sum,
-// outputs) of each in the workspace, and tree_combine joins them.
+// outputs) of each in the workspace, and tree_combine joins them.  Or, where the call knows that units are few, every unit has a cluster of CTAs, which join their shares
+// themselves (cluster_of says when).
 constexpr int kNoCut = 1 << 30;                       // as the longest piece: longer than any unit
 struct Share {
     int* plan;                                       // [0] tiles of a piece at most, [1 + s] the first share of sequence s; written by CTA 0 for tree_combine
