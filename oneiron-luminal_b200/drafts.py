@@ -115,7 +115,8 @@ class KvMap:
 
 
 def _rows_of(name, t, device, width, rows):
-    """(address, row stride) of a tensor whose rows are ``width`` elements, dense in a row."""
+    """(address, row stride) of a tensor whose rows are ``width`` elements, dense in a row, one behind the other (a row stride of 0, of a tensor expanded along
+    its rows, would mean rows without gaps to the call, far more memory than the tensor has)."""
     shape = t.shape
     if t.device != device or len(shape) < 2 or shape[0] != rows:
         _bad(f"{name}: {rows} rows on {device} are wanted, got {tuple(shape)} on {t.device}")
@@ -128,6 +129,8 @@ def _rows_of(name, t, device, width, rows):
         inner *= size
     if inner != width:
         _bad(f"{name}: rows of {width} elements are wanted, got {tuple(t.shape[1:])}")
+    if rows > 1 and t.stride(0) < width:
+        _bad(f"{name}: rows {t.stride(0)} elements apart overlap, rows of {width} are wanted in a place each (an expanded tensor needs .contiguous())")
     return t.data_ptr(), (t.stride(0) if rows > 1 else width)
 
 
@@ -192,9 +195,10 @@ def tree_accept(tree: DraftTree, tokens, *, logits=None, picks=None, path_len: i
         _bad(f"tree_accept: {tokens.numel()} tokens for {rows} rows")
     l_at, vocab, ld = None, 0, 0
     if logits is not None:
-        if logits.dtype != torch.float32 or logits.dim() != 2 or logits.device != device or logits.shape[0] != rows or logits.stride(1) != 1:
-            _bad(f"tree_accept: logits must be [{rows}, vocab] f32 on {device}, dense in a row")
-        l_at, vocab, ld = logits.data_ptr(), logits.shape[1], (logits.stride(0) if rows > 1 else 0)
+        if logits.dtype != torch.float32 or logits.dim() != 2:
+            _bad(f"tree_accept: logits must be [{rows}, vocab] f32 on {device}, got {tuple(logits.shape)} {logits.dtype}")
+        vocab = logits.shape[1]
+        l_at, ld = _rows_of("logits", logits, device, vocab, rows)
     lib = load_library()
     with _Here(device.index):
         need = lib.lum_op_tree_accept_workspace(tree.ref, vocab) if logits is not None else 0

@@ -130,6 +130,27 @@ def test_python_calls_refuse_tensors_of_the_wrong_kind(pkg):
         d.kv_planes([])
 
 
+@pytest.mark.parametrize("rows, ok", [(1, True), (2, False), (7, False)])
+def test_rows_that_share_memory_are_refused(pkg, rows, ok):
+    """A row stride of 0 (or less than a row) must not reach a call, where 0 means rows without gaps."""
+    import torch
+    d = pkg.drafts
+    d._use_torch()
+    cpu = torch.device("cpu")
+    dense = torch.zeros(rows, 16)
+    assert d._rows_of("x", dense, cpu, 16, rows) == (dense.data_ptr(), 16)
+    padded = torch.zeros(rows, 24)[:, :16]
+    assert d._rows_of("x", padded, cpu, 16, rows) == (padded.data_ptr(), 24 if rows > 1 else 16)
+    room = torch.zeros(16 * rows + 16)
+    for t in (torch.zeros(1, 16).expand(rows, 16), torch.zeros(1, 2, 8).expand(rows, 2, 8), room.as_strided((rows, 16), (15, 1)), room.as_strided((rows, 2, 8), (8, 8, 1))):
+        if ok:
+            assert d._rows_of("x", t, cpu, 16, rows)[1] == 16
+        else:
+            with pytest.raises(pkg.LumError) as e:
+                d._rows_of("x", t, cpu, 16, rows)
+            assert e.value.code == -1
+
+
 # ---- the drafter and the loop
 
 

@@ -318,6 +318,26 @@ def test_attention_takes_the_rows_of_an_unknown_page_as_zeros(torch, ops, pkg, q
     assert (np.abs(got.double().cpu().numpy() - want[:5]) <= bound).all()
 
 
+def test_tensors_expanded_along_their_rows_are_refused(torch, ops, pkg):
+    """Their rows are all one: nothing is launched, out and what lies behind stay as they are."""
+    b = Batch(torch, ops, [4, 3], [30, 9], q="f32", cache="f32")
+    out = torch.full_like(b.q, 2.0)
+    one = lambda t: t[:1].clone().expand(t.shape)  # noqa: E731
+    call = lambda q=b.q, k=b.k, v=b.v, out=out: ops.attn_tree(q, k, v, b.tree, b.map, n_kv_heads=b.n_kv, head_dim=b.dim, out=out)  # noqa: E731
+    for kw in (dict(q=one(b.q)), dict(k=one(b.k)), dict(v=one(b.v)), dict(k=one(b.k), v=one(b.v)), dict(out=one(out)), dict(q=one(b.q).unflatten(1, (b.heads, b.dim)))):
+        with pytest.raises(pkg.LumError) as e:
+            call(**kw)
+        assert e.value.code == -1
+    tokens = torch.zeros(b.rows, dtype=torch.int32, device="cuda")
+    with pytest.raises(pkg.LumError) as e:
+        ops.tree_accept(b.tree, tokens, logits=torch.randn(1, 50, device="cuda").expand(b.rows, 50))
+    assert e.value.code == -1
+    torch.cuda.synchronize()
+    assert (out == 2.0).all()
+    b.check(call(k=b.k, v=b.v))
+    ops.status()
+
+
 # ---------------------------------------------------------------------------------------------------- accepted nodes
 
 
