@@ -381,7 +381,9 @@ int32_t lum_batch_get_logits(lum_rt* rt, int32_t seq, float* host_out, size_t n)
  * follow node 0 (counts[s] >= 1: the guesses that stand and the sample behind them) and which (tokens_out [n_seq][len], len at least the
  * nodes of the largest tree); the cache then holds positions[s] + counts[s] rows of the sequence (pages behind them have gone back), and the last
  * token is node 0 of the next step.  The selected sequence's single-token steps (lum_decode_greedy) go on from there.
+ * A pass takes lum_draft_capacity nodes in all, at least max_batch (the cache's rows per sequence, 4096 at most; 32 at least).
  * Needs what lum_batch_begin needs, with max_batch 1 too. */
+int32_t lum_draft_capacity(lum_rt* rt, int32_t* nodes);
 int32_t lum_draft_verify(lum_rt* rt, int32_t n_seq, const int32_t* slots, const int32_t* positions, const int32_t* row_start, const int32_t* tokens,
                          const int32_t* parents);
 int32_t lum_draft_get(lum_rt* rt, int32_t* counts, int32_t* tokens_out, size_t len);

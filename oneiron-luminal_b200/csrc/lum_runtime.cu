@@ -2777,10 +2777,24 @@ int32_t lum_batch_get_logits(lum_rt* rt, int32_t seq, float* host_out, size_t n)
 
 // ---- drafted trees -------------------------------------------------------------------------------------------------------
 
+// whether the loaded model can verify drafted trees
+static int draft_ready(lum_rt* rt, const char* who) {
+    if (rt->d.block_kind != 0 || !rows_supported(rt) || rt->d.tied_head || !rt->lm_head.kc || (rt->mega_ok && rt->use_mega))
+        return fail(rt, LUM_E_UNSUPPORTED, "%s needs packed Q8_0 weights with a Q8_0 vocabulary projection on one GPU, and an executor of one kernel per operation", who);
+    return 0;
+}
+int32_t lum_draft_capacity(lum_rt* rt, int32_t* nodes) {
+    if (!rt || !rt->has_model || !nodes) return fail(rt, LUM_E_INVALID, "draft_capacity: no model or null output");
+    if (int r = draft_ready(rt, "draft_capacity")) return r;
+    CU(rt, cudaSetDevice(rt->cfg.device));
+    if (int r = ensure_rows(rt, 1)) return r;
+    *nodes = rt->rows.cap;
+    return 0;
+}
+
 int32_t lum_draft_verify(lum_rt* rt, int32_t n_seq, const int32_t* slots, const int32_t* positions, const int32_t* row_start, const int32_t* tokens, const int32_t* parents) {
     if (!rt || !rt->has_model || !positions || !row_start || !tokens || !parents) return fail(rt, LUM_E_INVALID, "draft_verify: no model or null argument");
-    if (rt->d.block_kind != 0 || !rows_supported(rt) || rt->d.tied_head || !rt->lm_head.kc || (rt->mega_ok && rt->use_mega))
-        return fail(rt, LUM_E_UNSUPPORTED, "draft_verify needs packed Q8_0 weights with a Q8_0 vocabulary projection on one GPU, and an executor of one kernel per operation");
+    if (int r = draft_ready(rt, "draft_verify")) return r;
     if (n_seq < 1 || n_seq > rt->max_batch) return fail(rt, LUM_E_INVALID, "draft_verify: %d sequences, the model was loaded with max_batch %d", n_seq, rt->max_batch);
     if (row_start[0] != 0) return fail(rt, LUM_E_INVALID, "draft_verify: the first sequence's rows start at %d, not 0", row_start[0]);
     std::vector<char> taken((size_t)rt->max_batch, 0);

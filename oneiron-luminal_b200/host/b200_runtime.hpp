@@ -133,6 +133,7 @@ public:
     }
     // Speculative decoding: a tree of drafted tokens per sequence (node 0: the token that comes next at its position, parent -1) verified in one pass;
     // returns the tokens that follow node 0 of every sequence, at least one
+    int draft_capacity() { int32_t n = 0; ck(lum_draft_capacity(h_, &n)); return n; }      // nodes of all trees of a call
     struct DraftTree { std::vector<int32_t> tokens, parents; };
     std::vector<std::vector<int32_t>> draft_verify(const std::vector<DraftTree>& trees, const std::vector<int32_t>& positions, const std::vector<int32_t>& slots) {
         if (positions.size() != trees.size() || slots.size() != trees.size()) throw Error(LUM_E_INVALID, "draft_verify: one entry per tree in each list");

@@ -233,6 +233,7 @@ unsafe extern "C" {
     pub fn lum_batch_decode(rt: *mut lum_rt, n_steps: i32) -> i32;
     pub fn lum_batch_get_decoded(rt: *mut lum_rt, host_out: *mut i32, n_steps: usize) -> i32;
     pub fn lum_batch_get_logits(rt: *mut lum_rt, seq: i32, host_out: *mut f32, n: usize) -> i32;
+    pub fn lum_draft_capacity(rt: *mut lum_rt, nodes: *mut i32) -> i32;
     pub fn lum_draft_verify(rt: *mut lum_rt, n_seq: i32, slots: *const i32, positions: *const i32, row_start: *const i32, tokens: *const i32, parents: *const i32) -> i32;
     pub fn lum_draft_get(rt: *mut lum_rt, counts: *mut i32, tokens_out: *mut i32, len: usize) -> i32;
 

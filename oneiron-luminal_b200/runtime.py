@@ -299,6 +299,7 @@ def load_library() -> C.CDLL:
         "lum_batch_decode": (i32, [vp, i32]),
         "lum_batch_get_decoded": (i32, [vp, P(i32), sz]),
         "lum_batch_get_logits": (i32, [vp, i32, P(C.c_float), sz]),
+        "lum_draft_capacity": (i32, [vp, P(i32)]),
         "lum_draft_verify": (i32, [vp, i32, P(i32), P(i32), P(i32), P(i32), P(i32)]),
         "lum_draft_get": (i32, [vp, P(i32), P(i32), sz]),
         "lum_profile": (i32, [vp, i32, P(C.c_double), C.c_char_p, sz]),
@@ -813,6 +814,12 @@ class B200Runtime:
         out = np.empty(self.desc.vocab, dtype=np.float32)
         self._ck(self._lib.lum_batch_get_logits(self._h, seq, out.ctypes.data_as(C.POINTER(C.c_float)), out.size))
         return out
+
+    def draft_capacity(self) -> int:
+        """Nodes that one :meth:`draft_verify` takes, of all its trees: at least ``max_batch``."""
+        n = C.c_int32()
+        self._ck(self._lib.lum_draft_capacity(self._h, C.byref(n)))
+        return n.value
 
     def draft_verify(self, trees, positions: Sequence[int], slots: Optional[Sequence[int]] = None) -> List[List[int]]:
         """One pass of the model over a tree of drafted tokens per sequence: ``trees[s]`` = (tokens, parents), node 0 the token that comes next at

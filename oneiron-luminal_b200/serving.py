@@ -11,7 +11,8 @@ finished request's pages back.
 
 With a ``drafter`` the steps are speculative: every live sequence brings a tree of guesses of what follows its last token, one pass of
 the model verifies them all (``draft_verify``), and a sequence moves on by as many tokens as it guessed right, plus one — the tokens are
-those of plain decoding.  :class:`PromptLookup` is a drafter that needs no second model.
+those of plain decoding.  :class:`PromptLookup` is a drafter that needs no second model.  What one pass takes (``draft_capacity``, where the runtime
+has it) is shared out evenly among the sequences' guesses.
 
 Everything here is host-side bookkeeping over four calls of the runtime: ``seq_select`` + ``execute`` (admission),
 ``kv_copy`` (prefix reuse), ``batch_begin_slots`` + ``batch_decode`` (the steps).  The runtime object only needs those methods
@@ -114,6 +115,7 @@ class ContinuousBatcher:
         self.rows_run = 0           # rows those steps carried (sum of live sequences per step; with a drafter, of nodes)
         self.drafted = 0            # guesses made, and those that stood
         self.stood = 0
+        self.pass_nodes: Optional[int] = None        # nodes that a pass takes, of all trees (asked for by the first speculative step)
 
     # ---- requests ------------------------------------------------------------------------------------------------
     def submit(self, prompt: Sequence[int], max_new: int, eos: Optional[Iterable[int]] = None) -> int:
@@ -221,13 +223,19 @@ class ContinuousBatcher:
         """One speculative step of every live sequence.  False: a request has ended, its slot can be filled."""
         slots = sorted(self.live)
         reqs = [self.live[s] for s in slots]
+        if self.pass_nodes is None:
+            capacity = getattr(self.rt, "draft_capacity", None)
+            self.pass_nodes = 1 << 30 if capacity is None else capacity()
         trees = []
-        for r in reqs:
-            # guesses that could all stand without passing what the request may still generate (the sample behind them is one more)
-            room = min(r.max_new - len(r.tokens) - 1, self.max_nodes - 1)
+        left = self.pass_nodes - len(reqs)               # guesses that the pass has room for, next to a node of every sequence
+        for i, r in enumerate(reqs):
+            # guesses that could all stand without passing what the request may still generate (the sample behind them is one more), and no more than an
+            # even share of what the sequences before have left
+            room = min(r.max_new - len(r.tokens) - 1, self.max_nodes - 1, left // (len(reqs) - i))
             tokens, parents = self.drafter(r.prompt + r.tokens, room) if room > 0 else ([], [])
             if len(tokens) > room or len(tokens) != len(parents) or any(not 0 <= p <= i for i, p in enumerate(parents)):
                 raise ValueError(f"the drafter returned {len(tokens)} tokens and {len(parents)} parents for room {room}, or a parent that is no earlier guess")
+            left -= len(tokens)
             trees.append(([r.cur] + [int(t) for t in tokens], [-1] + [int(p) for p in parents]))
         self.steps_run += 1
         ended = False

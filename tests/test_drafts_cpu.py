@@ -243,3 +243,45 @@ def test_a_drafter_that_breaks_its_promise_is_refused(pkg):
         b.submit([1, 2], max_new=6)
         with pytest.raises(ValueError):
             b.run()
+
+
+class Narrow(Stand):
+    """A stand-in whose passes take a limited number of nodes, as those of lum_draft_verify."""
+
+    def __init__(self, capacity, **kw):
+        super().__init__(**kw)
+        self.capacity, self.widest = capacity, 0
+
+    def draft_capacity(self):
+        return self.capacity
+
+    def draft_verify(self, trees, positions, slots):
+        n = sum(len(t) for t, _ in trees)
+        assert n <= self.capacity, f"{n} nodes in all, a pass takes {self.capacity}"
+        self.widest = max(self.widest, n)
+        return super().draft_verify(trees, positions, slots)
+
+
+@pytest.mark.parametrize("sequences, capacity, max_seq", [(32, 256, 256), (8, 128, 128), (5, 5, 64), (7, 9, 64), (3, 1000, 64)])
+def test_the_loop_keeps_to_the_nodes_that_a_pass_takes(pkg, sequences, capacity, max_seq):
+    rt = Narrow(capacity, max_batch=sequences, max_seq=max_seq)
+    b = pkg.serving.ContinuousBatcher(rt, drafter=pkg.serving.PromptLookup())
+    prompts = [[(i + j) % 5 for j in range(5)] * 4 + [i % 5] for i in range(sequences + 3)]
+    ids = [b.submit(p, max_new=30) for p in prompts]
+    got = b.run()
+    assert [got[i] for i in ids] == [generate(p, 30) for p in prompts]
+    assert b.stats()["drafted"] > 0 or capacity == sequences
+
+
+def test_room_that_one_sequence_does_not_use_goes_to_the_next_ones(pkg):
+    rt, rooms = Narrow(11, max_batch=3), []
+
+    def drafter(text, room):
+        rooms.append(room)
+        return ([], []) if len(rooms) % 3 == 1 else ([4] * room, list(range(room)))
+
+    b = pkg.serving.ContinuousBatcher(rt, steps_per_round=1, drafter=drafter)
+    for i in range(3):
+        b.submit([i, 1, 2], max_new=20)
+    b.round()
+    assert rooms == [2, 4, 4] and rt.widest == 11

@@ -205,3 +205,46 @@ def test_serving_with_a_drafter(pkg, page):
         finally:
             rt.close()
     assert out[0] == out[1]
+
+
+def test_serving_with_more_guesses_than_a_pass_takes(pkg, monkeypatch):
+    """Passes of 32 rows, and a drafter that would fill 41 for each of three sequences: the loop shares the rows out."""
+    monkeypatch.setenv("LUM_ROWS_CAP", "32")
+    out = []
+
+    def look(text, room):
+        tokens, parents = pkg.serving.PromptLookup(length=20, match=1, places=2)(text, room)
+        return tokens + [3] * (room - len(tokens)), parents + [0] * (room - len(tokens))
+
+    for drafter in (None, look):
+        rt = runtime(pkg, max_batch=3, max_seq=256)
+        try:
+            b = pkg.serving.ContinuousBatcher(rt, steps_per_round=4, drafter=drafter)
+            ids = [b.submit(p, max_new=20) for p in PROMPTS + [[6, 5, 4, 6, 5, 4, 6, 5], [2] * 12]]
+            res = b.run()
+            out.append([res[i] for i in ids])
+            if drafter:
+                assert rt.draft_capacity() == 32
+                with pytest.raises(pkg.LumError) as e:   # the runtime itself still refuses what does not fit
+                    rt.draft_verify([([1] * 33, [-1] + [0] * 32)], [5], [0])
+                assert e.value.code == -1
+        finally:
+            rt.close()
+    assert out[0] == out[1]
+
+
+def test_capacity_of_a_model_that_cannot_verify(pkg):
+    rt = runtime(pkg, "tiny_f32")
+    try:
+        with pytest.raises(pkg.LumError) as e:
+            rt.draft_capacity()
+        assert e.value.code == -3
+    finally:
+        rt.close()
+    rt = runtime(pkg, max_seq=64)
+    try:
+        assert rt.draft_capacity() == 64
+        rt.set_data([1, 2, 3]); rt.execute({"s": 3, "p": 0})
+        assert len(rt.draft_verify([([rt.get_token()] + [1] * 60, [-1] + [0] * 60)], [3])[0]) >= 1
+    finally:
+        rt.close()
