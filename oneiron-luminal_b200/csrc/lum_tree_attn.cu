@@ -174,12 +174,16 @@ template <typename T> __device__ __forceinline__ T out_of(float x);
 template <> __device__ __forceinline__ float out_of<float>(float x) { return x; }
 template <> __device__ __forceinline__ __nv_bfloat16 out_of<__nv_bfloat16>(float x) { return __float2bfloat16_rn(x); }      // the one rounding of the result
 
+// x / sum; a sum that is not positive is undefined: a row all of whose visible scores are -inf is 0 / 0 (a finite score adds 1 to its row's sum, or a share that is
+// scaled against one that has)
+__device__ __forceinline__ float tree_ratio(float x, float sum) { return sum > 0.0f ? x / sum : __int_as_float(0x7fffffff); }
+// What a share (maximum m, sum l) of a row weighs against the row's maximum; a share with no score above -inf weighs nothing, undefined sums stay undefined.
+__device__ __forceinline__ float share_factor(float m, float l, float top) { return l != l ? 1.0f : m == -INFINITY ? 0.0f : m == top ? 1.0f : exp2f(m - top); }
 // The factor of a finished row: out = o / l, with the sink's part in l.
 __device__ __forceinline__ float tree_inverse(const TreeAttnArgs& a, int h, float m, float l) {
-    if (!a.sinks) return l > 0.0f ? 1.0f / l : l;    // (undefined stays undefined)
+    if (!a.sinks) return tree_ratio(1.0f, l);
     const float sink = a.sinks[h] * kLog2e, top = fmaxf(m, sink), c = m == -INFINITY ? 0.0f : exp2f(m - top);
-    const float sum = l * c + exp2f(sink - top);
-    return sum > 0.0f ? c / sum : sum;
+    return tree_ratio(c, l * c + exp2f(sink - top));
 }
 
 __device__ __forceinline__ float2 cluster_ld2(uint32_t at) { float2 v; asm volatile("ld.shared::cluster.v2.f32 {%0, %1}, [%2];" : "=f"(v.x), "=f"(v.y) : "r"(at) : "memory"); return v; }
@@ -218,14 +222,14 @@ __device__ __forceinline__ void join_cluster(const TreeAttnArgs& a, const Share&
         for (int i = 0; i < HD / 32; i++) z[i] = 0.0f;
 #pragma unroll
         for (int c = 0; c < kClusterMax; c++) {
-            if (ml[c].x == -INFINITY && ml[c].y == 0.0f) continue;   // no key that this row sees
-            const float f = ml[c].x == top || ml[c].y != ml[c].y ? 1.0f : exp2f(ml[c].x - top);      // (undefined sums stay undefined)
+            if (c >= C) continue;
+            const float f = share_factor(ml[c].x, ml[c].y, top);
             const float* part_of = (const float*)&y[c];
             sum = fmaf(ml[c].y, f, sum);
 #pragma unroll
             for (int i = 0; i < HD / 32; i++) z[i] = fmaf(part_of[i], f, z[i]);
         }
-        const float inv = sum > 0.0f ? 1.0f / sum : sum;
+        const float inv = tree_ratio(1.0f, sum);
         TQ* dst = (TQ*)a.out + (size_t)(x.q.r0 + node) * a.out_stride + (size_t)h * HD + lane * (HD / 32);
 #pragma unroll
         for (int i = 0; i < HD / 32; i++) dst[i] = out_of<TQ>(z[i] * inv);
@@ -1022,9 +1026,8 @@ __global__ void __launch_bounds__(256, kJoinCtas) tree_combine(const TreeAttnArg
 #pragma unroll
             for (int i = 16; i > 0; i >>= 1) t = fmaxf(t, __shfl_xor_sync(0xffffffffu, t, i));
             const float before = top == t ? 1.0f : exp2f(top - t);
-            // negative: a share without a key that this row sees; undefined sums stay undefined
-            const float factor = m == -INFINITY && l == 0.0f ? -1.0f : m == t || l != l ? 1.0f : exp2f(m - t);
-            sum = sum * before + warp_sum(factor >= 0.0f ? l * factor : 0.0f);
+            const float factor = share_factor(m, l, t);
+            sum = sum * before + warp_sum(l * factor);
             top = t;
 #pragma unroll
             for (int i = 0; i < DPL; i++) o[i] *= before;
@@ -1033,7 +1036,7 @@ __global__ void __launch_bounds__(256, kJoinCtas) tree_combine(const TreeAttnArg
 #pragma unroll
                 for (int u = 0; u < 4; u++) {
                     const float g = __shfl_sync(0xffffffffu, factor, min(c + u, 31));
-                    if (c + u < n && g >= 0.0f) {
+                    if (c + u < n) {
                         const float* z = (const float*)&y[u];
 #pragma unroll
                         for (int i = 0; i < DPL; i++) o[i] = fmaf(z[i], g, o[i]);
@@ -1041,7 +1044,7 @@ __global__ void __launch_bounds__(256, kJoinCtas) tree_combine(const TreeAttnArg
                 }
             }
         }
-        const float inv = sum > 0.0f ? 1.0f / sum : sum;
+        const float inv = tree_ratio(1.0f, sum);
         TQ* dst = (TQ*)a.out + (size_t)row * a.out_stride + (size_t)h * HD + lane * DPL;
 #pragma unroll
         for (int i = 0; i < DPL; i++) dst[i] = out_of<TQ>(o[i] * inv);

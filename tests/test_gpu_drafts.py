@@ -207,6 +207,29 @@ def test_attention_large_scores(torch, ops, q, cache):
     assert np.abs(got - want).max() < 0.05
 
 
+@pytest.mark.parametrize("q, cache", TYPES)
+@pytest.mark.parametrize("hint", [0, 30000])
+@pytest.mark.parametrize("prefix", [40, 1000])
+@pytest.mark.parametrize("dim, sinks", [(64, False), (128, False), (64, True)])
+def test_attention_of_rows_whose_scores_are_all_minus_infinity(torch, ops, q, cache, hint, prefix, dim, sinks):
+    """The definition's 0 / 0: undefined, unless a sink is in the denominator (then nothing).  A node that sees one finite score takes that key alone."""
+    b = Batch(torch, ops, [3, 2], [prefix, 50], dim=dim, q=q, cache=cache, kind="star", hint=hint, sinks=sinks, seed=prefix)
+    b.q[:] = b.q.abs() + 2.0 ** -10
+    want, off = b.want()
+    at = b.where[0]
+    b.k[[int(r) for r in at[:prefix + 2]]] = float("-inf")   # all but node 2's
+    got = b.run().double().cpu().numpy()
+    assert np.isnan(got[:2]).all() if not sinks else (got[:2] == 0.0).all()
+    k, v, x = (t.double().cpu().numpy() for t in (b.k[int(at[prefix + 2])], b.v[int(at[prefix + 2])], b.q[2]))
+    sink = None if b.sinks is None else b.sinks.double().cpu().numpy()
+    one, one_off = plain.attention(x.reshape(1, b.heads, dim), k.reshape(1, b.n_kv, dim), v.reshape(1, b.n_kv, dim), [-1], 0, b.n_kv, 0, sink)
+    want[2], off[2] = one.reshape(-1), one_off.reshape(-1)
+    bound = off[2:] + (2.0 ** -8 * (np.abs(want[2:]) + off[2:]) + 2.0 ** -16 * np.abs(v).max() if q == "bf16" else 0.0)
+    bound[1:] += 2.0 ** -14 if q == "bf16" else 0.0          # (weights in two terms, of values up to 4)
+    assert (np.abs(got[2:] - want[2:]) <= bound).all()
+    ops.status()
+
+
 def test_attention_under_capture_on_another_stream_and_twice_at_once(torch, ops):
     b = Batch(torch, ops, [9, 30], [700, 90], dim=128, group=4, page=64)
     c = Batch(torch, ops, [3], [2000], dim=64, group=8, q="f32", seed=5)
