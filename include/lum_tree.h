@@ -58,8 +58,8 @@ typedef struct lum_kv_map {
  * itself; with `window` > 0 only what is fewer than `window` places before its own.  q and out: [n_rows][n_q_heads][head_dim], rows q_stride /
  * out_stride elements apart; k and v: rows kv_stride elements apart, each [n_kv_heads][head_dim]; query head h reads K/V head
  * h / (n_q_heads / n_kv_heads).  sinks (device [n_q_heads], or NULL): a logit per head that joins the softmax's denominator.  A row all of whose
- * visible scores are -inf is 0 / 0 and comes out as NaN (as 0 with a sink above -inf); so is one that sees a score that is NaN or +inf.  out must not
- * overlap q. */
+ * visible scores are -inf is 0 / 0 and comes out as NaN (as 0 with a sink above -inf); so is one that sees a score that is NaN or +inf.  A sink of -inf is none, one of +inf leaves zeros.
+ * out must not overlap q. */
 typedef struct lum_tree_attn {
     uint32_t q_dtype;          /* LUM_BF16 or LUM_F32, of q and out */
     uint32_t kv_dtype;         /* LUM_BF16, or LUM_F32 with queries in f32 */

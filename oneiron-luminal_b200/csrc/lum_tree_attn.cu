@@ -179,11 +179,13 @@ template <> __device__ __forceinline__ __nv_bfloat16 out_of<__nv_bfloat16>(float
 __device__ __forceinline__ float tree_ratio(float x, float sum) { return sum > 0.0f ? x / sum : __int_as_float(0x7fffffff); }
 // What a share (maximum m, sum l) of a row weighs against the row's maximum; a share with no score above -inf weighs nothing, undefined sums stay undefined.
 __device__ __forceinline__ float share_factor(float m, float l, float top) { return l != l ? 1.0f : m == -INFINITY ? 0.0f : m == top ? 1.0f : exp2f(m - top); }
+// What a sink adds to the sum against the maximum `top`, which is not below it: nothing where it is -inf, 1 where it is the maximum (+inf leaves nothing to the keys).
+__device__ __forceinline__ float sink_part(float sink, float top) { return sink == -INFINITY ? 0.0f : sink == top ? 1.0f : exp2f(sink - top); }
 // The factor of a finished row: out = o / l, with the sink's part in l.
 __device__ __forceinline__ float tree_inverse(const TreeAttnArgs& a, int h, float m, float l) {
     if (!a.sinks) return tree_ratio(1.0f, l);
-    const float sink = a.sinks[h] * kLog2e, top = fmaxf(m, sink), c = m == -INFINITY ? 0.0f : exp2f(m - top);
-    return tree_ratio(c, l * c + exp2f(sink - top));
+    const float sink = a.sinks[h] * kLog2e, top = fmaxf(m, sink), c = share_factor(m, l, top);
+    return tree_ratio(c, fmaf(l, c, sink_part(sink, top)));
 }
 
 __device__ __forceinline__ float2 cluster_ld2(uint32_t at) { float2 v; asm volatile("ld.shared::cluster.v2.f32 {%0, %1}, [%2];" : "=f"(v.x), "=f"(v.y) : "r"(at) : "memory"); return v; }
@@ -217,7 +219,7 @@ __device__ __forceinline__ void join_cluster(const TreeAttnArgs& a, const Share&
         float top = sink, z[HD / 32];
 #pragma unroll
         for (int c = 0; c < kClusterMax; c++) top = fmaxf(top, ml[c].x);
-        float sum = !a.sinks ? 0.0f : sink == top ? 1.0f : exp2f(sink - top);
+        float sum = sink_part(sink, top);
 #pragma unroll
         for (int i = 0; i < HD / 32; i++) z[i] = 0.0f;
 #pragma unroll
@@ -1003,7 +1005,7 @@ __global__ void __launch_bounds__(256, kJoinCtas) tree_combine(const TreeAttnArg
         if (shares == 1) continue;                       // finished by its CTA
         const int f = (row - q.r0) * G + h % G, R = part.tile_rows, first = first_of_seq + (h / G * ((q.n * G + R - 1) / R) + f / R) * shares, r = f % R;
         const float sink = a.sinks ? a.sinks[h] * kLog2e : -INFINITY;
-        float top = sink, sum = a.sinks ? 1.0f : 0.0f, o[DPL];
+        float top = sink, sum = sink_part(sink, sink), o[DPL];
 #pragma unroll
         for (int i = 0; i < DPL; i++) o[i] = 0.0f;
         // 32 shares at a time: a lane has the factor of one, all have their dimensions of each, four on their way

@@ -230,6 +230,23 @@ def test_attention_of_rows_whose_scores_are_all_minus_infinity(torch, ops, q, ca
     ops.status()
 
 
+@pytest.mark.parametrize("q, cache", TYPES)
+@pytest.mark.parametrize("hint", [0, 30000])
+@pytest.mark.parametrize("prefix", [40, 1000])
+@pytest.mark.parametrize("dim", [64, 128])
+def test_attention_with_infinite_sinks(torch, ops, q, cache, hint, prefix, dim):
+    """-inf is no sink, +inf leaves nothing to the keys, whatever way the work is shared out; an undefined one stays undefined."""
+    b = Batch(torch, ops, [3, 2], [prefix, 50], group=4, n_kv=1, dim=dim, q=q, cache=cache, hint=hint, sinks=True, seed=prefix)
+    b.sinks.copy_(torch.tensor([float("-inf"), 0.7, float("inf"), float("nan")]))
+    got = b.run().unflatten(1, (4, dim))
+    ops.status()
+    assert (got[:, 2] == 0.0).all() and torch.isnan(got[:, 3]).all()
+    b.sinks.copy_(torch.tensor([-1e30, 0.7, 0.0, 0.0]))      # (-inf in the float64 statement's exponentials)
+    want, off = (x.reshape(5, 4, dim)[:, :2] for x in b.want())
+    bound = off + (2.0 ** -8 * (np.abs(want) + off) + 2.0 ** -16 * np.abs(b.v[np.concatenate(b.where)].double().cpu().numpy()).max() if q == "bf16" else 0.0)
+    assert (np.abs(got[:, :2].double().cpu().numpy() - want) <= bound).all()
+
+
 def test_attention_under_capture_on_another_stream_and_twice_at_once(torch, ops):
     b = Batch(torch, ops, [9, 30], [700, 90], dim=128, group=4, page=64)
     c = Batch(torch, ops, [3], [2000], dim=64, group=8, q="f32", seed=5)
