@@ -616,10 +616,12 @@ __global__ void __launch_bounds__(kTcThreads, TcShape<HD, F32>::ctas) attn_tree_
         const CUtensorMap* map = keys ? &map_k : &map_v;
         const uint32_t dst0 = base + (keys ? S::off_k : S::off_v), full = keys ? bar_k : bar_v, used = keys ? bar_s : bar_o;
         int last = -1;
-        // Where this lane's box of tile t starts in the cache (a lane per box); a page-table entry is on its way while the tile before is waited for.
+        // Where this lane's box of tile t starts in the cache (a lane per box; a box of a whole tile is every lane's, whichever is elected to ask for it); a
+        // page-table entry is on its way while the tile before is waited for.
+        const int boxes = kTileKeys / box_rows, box = boxes == 1 ? 0 : lane;
         auto box_row = [&](int t) {
-            const int j = (t_first + t) * kTileKeys + lane * box_rows;
-            if (t >= n_tiles || lane >= kTileKeys / box_rows || j >= w.n_keys || j + box_rows <= w.low) return (int)a.m.rows;     // outside the tensor: zeros
+            const int j = (t_first + t) * kTileKeys + box * box_rows;
+            if (t >= n_tiles || box >= boxes || j >= w.n_keys || j + box_rows <= w.low) return (int)a.m.rows;     // outside the tensor: zeros
             const long long row = tree_row(a.m, q.slot, j, a.status);
             return (int)(row < 0 ? a.m.rows : row);
         };
@@ -634,7 +636,7 @@ __global__ void __launch_bounds__(kTcThreads, TcShape<HD, F32>::ctas) attn_tree_
             __syncwarp();
             // a box holds its halves of 64 dimensions one behind the other; a whole tile's are kTileKeys rows apart
             if (box_rows == kTileKeys) { if (elect_one()) tma_box(dst, map, row, kvh * kHalves, bar); }
-            else if (lane < kTileKeys / box_rows)
+            else if (lane < boxes)
 #pragma unroll
                 for (int h = 0; h < kHalves; h++) tma_box(dst + h * (kTileKeys * 128) + lane * box_rows * 128, map, row, kvh * kHalves + h, bar);
             last = t;
