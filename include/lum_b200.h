@@ -418,6 +418,9 @@ int32_t lum_debug_wait_timeout(lum_rt* rt);
 /* Test hook: the next n graph captures that ask for programmatic dependent launch fail, as on a driver that cannot capture its edges; the
  * runtime then captures ordinary dependencies. */
 int32_t lum_debug_fail_pdl_captures(lum_rt* rt, int32_t n);
+/* Test hook: leaves `bits` in the device status word, in the order of the runtime's stream, as a kernel does that found something wrong; the
+ * next call that waits reports them as LUM_E_DEVICE. */
+int32_t lum_debug_set_status(lum_rt* rt, uint32_t bits);
 
 /* ---------------------------------------------------------------------------------------------
  * Tensor parallelism over the GPUs of one node: one process and one runtime per GPU (the reference is single-GPU:

@@ -536,10 +536,12 @@ int check_status(lum_rt* rt) {
             cudaMemsetAsync(rt->job_ctr, 0, (size_t)kJobCtrRing * kMaxKRanges * sizeof(unsigned int), rt->stream);
             rt->gbar_base = 0;
         }
-        return fail(rt, LUM_E_DEVICE, "device status 0x%x (%s%s%s%s%s%s)", st, (st & LUM_ST_WAIT_GRID) ? "grid barrier timed out; " : "",
+        return fail(rt, LUM_E_DEVICE, "device status 0x%x (%s%s%s%s%s%s%s%s)", st, (st & LUM_ST_WAIT_GRID) ? "grid barrier timed out; " : "",
                     (st & LUM_ST_WAIT_FULL) ? "stage wait timed out; " : "",
                     (st & LUM_ST_WAIT_EMPTY) ? "producer wait timed out; " : "", (st & LUM_ST_WAIT_DRAIN) ? "drain wait timed out; " : "",
-                    (st & LUM_ST_BAD_TOKEN) ? "token id out of range; " : "", (st & LUM_ST_BAD_POS) ? "position out of range; " : "");
+                    (st & LUM_ST_BAD_TOKEN) ? "token id out of range; " : "", (st & LUM_ST_BAD_POS) ? "position out of range; " : "",
+                    (st & LUM_ST_BAD_TREE) ? "drafted tokens that are no tree, or no path through one; " : "",
+                    (st & LUM_ST_BAD_PAGE) ? "cache row or page out of range; " : "");
         // (0x40 tensor-memory hand-over and 0x80 a word from another GPU that never came show in the hexadecimal value)
     }
     return 0;
@@ -2945,6 +2947,14 @@ int32_t lum_debug_wait_timeout(lum_rt* rt) {
 int32_t lum_debug_fail_pdl_captures(lum_rt* rt, int32_t n) {
     if (!rt || n < 0) return fail(rt, LUM_E_INVALID, "debug_fail_pdl_captures: no runtime or a negative count");
     rt->fail_pdl_captures = n;
+    return 0;
+}
+
+// Test hook: the status word as a kernel that found something wrong leaves it.
+int32_t lum_debug_set_status(lum_rt* rt, uint32_t bits) {
+    if (!rt || !rt->has_model) return fail(rt, LUM_E_INVALID, "debug_set_status: no model");
+    CU(rt, cudaSetDevice(rt->cfg.device));
+    CU(rt, cudaMemcpyAsync(rt->status, &bits, sizeof bits, cudaMemcpyHostToDevice, rt->stream));              // pageable source: staged before the call returns
     return 0;
 }
 

@@ -279,6 +279,7 @@ def load_library() -> C.CDLL:
         "lum_get_stats": (i32, [vp, P(Stats)]),
         "lum_debug_wait_timeout": (i32, [vp]),
         "lum_debug_fail_pdl_captures": (i32, [vp, i32]),
+        "lum_debug_set_status": (i32, [vp, C.c_uint32]),
         "lum_op_status": (i32, [vp]),
         "lum_get_output": (i32, [vp, C.c_int64, P(C.c_float), sz]),
         "lum_get_output_raw": (i32, [vp, C.c_int64, vp, sz, P(u32), P(sz)]),
@@ -630,6 +631,10 @@ class B200Runtime:
     def debug_fail_pdl_captures(self, n: int) -> None:
         """Test hook: the next `n` graph captures with programmatic dependent launch fail; ordinary dependencies take their place."""
         self._ck(self._lib.lum_debug_fail_pdl_captures(self._h, n))
+
+    def debug_set_status(self, bits: int) -> None:
+        """Test hook: bits of the device status word, as a kernel that found something wrong leaves them."""
+        self._ck(self._lib.lum_debug_set_status(self._h, bits))
 
     def stats(self) -> Stats:
         st = Stats()

@@ -248,3 +248,18 @@ def test_capacity_of_a_model_that_cannot_verify(pkg):
         assert len(rt.draft_verify([([rt.get_token()] + [1] * 60, [-1] + [0] * 60)], [3])[0]) >= 1
     finally:
         rt.close()
+
+
+@pytest.mark.parametrize("bits, words", [(1 << 8, "no tree"), (1 << 9, "cache row or page"), (1 << 8 | 1 << 9, "no path through one; cache row or page")])
+def test_the_runtime_says_what_was_wrong_with_a_tree_or_a_page(pkg, bits, words):
+    rt = runtime(pkg, max_seq=64)
+    try:
+        rt.set_data([1, 2, 3]); rt.execute({"s": 3, "p": 0})
+        cur = rt.get_token()
+        rt.debug_set_status(bits)
+        with pytest.raises(pkg.LumError) as e:
+            rt.draft_verify([([cur, 1], [-1, 0])], [3])
+        assert e.value.code == -4 and words in str(e.value) and hex(bits) in str(e.value)
+        assert len(rt.draft_verify([([cur, 1], [-1, 0])], [3])[0]) >= 1                  # and goes on
+    finally:
+        rt.close()
