@@ -13,6 +13,7 @@
 // append + attention] -> [o projection + residual] -> [RMSNorm + gate,up projections + SwiGLU] ->
 // [down projection + residual] } -> [RMSNorm + lm_head + greedy sample + state advance]:
 // 5 launches per layer, each bracket one kernel.
+#include <algorithm>
 #include <cmath>
 #include <cstdarg>
 #include <cstdio>
@@ -1448,13 +1449,22 @@ int run_rows_sequential(lum_rt* rt, int M, int* d_tok, int* d_pos, const int* d_
     return 0;
 }
 
-// room for `want` elements of a buffer of the drafted-tree steps, which grows
+// Room for `want` elements of a buffer of the drafted-tree steps, whose contents are over.  It grows by half, up to `most` (what the largest step
+// needs), so that steps that grow little by little seldom come here; the outgrown one goes back first, and where the reserve does not fit the step's own need is taken.
 template <typename T>
-int draft_room(lum_rt* rt, T** p, size_t* cap, size_t want) {
+int draft_room(lum_rt* rt, T** p, size_t* cap, size_t want, size_t most) {
     if (want <= *cap) return 0;
-    const size_t n = want + want / 2;
-    *cap = 0;
-    if (int r = dev_alloc(rt, (void**)p, n * sizeof(T))) return r;
+    if (*cap) {
+        CU(rt, cudaStreamSynchronize(rt->stream));       // the steps before read it
+        rt->allocs.erase(std::find(rt->allocs.begin(), rt->allocs.end(), (void*)*p));
+        cudaFree(*p);
+        *p = nullptr;
+        *cap = 0;
+    }
+    size_t n = std::max(want, std::min(want + want / 2, most));
+    int r = dev_alloc(rt, (void**)p, n * sizeof(T));
+    if (r && n > want) { cudaGetLastError(); r = dev_alloc(rt, (void**)p, (n = want) * sizeof(T)); }
+    if (r) { cudaGetLastError(); return r; }             // (not the next launch's error)
     *cap = n;
     return 0;
 }
@@ -2839,7 +2849,8 @@ int32_t lum_draft_verify(lum_rt* rt, int32_t n_seq, const int32_t* slots, const 
     up.insert(up.end(), tokens, tokens + R);
     up.insert(up.end(), parents, parents + R);
     for (const std::vector<int32_t>* v : {&place, &at, &seq, &draw}) up.insert(up.end(), v->begin(), v->end());
-    if (int r = draft_room(rt, &w.ints, &w.ints_cap, up.size() + R)) return r;
+    const size_t most_rows = (size_t)rt->rows.cap, most_seq = (size_t)rt->max_batch;                          // of any step
+    if (int r = draft_room(rt, &w.ints, &w.ints_cap, up.size() + R, 3 * most_seq + 1 + 7 * most_rows)) return r;
     CU(rt, cudaMemcpyAsync(w.ints, up.data(), up.size() * 4, cudaMemcpyHostToDevice, rt->stream));            // pageable source: staged before the call returns
     int *d_tok = w.ints + rows0, *d_parent = d_tok + R, *d_place = d_parent + R, *d_at = d_place + R, *d_seq = d_at + R, *d_draw = d_seq + R, *d_pick = d_draw + R;
     TreeRows tree{};
@@ -2848,9 +2859,9 @@ int32_t lum_draft_verify(lum_rt* rt, int32_t n_seq, const int32_t* slots, const 
     tree.at = d_at;
     const TreeAttnArgs probe = tree_attn_args(rt, tree);
     const size_t attn_ws = tree_attn_workspace(probe, rt->sm_count), accept_ws = tree_accept_workspace(tree.t, rt->vocab_l, rt->sm_count);
-    if (int r = draft_room(rt, &w.ws, &w.ws_cap, attn_ws > accept_ws ? attn_ws : accept_ws)) return r;
-    if (int r = draft_room(rt, &w.found, &w.found_cap, 2 * n + n * (size_t)max_rows)) return r;
-    if (int r = draft_room(rt, &w.logits, &w.logits_cap, rows_parts_floats(rt, rt->vocab_l, rt->d.hidden, M))) return r;
+    if (int r = draft_room(rt, &w.ws, &w.ws_cap, attn_ws > accept_ws ? attn_ws : accept_ws, SIZE_MAX)) return r;
+    if (int r = draft_room(rt, &w.found, &w.found_cap, 2 * n + n * (size_t)max_rows, (2 + (size_t)kTreeMax) * most_seq)) return r;
+    if (int r = draft_room(rt, &w.logits, &w.logits_cap, rows_parts_floats(rt, rt->vocab_l, rt->d.hidden, M), rows_parts_floats(rt, rt->vocab_l, rt->d.hidden, rt->rows.cap))) return r;
     tree.ws = w.ws; tree.ws_bytes = w.ws_cap; tree.logits = w.logits;
     if (int r = run_rows(rt, M, d_tok, d_place, d_seq, 0, 3, &tree)) return r;
     TreeAcceptArgs a{};

@@ -263,3 +263,21 @@ def test_the_runtime_says_what_was_wrong_with_a_tree_or_a_page(pkg, bits, words)
         assert len(rt.draft_verify([([cur, 1], [-1, 0])], [3])[0]) >= 1                  # and goes on
     finally:
         rt.close()
+
+
+def test_steps_that_grow_keep_no_more_memory_than_the_largest_one(pkg):
+    """The buffers of a step that was outgrown go back: what is left is what a runtime holds that ran the largest step first."""
+    import torch
+    used = []
+    for sizes in ([256], [256], [8, 30, 60, 100, 150, 200, 256]):                        # (the first time loads the kernels)
+        before = torch.cuda.mem_get_info()[0]
+        rt = runtime(pkg, max_batch=8, max_seq=2048)
+        try:
+            for n in sizes:
+                rt.draft_verify([([1] * n, [-1] + [0] * (n - 1))] * 8, [0] * 8)
+            used.append(before - torch.cuda.mem_get_info()[0])
+        finally:
+            rt.close()
+    # a block of the allocator (2 MB) for each of the step's four buffers.  Without giving back, the logits alone (2048 values of f32) leave 1.5 x 8 x
+    # (8 + 30 + 60 + 100 + 200) rows of 8 KB: 39 MB, where the largest step needs 17
+    assert used[2] <= used[1] + 8 * 2 ** 20, used
