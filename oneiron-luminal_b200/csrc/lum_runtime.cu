@@ -1124,9 +1124,12 @@ int kv_page_upload(lum_rt* rt, int seq, int lp) {
 void kv_page_unref(lum_rt* rt, int page) {
     if (page >= 0 && --rt->page_ref[(size_t)page] == 0) rt->page_free.push_back(page);
 }
+int kv_pool_empty(lum_rt* rt) {
+    return fail(rt, LUM_E_NOMEM, "the K/V page pool is exhausted (%d pages of %d rows): release a sequence (lum_kv_release) or load the model with more kv_pool_pages", rt->pool_pages,
+                rt->page_rows);
+}
 int kv_page_take(lum_rt* rt, int* page) {
-    if (rt->page_free.empty()) return fail(rt, LUM_E_NOMEM, "the K/V page pool is exhausted (%d pages of %d rows): release a sequence (lum_kv_release) or load the model with more kv_pool_pages",
-                                           rt->pool_pages, rt->page_rows);
+    if (rt->page_free.empty()) return kv_pool_empty(rt);
     *page = rt->page_free.back();
     rt->page_free.pop_back();
     rt->page_ref[(size_t)*page] = 1;
@@ -1149,6 +1152,20 @@ int kv_ensure(lum_rt* rt, int seq, int from, int to) {
         if (int r = kv_page_upload(rt, seq, lp)) return r;
     }
     return 0;
+}
+// Whether the pool has what kv_ensure takes for rows [from[i], to[i]) of sequence seq[i], for all of them: nothing is taken for some where it has not.
+// (A page that several of them share is copied for all but the last owner.)
+bool kv_pool_has(const lum_rt* rt, const std::vector<int32_t>& seq, const int32_t* from, const std::vector<int32_t>& to) {
+    if (!rt->page_rows) return true;
+    std::map<int, int> let_go;
+    size_t need = 0;
+    for (size_t i = 0; i < seq.size(); i++)
+        for (int lp = from[i] >> rt->page_lg; lp <= (to[i] - 1) >> rt->page_lg; lp++) {
+            const int e = rt->h_page_table[(size_t)seq[i] * rt->pages_per_seq + lp];
+            if (e < 0) need++;
+            else if (rt->page_ref[(size_t)e] > 1 && rt->page_ref[(size_t)e] - let_go[e] > 1) { let_go[e]++; need++; }
+        }
+    return need <= rt->page_free.size();
 }
 void kv_release_seq(lum_rt* rt, int seq) {
     for (int lp = 0; lp < rt->pages_per_seq; lp++) {
@@ -2812,7 +2829,7 @@ int32_t lum_draft_verify(lum_rt* rt, int32_t n_seq, const int32_t* slots, const 
     std::vector<char> taken((size_t)rt->max_batch, 0);
     lum_rt::Drafts& w = rt->drafts;
     w.n_seq = 0;
-    std::vector<int32_t> place, at, seq, draw, slot((size_t)n_seq);
+    std::vector<int32_t> place, at, seq, draw, slot((size_t)n_seq), end((size_t)n_seq);
     int max_rows = 1, max_prefix = 0;
     for (int s = 0; s < n_seq; s++) {
         const int n = row_start[s + 1] - row_start[s], p = positions[s], sl = slots ? slots[s] : s;
@@ -2821,6 +2838,7 @@ int32_t lum_draft_verify(lum_rt* rt, int32_t n_seq, const int32_t* slots, const 
         if (p < 0 || p > rt->d.max_seq - n) return fail(rt, LUM_E_INVALID, "draft_verify: %d nodes behind position %d pass the cache capacity %d", n, p, rt->d.max_seq);
         taken[(size_t)sl] = 1;
         slot[(size_t)s] = sl;
+        end[(size_t)s] = p + n;
         if (n > max_rows) max_rows = n;
         if (p > max_prefix) max_prefix = p;
         for (int i = 0; i < n; i++) {
@@ -2838,8 +2856,8 @@ int32_t lum_draft_verify(lum_rt* rt, int32_t n_seq, const int32_t* slots, const 
     if (int r = ensure_rows(rt, 1)) return r;
     if (M > rt->rows.cap) return fail(rt, LUM_E_INVALID, "draft_verify: %d nodes in all, a pass takes %d", M, rt->rows.cap);
     if (!kv_movable(rt)) return fail(rt, LUM_E_UNSUPPORTED, "draft_verify: cache rows that are no multiple of 16 bytes, or 2^31 of them");
+    if (!kv_pool_has(rt, slot, positions, end)) return kv_pool_empty(rt);
     if (int r = kv_planes(rt)) return r;
-    for (int s = 0; s < n_seq; s++) if (int r = kv_ensure(rt, slot[(size_t)s], positions[s], positions[s] + row_start[s + 1] - row_start[s])) return r;
     // one upload: row_start, prefix, slot, then per row token, parent, place, cache row, slot, position of the token drawn there (and room for the picks)
     const size_t n = (size_t)n_seq, R = (size_t)M;
     std::vector<int32_t> up(row_start, row_start + n + 1);
@@ -2863,6 +2881,8 @@ int32_t lum_draft_verify(lum_rt* rt, int32_t n_seq, const int32_t* slots, const 
     if (int r = draft_room(rt, &w.found, &w.found_cap, 2 * n + n * (size_t)max_rows, (2 + (size_t)kTreeMax) * most_seq)) return r;
     if (int r = draft_room(rt, &w.logits, &w.logits_cap, rows_parts_floats(rt, rt->vocab_l, rt->d.hidden, M), rows_parts_floats(rt, rt->vocab_l, rt->d.hidden, rt->rows.cap))) return r;
     tree.ws = w.ws; tree.ws_bytes = w.ws_cap; tree.logits = w.logits;
+    // (pages last: a call that is refused takes none)
+    for (int s = 0; s < n_seq; s++) if (int r = kv_ensure(rt, slot[(size_t)s], positions[s], end[(size_t)s])) return r;
     if (int r = run_rows(rt, M, d_tok, d_place, d_seq, 0, 3, &tree)) return r;
     TreeAcceptArgs a{};
     a.t = tree.t; a.tokens = d_tok; a.vocab = rt->vocab_l; a.ld = rt->vocab_l; a.path = w.found + 2 * n; a.path_len = max_rows; a.n_accepted = w.found; a.next = w.found + n;
