@@ -285,23 +285,23 @@ def test_steps_that_grow_keep_no_more_memory_than_the_largest_one(pkg):
 
 def test_a_step_that_the_pool_cannot_hold_takes_no_page(pkg):
     """Three sequences that share a prompt's pages; the pool runs out at the third.  One page more and the same step goes through."""
-    prompt = [(3 * i + 1) % 2000 for i in range(40)]
+    prompt = [(3 * i + 1) % 2000 for i in range(160)]
     for pages, ok in ((5, False), (6, True)):
-        rt = runtime(pkg, max_batch=4, kv_page_rows=16, max_seq=128, kv_pool_pages=pages)
+        rt = runtime(pkg, max_batch=4, kv_page_rows=64, max_seq=256, kv_pool_pages=pages)
         try:
-            rt.set_data(prompt); rt.execute({"s": 40, "p": 0})                           # 3 pages, the last one half full
+            rt.set_data(prompt); rt.execute({"s": 160, "p": 0})                          # 3 pages, the last one half full
             cur = rt.get_token()
-            rt.kv_copy(0, 1, 32); rt.kv_copy(0, 2, 32)                                   # two of them shared
+            rt.kv_copy(0, 1, 128); rt.kv_copy(0, 2, 128)                                 # two of them shared
             assert rt.kv_pool()[1] == pages - 3
             tree = ([cur, 1], [-1, 0])
-            # a page each for sequences 1 and 2 behind row 32, and a copy of the second page, whose last row sequence 1 writes
-            trees, positions, slots = [tree, tree, ([cur], [-1])], [31, 32, 40], [1, 2, 0]
+            # a page each for sequences 1 and 2 behind row 128, and a copy of the second page, whose last row sequence 1 writes
+            trees, positions, slots = [tree, tree, ([cur], [-1])], [127, 128, 160], [1, 2, 0]
             if ok:
                 assert [len(x) >= 1 for x in rt.draft_verify(trees, positions, slots)] == [True] * 3
             else:
                 with pytest.raises(pkg.LumError) as e:
                     rt.draft_verify(trees, positions, slots)
                 assert e.value.code == -5 and "pool" in str(e.value) and rt.kv_pool()[1] == pages - 3
-            assert len(rt.draft_verify([([cur, 1, 2], [-1, 0, 1])], [40], [0])[0]) >= 1   # and goes on
+            assert len(rt.draft_verify([([cur, 1, 2], [-1, 0, 1])], [160], [0])[0]) >= 1   # and goes on
         finally:
             rt.close()
