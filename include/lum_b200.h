@@ -380,7 +380,8 @@ int32_t lum_batch_get_logits(lum_rt* rt, int32_t seq, float* host_out, size_t n)
  * what decoding token by token gives, up to rounding.  Asynchronous.  lum_draft_get waits and reads, per sequence, how many tokens
  * follow node 0 (counts[s] >= 1: the guesses that stand and the sample behind them) and which (tokens_out [n_seq][len], len at least the
  * nodes of the largest tree); the cache then holds positions[s] + counts[s] rows of the sequence (pages behind them have gone back), and the last
- * token is node 0 of the next step.  The selected sequence's single-token steps (lum_decode_greedy) go on from there.
+ * token is node 0 of the next step.  Where it fails (LUM_E_DEVICE) the sequences are as long as before the step.  The selected sequence's
+ * single-token steps (lum_decode_greedy) go on from there.
  * A pass takes lum_draft_capacity nodes in all, at least max_batch (the cache's rows per sequence, 4096 at most; 32 at least).
  * Needs what lum_batch_begin needs, with max_batch 1 too. */
 int32_t lum_draft_capacity(lum_rt* rt, int32_t* nodes);

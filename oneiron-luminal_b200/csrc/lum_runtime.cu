@@ -2925,11 +2925,15 @@ int32_t lum_draft_get(lum_rt* rt, int32_t* counts, int32_t* tokens_out, size_t l
     CU(rt, cudaMemcpyAsync(got.data(), w.found, got.size() * 4, cudaMemcpyDeviceToHost, rt->stream));
     CU(rt, cudaStreamSynchronize(rt->stream));
     w.n_seq = 0;
-    if (int r = check_status(rt)) return r;
+    int bad = check_status(rt);
+    for (size_t s = 0; s < n && !bad; s++) if (got[s] < 1 || got[s] > max_rows) bad = fail(rt, LUM_E_DEVICE, "draft_get: %d nodes of sequence %zu stand", got[s], s);
+    if (bad) {                                           // the sequences are where they were before the step, their pages too
+        for (size_t s = 0; s < n; s++) kv_trim_seq(rt, w.slot[s], w.position[s]);
+        return bad;
+    }
     for (size_t s = 0; s < n; s++) {
         const int k = got[s], next = got[n + s];
         const int32_t* path = got.data() + 2 * n + s * (size_t)max_rows;
-        if (k < 1 || k > max_rows) return fail(rt, LUM_E_DEVICE, "draft_get: %d nodes of sequence %zu stand", k, s);
         counts[s] = k;
         for (int i = 1; i < k; i++) tokens_out[s * len + (size_t)i - 1] = w.tokens[(size_t)(w.row_start[s] + path[i])];
         tokens_out[s * len + (size_t)k - 1] = next;

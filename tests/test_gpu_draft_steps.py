@@ -305,3 +305,20 @@ def test_a_step_that_the_pool_cannot_hold_takes_no_page(pkg):
             assert len(rt.draft_verify([([cur, 1, 2], [-1, 0, 1])], [160], [0])[0]) >= 1   # and goes on
         finally:
             rt.close()
+
+
+def test_pages_of_a_step_that_a_kernel_gave_up_go_back(pkg):
+    rt = runtime(pkg, max_batch=2, kv_page_rows=64, max_seq=256)
+    try:
+        prompt = [(3 * i + 1) % 2000 for i in range(64)]
+        first = prompts_in(rt, [prompt, prompt])
+        free = rt.kv_pool()[1]
+        trees = [([t] + [1] * 100, [-1] + list(range(100))) for t in first]              # two pages each behind the prompt's
+        rt.debug_set_status(1 << 9)
+        with pytest.raises(pkg.LumError) as e:
+            rt.draft_verify(trees, [64, 64])
+        assert e.value.code == -4 and rt.kv_pool()[1] == free
+        again = rt.draft_verify(trees, [64, 64])                                         # and the step can be made again
+        assert [len(x) >= 1 for x in again] == [True, True]
+    finally:
+        rt.close()
