@@ -2828,7 +2828,6 @@ int32_t lum_draft_verify(lum_rt* rt, int32_t n_seq, const int32_t* slots, const 
     if (row_start[0] != 0) return fail(rt, LUM_E_INVALID, "draft_verify: the first sequence's rows start at %d, not 0", row_start[0]);
     std::vector<char> taken((size_t)rt->max_batch, 0);
     lum_rt::Drafts& w = rt->drafts;
-    w.n_seq = 0;
     std::vector<int32_t> place, at, seq, draw, slot((size_t)n_seq), end((size_t)n_seq);
     int max_rows = 1, max_prefix = 0;
     for (int s = 0; s < n_seq; s++) {
@@ -2867,6 +2866,7 @@ int32_t lum_draft_verify(lum_rt* rt, int32_t n_seq, const int32_t* slots, const 
     up.insert(up.end(), tokens, tokens + R);
     up.insert(up.end(), parents, parents + R);
     for (const std::vector<int32_t>* v : {&place, &at, &seq, &draw}) up.insert(up.end(), v->begin(), v->end());
+    w.n_seq = 0;                                         // (results that nobody has read: over from here on, not by a call that was refused)
     const size_t most_rows = (size_t)rt->rows.cap, most_seq = (size_t)rt->max_batch;                          // of any step
     if (int r = draft_room(rt, &w.ints, &w.ints_cap, up.size() + R, 3 * most_seq + 1 + 7 * most_rows)) return r;
     CU(rt, cudaMemcpyAsync(w.ints, up.data(), up.size() * 4, cudaMemcpyHostToDevice, rt->stream));            // pageable source: staged before the call returns

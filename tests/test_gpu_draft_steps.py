@@ -322,3 +322,20 @@ def test_pages_of_a_step_that_a_kernel_gave_up_go_back(pkg):
         assert [len(x) >= 1 for x in again] == [True, True]
     finally:
         rt.close()
+
+
+def test_results_outlive_a_refused_step(pkg):
+    import ctypes as C
+    ints = lambda *v: (C.c_int32 * len(v))(*v)  # noqa: E731
+    rt = runtime(pkg, max_batch=2, max_seq=64)
+    try:
+        first = prompts_in(rt, PROMPTS[:1])[0]
+        want = rt.draft_verify([([first], [-1])], [len(PROMPTS[0])])[0]
+        verify = lambda p, *t: rt._lib.lum_draft_verify(rt._h, 1, None, ints(p), ints(0, len(t)), ints(*t), ints(*range(-1, len(t) - 1)))  # noqa: E731
+        counts, out = (C.c_int32 * 1)(), (C.c_int32 * 1)()
+        assert verify(len(PROMPTS[0]), first) == 0
+        assert verify(64, first) == -1 and verify(3, 10 ** 6) == -1 and verify(3, *[1] * 65) == -1
+        assert rt._lib.lum_draft_get(rt._h, counts, out, 1) == 0 and [counts[0], out[0]] == [1] + want
+        assert rt._lib.lum_draft_get(rt._h, counts, out, 1) == -1                        # read once
+    finally:
+        rt.close()
