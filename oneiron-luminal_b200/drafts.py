@@ -134,15 +134,24 @@ def _rows_of(name, t, device, width, rows):
     return t.data_ptr(), (t.stride(0) if rows > 1 else width)
 
 
+def _no_gradient(*tensors):
+    """There is no backward pass: a result that looks like a constant where a gradient is being recorded is refused."""
+    if torch is None:
+        _use_torch()
+    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors):
+        _bad("attn_tree has no gradient: call it under torch.no_grad(), or with tensors that require none")
+
+
 def attn_tree(q, k, v, tree: DraftTree, cache: KvMap, *, n_kv_heads: int, head_dim: int, scale: float = 0.0, window: int = 0, sinks=None, out=None, workspace=None):
     """Attention of the drafted nodes over their sequences' cached rows and their own ancestors.
 
     ``q`` [rows, heads * head_dim] (or [rows, heads, head_dim]) in bf16 or f32; ``k`` and ``v`` [cache rows, n_kv_heads * head_dim] in bf16, or in f32 with f32
     queries; rows may be strided.  ``scale`` 0: 1 / sqrt(head_dim).  ``window``: a node sees only what is fewer than so many places before its own.  ``sinks``
     [heads] f32: a logit per head that joins the softmax's denominator.  Returns ``out`` (like q; rows of no sequence are left as they were; without ``out``
-    given they are not set).  ``workspace``: scratch to use
-    (None: taken from torch); calls that may overlap need one each."""
+    given they are not set).  ``workspace``: scratch to use (None: taken from torch); calls that may overlap need one each.  There is no gradient: tensors that
+    require one are refused while gradients are recorded."""
     device, q_type, k_type = q.device, _types().get(q.dtype), _types().get(k.dtype)
+    _no_gradient(q, k, v, sinks)
     if device != tree.device or q_type is None or k_type is None or v.dtype != k.dtype:
         _bad(f"attn_tree: q {q.dtype} on {device}, tree on {tree.device}, k {k.dtype}, v {v.dtype}: bf16 or f32 on one device are wanted")
     rows = tree.n_rows

@@ -151,6 +151,22 @@ def test_rows_that_share_memory_are_refused(pkg, rows, ok):
             assert e.value.code == -1
 
 
+def test_gradients_are_refused_where_they_are_recorded(pkg):
+    import torch
+    d = pkg.drafts
+    x, y = torch.zeros(2, 64), torch.zeros(2, 64, requires_grad=True)
+    for tensors in ((y, x, x, None), (x, y, x, None), (x, x, y, None), (x, x, x, y)):
+        with pytest.raises(pkg.LumError) as e:
+            d._no_gradient(*tensors)
+        assert e.value.code == -1 and "gradient" in str(e.value)
+        with torch.no_grad():
+            d._no_gradient(*tensors)
+    d._no_gradient(x, x, x, None)
+    with pytest.raises(pkg.LumError) as e:
+        d.attn_tree(y, x, x, None, None, n_kv_heads=1, head_dim=64)
+    assert "gradient" in str(e.value)
+
+
 # ---- the drafter and the loop
 
 
