@@ -431,7 +431,9 @@ int32_t lum_op_attn_tree(const lum_tree_attn* desc, const lum_draft_tree* tree, 
 size_t lum_op_tree_accept_workspace(const lum_draft_tree* tree, int32_t vocab) {
     TreeBatch t{};
     Device d;
-    if (check_tree("tree_accept", tree, &t) || vocab < 1 || vocab > (1 << 30) || device_of("tree_accept", &d)) return (size_t)-1;
+    if (check_tree("tree_accept", tree, &t)) return (size_t)-1;
+    if (vocab < 1 || vocab > (1 << 30)) { refuse("tree_accept", "a vocabulary of 1 .. 2^30, got " + std::to_string(vocab)); return (size_t)-1; }
+    if (device_of("tree_accept", &d)) return (size_t)-1;
     return t.n_seq && t.n_rows ? tree_accept_workspace(t, vocab, d.sms) : 0;
 }
 

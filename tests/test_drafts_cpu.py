@@ -116,6 +116,14 @@ def test_accept_compact_and_copy_refuse(pkg):
     assert lib.lum_op_tree_accept_workspace(tree, 0) == C.c_size_t(-1).value
 
 
+def test_the_workspace_of_a_walk_says_why_it_refuses(pkg):
+    lib, tree = pkg.load_library(), pkg.runtime.DraftTreeDesc(**TREE)
+    for vocab in (0, -3, 2 ** 30 + 1):
+        assert lib.lum_op_attn_tree_workspace(None, tree, None) == C.c_size_t(-1).value              # another operator's message is the last one
+        assert lib.lum_op_tree_accept_workspace(tree, vocab) == C.c_size_t(-1).value
+        assert b"vocabulary" in lib.lum_last_error(None) and str(vocab).encode() in lib.lum_last_error(None)
+
+
 def test_python_calls_refuse_tensors_of_the_wrong_kind(pkg):
     import torch
     d = pkg.drafts
