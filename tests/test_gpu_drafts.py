@@ -207,6 +207,49 @@ def test_attention_large_scores(torch, ops, q, cache):
     assert np.abs(got - want).max() < 0.05
 
 
+def rounded(b, want, off):
+    """The bound of bf16 results: the rounding of the result, and weights in two bf16 terms against the largest value of the cache that is finite."""
+    if b.q.dtype != b.torch.bfloat16:
+        return off
+    v = b.v[np.concatenate(b.where)].double().cpu().numpy()
+    return off + 2.0 ** -8 * (np.abs(want) + off) + 2.0 ** -16 * np.abs(v[np.abs(v) < 1e30]).max()
+
+
+@pytest.mark.parametrize("q, cache", TYPES)
+@pytest.mark.parametrize("dim", [64, 128])
+@pytest.mark.parametrize("prefix", [70, 1000])
+@pytest.mark.parametrize("value", [float("inf"), float("-inf"), float("nan"), 3.0e38])
+def test_attention_beside_masked_values_keeps_its_bound(torch, ops, q, cache, dim, prefix, value):
+    """What nobody sees changes nothing, down to the bound of f32 arithmetic: one key more or less, of some 40, would be far outside it."""
+    b = Batch(torch, ops, [6, 4], [prefix, 66], dim=dim, q=q, cache=cache, kind="star", seed=3)
+    want, off = b.want(window=40)
+    bound = rounded(b, want, off)
+    for r in (b.where[0][prefix + 3], b.where[0][2], b.where[1][66 + 2]):                # node 3, a far row, node 2 of the other
+        b.k[int(r)], b.v[int(r)] = value, value
+    got = b.run(window=40).double().cpu().numpy()
+    keep = [i for i in range(10) if i not in (3, 6 + 2)]
+    assert (np.abs(got[keep] - want[keep]) <= bound[keep]).all()
+    ops.status()
+
+
+@pytest.mark.parametrize("q, cache", TYPES)
+@pytest.mark.parametrize("dim", [64, 128])
+@pytest.mark.parametrize("prefix", [40, 1000])
+def test_attention_without_a_key_of_minus_infinity_keeps_its_bound(torch, ops, q, cache, dim, prefix):
+    """A visible key whose score is -inf weighs nothing: the result is that of the sequence without it."""
+    b = Batch(torch, ops, [2], [prefix], dim=dim, q=q, cache=cache)
+    b.q[:] = b.q.abs() + 2.0 ** -10
+    b.k[int(b.where[0][7])] = float("-inf")
+    got = b.run().double().cpu().numpy()
+    ops.status()
+    k, v, x = (t.double().cpu().numpy() for t in (b.k, b.v, b.q))
+    rows = np.delete(b.where[0], 7)
+    shape = (len(rows), b.n_kv, dim)
+    want, off = plain.attention(x.reshape(2, b.heads, dim), k[rows].reshape(shape), v[rows].reshape(shape), b.parents[0], prefix - 1, b.n_kv)
+    want, off = want.reshape(2, -1), off.reshape(2, -1)
+    assert (np.abs(got - want) <= rounded(b, want, off)).all()
+
+
 @pytest.mark.parametrize("q, cache", TYPES)
 @pytest.mark.parametrize("hint", [0, 30000])
 @pytest.mark.parametrize("prefix", [40, 1000])
