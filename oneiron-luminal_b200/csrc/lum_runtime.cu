@@ -2901,7 +2901,7 @@ int32_t lum_draft_verify(lum_rt* rt, int32_t n_seq, const int32_t* slots, const 
         a.picks = d_pick;
     } else a.logits = w.logits;
     CU(rt, launch_tree_accept(a, rt->sm_count, rt->stream));
-    CU(rt, launch_kv_compact(rt->d_planes, 2 * (int)rt->L.size(), tree.m, tree.t, a.path, a.path_len, a.n_accepted, rt->status, rt->sm_count, rt->stream));
+    CU(rt, launch_kv_compact(rt->d_planes, 2 * (int)rt->L.size(), tree.m, tree.t, a.path, a.path_len, a.n_accepted, rt->status, rt->stream));
     rt->n_launches += 2;
     rt->n_tokens_run += R;
     w.tokens.assign(tokens, tokens + R);

@@ -280,7 +280,7 @@ cudaError_t launch_tree_accept(const TreeAcceptArgs& a, int sm_count, cudaStream
     return cudaLaunchKernelEx(&cfg, tree_follow, a, chunks, (const unsigned long long*)keys);
 }
 cudaError_t launch_kv_compact(const KvPlane* planes, int n_planes, const TreeMap& m, const TreeBatch& t, const int* path, int path_len, const int* n_accepted, uint32_t* status,
-                              int, cudaStream_t st) {
+                              cudaStream_t st) {
     kv_compact<<<dim3(n_planes, t.n_seq), 128, 0, st>>>(planes, m, t, path, path_len, n_accepted, status);
     return cudaGetLastError();
 }
@@ -496,7 +496,7 @@ int32_t lum_op_kv_compact(const lum_kv_plane* planes, int32_t n_planes, const lu
     if (m.table) NEED(on_device(op, "page_table", m.table, d.id));
     uint32_t* status = lum_tree_status_word();
     if (!status) return refuse(op, "no status word", LUM_E_CUDA);
-    const cudaError_t e = launch_kv_compact((const KvPlane*)planes, n_planes, m, t, path, path_len, n_accepted, status, d.sms, (cudaStream_t)stream);
+    const cudaError_t e = launch_kv_compact((const KvPlane*)planes, n_planes, m, t, path, path_len, n_accepted, status, (cudaStream_t)stream);
     return e == cudaSuccess ? 0 : cuda_failed(op, e);
 }
 

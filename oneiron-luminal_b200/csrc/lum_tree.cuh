@@ -82,7 +82,7 @@ cudaError_t launch_tree_attn(const TreeAttnArgs& a, int sm_count, cudaStream_t s
 size_t tree_accept_workspace(const TreeBatch& t, int vocab, int sm_count);
 cudaError_t launch_tree_accept(const TreeAcceptArgs& a, int sm_count, cudaStream_t st);
 cudaError_t launch_kv_compact(const KvPlane* planes, int n_planes, const TreeMap& m, const TreeBatch& t, const int* path, int path_len, const int* n_accepted, uint32_t* status,
-                              int sm_count, cudaStream_t st);
+                              cudaStream_t st);
 cudaError_t launch_kv_copy(const KvPlane* planes, int n_planes, long long rows, const int* spans, int n_spans, int max_rows, uint32_t* status, int sm_count, cudaStream_t st);
 
 }  // namespace lum

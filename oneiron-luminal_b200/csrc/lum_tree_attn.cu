@@ -1122,7 +1122,6 @@ cudaError_t combine(const TreeAttnArgs& a, const Share& p, cudaStream_t st) {
     return cudaLaunchKernelEx(&cfg, tree_combine<HD, TQ>, a, p);
 }
 
-// A cache as a tensor [dimension groups of 64][row][64]: one copy brings both halves of a head of 128.
 using EncodeTiled = CUresult (*)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*, const cuuint64_t*, const cuuint32_t*, const cuuint32_t*, CUtensorMapInterleave,
                                  CUtensorMapSwizzle, CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
 cudaError_t encode_bf16(CUtensorMap* map, const void* p, int rank, const cuuint64_t* dims, const cuuint64_t* strides, const cuuint32_t* box) {
@@ -1197,7 +1196,7 @@ cudaError_t tc_launch(const TreeAttnArgs& a, const Share& p, cudaStream_t st) {
 bool tree_attn_supported(const TreeAttnArgs& a) {
     if (a.kv_bf16 && a.n_q / a.n_kv > 128) return false;
     const Bounds b = bounds_of(a, a.kv_bf16 ? 128 / copies_of(a) / (a.n_q / a.n_kv) * (a.n_q / a.n_kv) : kRowsTile);
-    // tiles are counted in 32 bits, and tree_combine has a CTA for eight (row, head)
+    // tiles are counted in 32 bits, and so are tree_combine's items of eight (row, head)
     return b.units < 0x40000000ll && b.units * b.tiles < 0x7fffffffll && (long long)a.t.n_rows * ((a.n_q + 7) / 8) < 0x7fffffffll;
 }
 size_t tree_attn_workspace(const TreeAttnArgs& a, int sm_count) { return share_bytes(a, share_of(a, sm_count)); }
