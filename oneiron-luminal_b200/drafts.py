@@ -134,11 +134,11 @@ def _rows_of(name, t, device, width, rows):
     return t.data_ptr(), (t.stride(0) if rows > 1 else width)
 
 
-def _no_gradient(*tensors):
+def _no_gradient(q, k, v, sinks):
     """There is no backward pass: a result that looks like a constant where a gradient is being recorded is refused."""
     if torch is None:
         _use_torch()
-    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors):
+    if torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or v.requires_grad or (sinks is not None and sinks.requires_grad)):
         _bad("attn_tree has no gradient: call it under torch.no_grad(), or with tensors that require none")
 
 
