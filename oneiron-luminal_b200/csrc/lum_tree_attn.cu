@@ -252,7 +252,8 @@ __device__ __forceinline__ F2 add2(F2 a, F2 b) { F2 r; asm("add.rn.f32x2 %0, %1,
 // ---- products on CUDA cores, in 32 bits: an f32 cache
 // A unit has 32 query rows; 8 warps of 4 query rows.  A tile of 64 keys lies in shared memory as f32: a lane multiplies two keys with the warp's four rows, and then four
 // (two) dimensions of the values with their weights.  Bound by what is read from shared memory: every warp reads all keys and values.  8 trees of 8 nodes over 4000 rows, 8 K/V
-// heads of 4 query heads of 128 (8.4 GFLOP): 208 us, 40 TFLOP/s; with one key a lane and no pairs 291.
+// heads of 4 query heads of 128 (8.4 GFLOP): 208 us, 40 TFLOP/s; with one key a lane and no pairs 291.  4 trees of 47 over 7030 rows, 2 K/V heads of 7 query heads (9.5 GFLOP): 442 us, 21
+// TFLOP/s.  Shared memory's data pipe is 63 to 70 % busy, issue 40 %.
 constexpr int kRowsTile = 32, kRowsKeys = kTileKeys;
 template <int HD>
 constexpr int rows_smem() { return (kRowsTile * HD + kRowsKeys * (HD + 4) + kRowsKeys * HD + 2 * kRowsTile * kRowsKeys) * 4 + (int)sizeof(Piece) + (int)sizeof(TreeNodes); }
@@ -450,10 +451,12 @@ __global__ void __launch_bounds__(256, 2) attn_tree_rows(const TreeAttnArgs a, c
 //     thousands of keys the cuts add up.  Low terms go first.
 // A key that a row does not see has weight 0, but 0 times infinity is no zero: rows of V behind the last node or before the window are zeroed, and a row whose
 // result is not finite is computed again by tree_row_plain, key by key.
-// What bounds it, and what it measured (in a graph, SM clock 1.9 GHz): 16 trees of 32 nodes over up to 32768 rows in pages of 16, 8 K/V heads of 4 query heads of 128 (1.28 GB):
-// 268 us, 4.8 TB/s; with more products per byte than HBM alone would let them wait for, it slows down with the SMs' clock (328 us at the 1.4 GHz that a second of such calls is
-// held to).  8 trees of 64 over 4096 rows, 8 query heads of 64 per K/V head (34.6 GFLOP): 82 us, 420 TFLOP/s; bound by the softmax warps (ALU and exponentials busy half of the
-// time each, issue 46 %).  32 trees of up to 16 over up to 2048 rows (0.18 GB): 49 us, 3.7 TB/s, of which launch, first tiles and joining are 15.  Tried without gain: two
+// What bounds it, and what it measured (20 passes in a graph over the same data, SM clock 1.9 GHz): 16 trees of 32 nodes over up to 32768 rows in pages of 16, 8 K/V heads of 4 query
+// heads of 128 (1.28 GB): 268 us, 4.8 TB/s; with more products per byte than HBM alone would let them wait for, it slows down with the SMs' clock: 327 us, 3.9 TB/s, in calls that
+// go on for a second, which are held to 1.1 - 1.4 GHz.  8 trees of 64 over 4096 rows, 8 query heads of 64 per K/V head (34.6 GFLOP): 82 us, 420 TFLOP/s; bound by the softmax warps (ALU and exponentials busy half of the
+// time each, issue 46 %).  32 trees of up to 16 over up to 2048 rows (0.18 GB): 50 us, 3.6 TB/s (56 where nothing is in L2), of which launch, first tiles and joining are 15.
+// f32 queries, whose terms leave room for one CTA an SM with heads of 128 and whose outputs pass through registers every tile: 8 trees of 64 over 4096 rows, 4 query heads of 128 per
+// K/V head 108 us where bf16 queries take 63 (tensor pipe 43 %, issue 35 %), 32 of up to 16 over up to 2048 88 / 50, 16 of 32 over up to 32768 581 / 268.  Tried without gain: two
 // threads per query row (104 us to 107 where this came to 104), weights by the maximum of the tile before with a second try where it grew (112), room for four tiles
 // (n_seq 1 .. 8 with 4000 .. 16000 rows: 13.9 / 14.1, 27.8 / 29.7, 36.4 / 32.2, 25.1 / 37.0: with that much shared memory clusters no longer fit beside one another).
 constexpr int kTcGroup = 128 * 16 + 16;              // f32 queries' terms: 16-byte column groups of 128 rows, the next one 16 bytes further on (banks)
@@ -1055,7 +1058,8 @@ __global__ void __launch_bounds__(256, kJoinCtas) tree_combine(const TreeAttnArg
     }
 }
 
-// Copies of the query rows in a tile of 128 (see attn_tree_tc): as many as there is room for.  Measured with / without, us: 32 trees of 16 nodes of 4 query heads (2 copies) 53 / 65
+// Copies of the query rows in a tile of 128 (see attn_tree_tc): as many as there is room for, since the lengths, which tell who waits for HBM, are on the device.  Two of the pairs
+// below lose 5 % by it, the others gain 9 to 18.  Measured with / without, us: 32 trees of 16 nodes of 4 query heads (2 copies) 53 / 65
 // when they came in, 10 trees of 8 over 850 rows (4) 20.3 / 22.2, 16 of 16 over 16000 (2) 212 / 241, 16 of 8 over 16000 (4; bound by HBM) 185 / 177, one of 8 over 500 10.0 / 9.5.
 int copies_of(const TreeAttnArgs& a) {
     const int rows = a.t.max_rows * (a.n_q / a.n_kv);
@@ -1069,7 +1073,7 @@ Bounds bounds_of(const TreeAttnArgs& a, int tile_rows) {
     if (a.window > 0) tiles = std::min(tiles, ((long long)a.window + a.t.max_rows) / kTileKeys + 2);
     return {(long long)a.t.n_seq * a.n_kv * ((a.t.max_rows * G + tile_rows - 1) / tile_rows), tiles};
 }
-// Few units of not too many tiles: a cluster for each, whose CTAs share its tiles evenly and join their shares through distributed shared memory.  One launch, no scratch, and
+// Few units of not too many tiles (as the call's bounds have it: a graph captured with large ones keeps to pieces): a cluster for each, whose CTAs share its tiles evenly and join their shares through distributed shared memory.  One launch, no scratch, and
 // no search for pieces.  Measured against pieces and tree_combine (or, below 9 tiles, whole units), us in a graph, 8 K/V heads of 4 query heads of 128 in bf16, trees of 8:
 // 1 x 4 tiles 10.1 / 10.6 (of 32 nodes 13.7 / 12.6: more rows to join), 1 x 8 9.9 / 13.0, 1 x 63 13.7 / 17.5, 4 x 63 19.9 / 24.6, 1 x 251 27.6 / 34.7, 2 x 251 41.9 / 40.7, 1 x 501
 // 55.0 / 45.1 (8 CTAs a unit are too few).  From an f32 cache, whose tiles take CUDA cores 7 us, only one tile a CTA: 1 x 4 17.8 / 18.9, 1 x 8 19.1 / 20.5,
